@@ -30,17 +30,17 @@ def listed():
         # the states of the support vectors of a 12-qubit model, read back by their row numbers
         dict(name="read 12 qubits", op="read", rows=20001, of=40000, dim=4096, single=True),
         # the bundled cross-validation set through a 4-qubit circuit: 100 rows, what a search evaluates all day
-        dict(name="gram 4 qubits", op="gram", rows=100, cols=0, dim=16),
-        # 8 qubits, 4096 rows, train x train
-        dict(name="gram 8 qubits", op="gram", rows=4096, cols=0, dim=256),
-        # 16 qubits, train x train: the matrix product at its longest
-        dict(name="gram 16 qubits", op="gram", rows=12000, cols=0, dim=65536),
+        dict(name="gram 4 qubits", op="gram", rows=100, cols=0, dim=16, half=False),
+        # 8 qubits, 4096 rows, train x train, K in half precision: what it writes is most of its traffic
+        dict(name="gram 8 qubits", op="gram", rows=4096, cols=0, dim=256, half=True),
+        # 16 qubits, train x train, K in half precision: the matrix product at its longest
+        dict(name="gram 16 qubits", op="gram", rows=12000, cols=0, dim=65536, half=True),
         # one new sample against 65536 cached ones of 12 qubits: the kernel row of a served prediction
-        dict(name="gram one row", op="gram", rows=1, cols=65536, dim=4096),
+        dict(name="gram one row", op="gram", rows=1, cols=65536, dim=4096, half=False),
         # one generation of a search at the bundled data's size: 50 genomes of 4 to 10 qubits over 100 rows
-        dict(name="population", op="group", groups=50, rows_lo=100, rows_hi=100, dim_lo=16, dim_hi=1024, sizes=1),
+        dict(name="population", op="group", groups=50, rows_lo=100, rows_hi=100, dim_lo=16, dim_hi=1024, sizes=1, half=False),
         # a population whose genomes bring their own rows: a few large kernels among small ones
-        dict(name="population ragged", op="group", groups=12, rows_lo=33, rows_hi=4097, dim_lo=16, dim_hi=4096, sizes=2),
+        dict(name="population ragged", op="group", groups=12, rows_lo=33, rows_hi=4097, dim_lo=16, dim_hi=4096, sizes=2, half=False),
         # the answer for one sample from 8192 support vectors of 10 qubits: latency
         dict(name="decide one", op="decide", rows=1, cols=8192, dim=1024, outs=1),
         # 16384 test rows against 16384 cached rows of 10 qubits, two classes
@@ -73,7 +73,7 @@ def draw(rng: random.Random):
     if op == "group":
         lo = _log(rng, 1, 300)
         return dict(op=op, groups=rng.randint(2, 60), rows_lo=lo, rows_hi=_log(rng, lo, 2000), dim_lo=4,
-                    dim_hi=1 << rng.randint(3, 11), sizes=rng.randint(0, 1 << 20))
+                    dim_hi=1 << rng.randint(3, 11), sizes=rng.randint(0, 1 << 20), half=rng.random() < 0.4)
     dim = _dim(rng)
     most = 1 << 28                                  # amplitudes of one side, and entries of the kernel matrix
     cols = _log(rng, 1, min(65536, most // dim))
@@ -84,6 +84,8 @@ def draw(rng: random.Random):
     case = dict(op=op, rows=rows, cols=cols, dim=dim)
     if op == "decide":
         case["outs"] = rng.choice([1, 1, 1, 2, 3, 10, 45, 64])
+    else:
+        case["half"] = rng.random() < 0.5
     return case
 
 
@@ -106,15 +108,16 @@ def work(case):
     if op in ("write", "read"):
         plain = case["rows"] * dim * (8 if case["single"] else 16)
         return {"bytes": plain + case["rows"] * (_row_bytes(dim) + (8 if op == "read" else 0)), "flops": 8.0 * case["rows"] * dim}
+    entry = 2 if case.get("half") else 4
     if op == "group":
-        return {"bytes": float(sum(n * _row_bytes(d) + 4 * n * n for n, d in sizes(case))),
+        return {"bytes": float(sum(n * _row_bytes(d) + entry * n * n for n, d in sizes(case))),
                 "flops": float(sum(8 * d * n * (n + 1) // 2 for n, d in sizes(case)))}
     m, n = case["rows"], case["cols"]
     if op == "gram" and n == 0:
-        return {"bytes": float(m * _row_bytes(dim) + 4 * m * m), "flops": 8.0 * dim * m * (m + 1) / 2}
+        return {"bytes": float(m * _row_bytes(dim) + entry * m * m), "flops": 8.0 * dim * m * (m + 1) / 2}
     bytes_ = (m + n) * _row_bytes(dim)
     if op == "gram":
-        return {"bytes": float(bytes_ + 4 * m * n), "flops": 8.0 * dim * m * n}
+        return {"bytes": float(bytes_ + entry * m * n), "flops": 8.0 * dim * m * n}
     c = case["outs"]
     return {"bytes": float(bytes_ + 4 * (n * c + c + m * c)), "flops": 8.0 * dim * m * n + 2.0 * m * n * c}
 
@@ -208,7 +211,7 @@ def _parts(codes, scales, dim):
     return q[:, :, 0].reshape(rows, -1)[:, :dim], q[:, :, 1].reshape(rows, -1)[:, :dim]
 
 
-def _kernel(x, y, dim):
+def _kernel(x, y, dim, dtype=torch.float32):
     """K = gain gain |<x|y>|^2; y is None: the rows with themselves, with a unit diagonal."""
     ar, ai = _parts(x[0], x[1], dim)
     br, bi = (ar, ai) if y is None else _parts(y[0], y[1], dim)
@@ -217,12 +220,13 @@ def _kernel(x, y, dim):
     K = (re.square() + im.square()) * x[2][:, None] * (x if y is None else y)[2][None, :]
     if y is None:
         K.fill_diagonal_(1.0)
-    return K
+    return K.to(dtype)
 
 
 def run(state):
     case = state["case"]
     op, dim = case["op"], case.get("dim", 0)
+    dtype = torch.float16 if case.get("half") else torch.float32          # of K
     if own:
         from quake_amd import device as qdev
         if op == "write":
@@ -234,11 +238,11 @@ def run(state):
             return store.read(state["index"], dtype=torch.complex64 if case["single"] else torch.complex128)
         if op == "group":
             stores = [qdev.States8.from_arrays(*s) for s in state["stores"]]
-            return qdev.gram8_jobs([dict(A=s) for s in stores])
+            return qdev.gram8_jobs([dict(A=s) for s in stores], dtype=dtype)
         x = qdev.States8.from_arrays(*state["x"], dim)
         y = qdev.States8.from_arrays(*state["y"], dim) if state["y"] else None
         if op == "gram":
-            return qdev.gram8(x, y)
+            return qdev.gram8(x, y, dtype=dtype)
         return qdev.decision8(x, y, state["coef"], state["intercept"])
     if op == "write":
         codes, scales, gains = _quantise(state["psi"])
@@ -247,8 +251,8 @@ def run(state):
         re, im = _parts(state["codes"][state["index"]], state["scales"][state["index"]], dim)
         return torch.complex(re, im) if case["single"] else torch.complex(re.double(), im.double())
     if op == "group":
-        return [_kernel((c, s, g), None, d) for c, s, g, d in state["stores"]]
-    K = _kernel(state["x"], state["y"], dim)
+        return [_kernel((c, s, g), None, d, dtype) for c, s, g, d in state["stores"]]
+    K = _kernel(state["x"], state["y"], dim, dtype)
     return K if op == "gram" else K @ state["coef"] + state["intercept"]
 
 
