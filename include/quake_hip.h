@@ -178,6 +178,68 @@ int qk_evaluate_f32(const qk_circuit* c, const double* X, int64_t N,
                     const double* Y, int64_t M, int n_features, double* K_host);
 
 /*
+ * 8-bit state stores (optional precision; no counterpart in the reference, whose states are always complex128).
+ * The states a kernel model keeps -- its training rows -- in e4m3 with one power-of-two scale for each block of 128
+ * amplitudes: 2 bytes per amplitude instead of 16.  A store is three device arrays the caller owns:
+ *   codes   rows x code_row_bytes(D): chunks of 64 amplitudes, 64 real codes then 64 imaginary ones (OCP e4m3), the
+ *           last chunk padded with zero codes; 16-byte aligned
+ *   scales  rows x scale_row_bytes(D): one byte e + 127 per block of 128 amplitudes, padded to whole 4 bytes with 127
+ *   gains   rows float32: ||psi||^2 / ||q||^2, what restores the row's norm (0 for a row without any code)
+ * The stored row is q = code * 2^e; e is the least integer (-127..127) with max|component| * 2^-e <= 448, every component
+ * is rounded once (nearest, ties to even; also from complex128).  A component that is not finite, or beyond FP32's range,
+ * is stored as NaN and makes the row's gain NaN.
+ * A component is off by at most 2^-4 of itself, so q and psi enclose an angle of at most asin(2^-4) (typically 0.026).
+ */
+typedef struct qk_states8 {
+    void* codes;
+    void* scales;
+    float* gains;
+    int64_t rows;
+} qk_states8;
+int qk_states8_layout(int64_t D, int64_t* code_row_bytes, int64_t* scale_row_bytes);
+/* Writes to->rows states (psi: row stride ldpsi amplitudes; complex64 if f32, else complex128) into the rows that *to points
+ * at: append by passing the pointers of the first free row.  D: 1 .. 2^26, any value. */
+int qk_states8_write_dev(const void* psi, int f32, int64_t ldpsi, int64_t D, const qk_states8* to, void* stream);
+/* Reads N rows back as q (no gain applied): row n of psi is row index[n] of the store (index == NULL: row n).  index is a
+ * device array; an index outside 0 .. from->rows - 1 gives a row of NaN. */
+int qk_states8_read_dev(const qk_states8* from, int64_t D, const int64_t* index, int64_t N, void* psi, int f32, int64_t ldpsi,
+                        void* stream);
+
+/*
+ * K[i][j] = gain_i gain_j |sum_b conj(A_i[b]) B_j[b]|^2 over 8-bit stores: the fidelity of the stored states, scaled back
+ * to the norms of the states they stand for (unit norm: K_ii = 1, K is a valid kernel, positive semidefinite).
+ * Jobs as in qk_gram_job, each with its own D: the kernels of a population of circuits of any sizes run together.
+ * K (and KT) are float32, or float16 / float64 by flag.  QK_GRAM_SYMMETRIC: the same store on both sides, only tiles on or
+ * above the diagonal are computed, the mirror is written and the diagonal is exactly 1.
+ * Sums are FP32.  ws: device memory of qk_gram8_workspace bytes (0 for most calls), 16-byte aligned, used until the call's
+ * work is done.  Results do not depend on the launch: no atomics, fixed order of summation.
+ */
+#define QK_GRAM8_F16 2
+#define QK_GRAM8_F64 4
+typedef struct qk_gram8_job {
+    qk_states8 A, B;
+    int64_t D;
+    void* K;
+    void* KT;
+    int64_t ldk, ldkt;
+    int32_t flags;
+    int32_t reserved;
+} qk_gram8_job;
+int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* bytes);
+int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Decision values of a kernel machine, K never written: out[m][c] = sum_j K(x_m, y_j) coef[j][c] + intercept[c]
+ * (SVC.decision_function on a precomputed kernel: coef = dual_coef_.T over the support vectors in y).  coef: y->rows x C
+ * float32, row stride ldc; intercept: C float32 or NULL; out: x->rows x C float32, row stride ldo.  The gradient of a loss by
+ * coef is the same call with the stores exchanged: dcoef = decision(y, x, dout).  An empty y gives the intercept.
+ */
+#define QK_DECISION8_MAX_C 64
+int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, size_t* bytes);
+int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_t D, const float* coef, int64_t ldc, int C,
+                     const float* intercept, float* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream);
+
+/*
  * Replaces: kernel.evaluate(x_vec, y_vec=None) of FidelityStatevectorKernel
  * (reference qsvm/train.py:92,152,154; qsvm_tester.py:684-686; genetic_v3.py:619).
  * Host pointers; Y == NULL gives the symmetric N x N matrix with unit diagonal.

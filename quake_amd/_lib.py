@@ -19,6 +19,9 @@ QK_ERR_NO_DEVICE = -3
 QK_ERR_UNSUPPORTED = -4
 QK_GRAM_SYMMETRIC = 1
 QK_GRAM_MAX_JOBS = 16
+QK_GRAM8_F16 = 2
+QK_GRAM8_F64 = 4
+QK_DECISION8_MAX_C = 64
 
 
 class QkError(RuntimeError):
@@ -39,6 +42,17 @@ class qk_gram_job(C.Structure):
 class qk_batch_opts(C.Structure):
     _fields_ = [("noise_mode", C.c_int32), ("reserved", C.c_int32), ("noise_param", C.c_double),
                 ("seed", C.c_uint64)]
+
+
+class qk_states8(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("gains", C.c_void_p), ("rows", C.c_int64)]
+
+
+class qk_gram8_job(C.Structure):
+    _fields_ = [
+        ("A", qk_states8), ("B", qk_states8), ("D", C.c_int64), ("K", C.c_void_p), ("KT", C.c_void_p),
+        ("ldk", C.c_int64), ("ldkt", C.c_int64), ("flags", C.c_int32), ("reserved", C.c_int32),
+    ]
 
 
 STATS_LEN = 8
@@ -68,6 +82,14 @@ SIGNATURES = {
     "qk_simulate_c64_dev": (C.c_int, [_P, _P, _I64, _I64, _P, _P, _P]),
     "qk_gram32_jobs_dev": (C.c_int, [C.POINTER(qk_gram_job), C.c_int, _I64, _P]),
     "qk_gram32_dev": (C.c_int, [_P, _I64, _P, _I64, _I64, _P, _I64, _P]),
+    "qk_states8_layout": (C.c_int, [_I64, C.POINTER(_I64), C.POINTER(_I64)]),
+    "qk_states8_write_dev": (C.c_int, [_P, C.c_int, _I64, _I64, C.POINTER(qk_states8), _P]),
+    "qk_states8_read_dev": (C.c_int, [C.POINTER(qk_states8), _I64, _P, _I64, _P, C.c_int, _I64, _P]),
+    "qk_gram8_workspace": (C.c_int, [C.POINTER(qk_gram8_job), C.c_int, C.POINTER(C.c_size_t)]),
+    "qk_gram8_jobs_dev": (C.c_int, [C.POINTER(qk_gram8_job), C.c_int, _P, C.c_size_t, _P]),
+    "qk_decision8_workspace": (C.c_int, [_I64, _I64, _I64, C.c_int, C.POINTER(C.c_size_t)]),
+    "qk_decision8_dev": (C.c_int, [C.POINTER(qk_states8), C.POINTER(qk_states8), _I64, _P, _I64, C.c_int, _P, _P, _I64, _P,
+                                   C.c_size_t, _P]),
     "qk_evaluate_f32": (C.c_int, [_P, _P, _I64, _P, _I64, C.c_int, _P]),
     "qk_evaluate": (C.c_int, [_P, _P, _I64, _P, _I64, C.c_int, _P]),
     "qk_rdm1_dev": (C.c_int, [_P, _I64, C.c_int, _P, _P]),

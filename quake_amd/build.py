@@ -11,7 +11,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 INCLUDE = PKG_DIR.parent / "include"
 LIB_PATH = PKG_DIR / "libquake_hip.so"
-SOURCES = ["qk_api.hip", "qk_circuit.cpp", "qk_sim.hip", "qk_wave.hip", "qk_reg.hip", "qk_gram.hip", "qk_pqk.hip", "qk_stats.hip"]
+SOURCES = ["qk_api.hip", "qk_circuit.cpp", "qk_sim.hip", "qk_wave.hip", "qk_reg.hip", "qk_gram.hip", "qk_fp8.hip", "qk_pqk.hip", "qk_stats.hip"]
 
 
 def hipcc() -> str:
@@ -47,7 +47,9 @@ def build_library(force: bool = False, verbose: bool = True, extra_flags=()) -> 
     uniform_flow = keep_in_regs + ["-mllvm", "-structurizecfg-skip-uniform-regions"]
     # (the LDS simulator's stage dispatch gains a few per cent from the same switch: 16 qubits ZZ r = 2 3.10 -> 3.02 ms per 4 GiB;
     # the Gram and projected-kernel files compile to the same code with and without it and are left alone)
-    per_file = {"qk_wave.hip": uniform_flow, "qk_reg.hip": uniform_flow, "qk_sim.hip": ["-mllvm", "-structurizecfg-skip-uniform-regions"]}
+    per_file = {"qk_wave.hip": uniform_flow, "qk_reg.hip": uniform_flow, "qk_sim.hip": ["-mllvm", "-structurizecfg-skip-uniform-regions"],
+                # no packed FP32 arithmetic: the compiler must not form it from pairs of ordinary float operations
+                "qk_fp8.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
     procs = []
     for s in SOURCES:
         obj = objdir / (s.rsplit(".", 1)[0] + ".o")
