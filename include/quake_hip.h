@@ -185,10 +185,10 @@ int qk_evaluate_f32(const qk_circuit* c, const double* X, int64_t N,
  *           last chunk padded with zero codes; 16-byte aligned
  *   scales  rows x scale_row_bytes(D): one byte e + 127 per block of 128 amplitudes, padded to whole 4 bytes with 127
  *   gains   rows float32: ||psi||^2 / ||q||^2, what restores the row's norm (0 for a row without any code)
- * The stored row is q = code * 2^e; e is the least integer (-127..127) with max|component| * 2^-e <= 448, every component
+ * The stored row is q = code * 2^e; e is the least integer >= -100 with max|component| * 2^-e <= 448, every component
  * is rounded once (nearest, ties to even; also from complex128).  A component that is not finite, or beyond FP32's range,
  * is stored as NaN and makes the row's gain NaN.
- * A component is off by at most 2^-4 of itself, so q and psi enclose an angle of at most asin(2^-4) (typically 0.026).
+ * A component is off by at most 2^-4 of itself (down to 2^-6 of the scale, by 2^-10 of the scale below), so q and psi enclose an angle of at most asin(2^-4) (typically 0.026).
  */
 typedef struct qk_states8 {
     void* codes;
@@ -208,7 +208,7 @@ int qk_states8_read_dev(const qk_states8* from, int64_t D, const int64_t* index,
 /*
  * K[i][j] = gain_i gain_j |sum_b conj(A_i[b]) B_j[b]|^2 over 8-bit stores: the fidelity of the stored states, scaled back
  * to the norms of the states they stand for (unit norm: K_ii = 1, K is a valid kernel, positive semidefinite).
- * Jobs as in qk_gram_job, each with its own D: the kernels of a population of circuits of any sizes run together.
+ * Jobs are those of qk_gram_jobs_dev (KT not with QK_GRAM_SYMMETRIC), each with its own D: the kernels of a population of circuits of any sizes run together.
  * K (and KT) are float32, or float16 / float64 by flag.  QK_GRAM_SYMMETRIC: the same store on both sides, only tiles on or
  * above the diagonal are computed, the mirror is written and the diagonal is exactly 1.
  * Sums are FP32.  ws: device memory of qk_gram8_workspace bytes (0 for most calls), 16-byte aligned, used until the call's

@@ -6,6 +6,7 @@ torch's current stream.  Used by ``bench.py`` and :mod:`quake_amd.sharded`.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import List, Optional, Sequence
 
@@ -195,6 +196,239 @@ def pqk(rdm_x: torch.Tensor, rdm_y: Optional[torch.Tensor], gamma: float,
     ldk = out.stride(0) if N > 1 else max(M, 1)
     _lib.check(_lib.load().qk_pqk_dev(_dp(rdm_x.contiguous()), N, _dp(rdm_y.contiguous()) if rdm_y is not None else None,
                                       M, n, float(gamma), _dp(out), ldk, _stream_ptr()))
+    return out
+
+
+# --------------------------------------------------------------------------- #
+# 8-bit state stores
+# --------------------------------------------------------------------------- #
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """Makes the tensor's GPU the current one for a launch (kernels run on the current stream of that GPU)."""
+    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _one_device(*tensors) -> None:
+    _require_gpu(*tensors)
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise ValueError("tensors are on different GPUs")
+
+
+class States8:
+    """Statevectors kept in 8 bits: e4m3 codes, one power-of-two scale for each block of 128 amplitudes, and one float per row
+    that restores the row's norm -- 2 bytes per amplitude instead of complex128's 16.  The training states of a kernel model:
+    written once (``write`` appends), read by every prediction (:func:`gram8`, :func:`decision8`).
+
+    ``codes`` uint8 [capacity, 128 * ceil(dim / 64)], ``scales`` uint8 [capacity, 4 * ceil(dim / 512)] and ``gains`` float32
+    [capacity] are plain tensors (layout and formulas: ``qk_states8`` in quake_hip.h); ``len(store)`` rows are written.  A
+    component is off by at most 2^-4 of itself, the fidelity of two states by up to 0.13 in the worst case and by about
+    0.07 sqrt(K / dim) for states spread over their ``dim`` amplitudes."""
+
+    def __init__(self, capacity: int, dim: int, device=None):
+        code, scale = self._layout(dim)
+        if capacity < 0:
+            raise ValueError("capacity must not be negative")
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError("device entry points need tensors in GPU memory")
+        self._set(torch.empty((capacity, code), dtype=torch.uint8, device=device),
+                  torch.empty((capacity, scale), dtype=torch.uint8, device=device),
+                  torch.empty((capacity,), dtype=torch.float32, device=device), dim, 0)
+
+    @staticmethod
+    def _layout(dim: int):
+        if not 1 <= dim <= 1 << 26:
+            raise ValueError("dim must be in 1..2^26")
+        return 128 * (-(-dim // 64)), 4 * (-(-dim // 512))
+
+    def _set(self, codes, scales, gains, dim, rows):
+        self.codes, self.scales, self.gains, self.dim, self._rows = codes, scales, gains, dim, rows
+
+    @classmethod
+    def from_arrays(cls, codes: torch.Tensor, scales: torch.Tensor, gains: torch.Tensor, dim: int) -> "States8":
+        """A store over arrays that hold written rows already (a saved store, a selection ``codes[rows], scales[rows],
+        gains[rows]`` of another one's); the arrays are used, not copied."""
+        code, scale = cls._layout(dim)
+        _one_device(codes, scales, gains)
+        rows = gains.shape[0] if gains.dim() == 1 else -1
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or gains.dtype != torch.float32 \
+                or codes.shape != (rows, code) or scales.shape != (rows, scale) \
+                or not (codes.is_contiguous() and scales.is_contiguous() and gains.is_contiguous()):
+            raise ValueError("need contiguous codes uint8 [rows, 128 ceil(dim / 64)], scales uint8 [rows, 4 ceil(dim / 512)], "
+                             "gains float32 [rows]")
+        store = cls.__new__(cls)
+        store._set(codes, scales, gains, dim, rows)
+        return store
+
+    def __len__(self) -> int:
+        return self._rows
+
+    @property
+    def capacity(self) -> int:
+        return self.gains.shape[0]
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def rows(self, start: int, stop: int) -> "States8":
+        """The written rows start .. stop - 1 as a store of their own (a view: nothing is copied)."""
+        if not 0 <= start <= stop <= self._rows:
+            raise ValueError(f"rows {start}..{stop} of a store that holds {self._rows}")
+        store = States8.__new__(States8)
+        store._set(self.codes[start:stop], self.scales[start:stop], self.gains[start:stop], self.dim, stop - start)
+        return store
+
+    def clear(self) -> None:
+        """Forgets the written rows; the memory stays."""
+        self._rows = 0
+
+    def _struct(self, start: int = 0, rows: Optional[int] = None) -> "_lib.qk_states8":
+        rows = self._rows if rows is None else rows
+        return _lib.qk_states8(self.codes.data_ptr() + start * self.codes.shape[1],
+                               self.scales.data_ptr() + start * self.scales.shape[1], self.gains.data_ptr() + 4 * start, rows)
+
+    def write(self, psi: torch.Tensor, at: Optional[int] = None) -> None:
+        """Quantises psi [rows, dim] (complex128 or complex64, unit column stride) behind the rows written so far, or from row
+        ``at`` on (overwriting; ``at`` may be at most the number of rows written so far)."""
+        psi = from_dlpack(psi)
+        _one_device(psi, self.codes)
+        if psi.dtype not in (torch.complex128, torch.complex64) or psi.dim() != 2 or psi.shape[1] != self.dim \
+                or (psi.shape[0] and self.dim > 1 and psi.stride(1) != 1) or psi.is_conj():
+            raise ValueError("psi must be a complex128 / complex64 [rows, dim] tensor with unit column stride")
+        n, at = psi.shape[0], self._rows if at is None else at
+        if not 0 <= at <= self._rows:
+            raise ValueError(f"at = {at}: the store holds {self._rows} rows")
+        if at + n > self.capacity:
+            raise ValueError(f"{n} rows from row {at} on do not fit a capacity of {self.capacity}")
+        ld = psi.stride(0) if n > 1 else self.dim
+        if ld < self.dim:
+            raise ValueError("the rows of psi overlap")
+        to = self._struct(at, n)
+        with _on(psi):
+            _lib.check(_lib.load().qk_states8_write_dev(_dp(psi), int(psi.dtype == torch.complex64), ld, self.dim, C.byref(to),
+                                                        _stream_ptr()))
+        self._rows = max(self._rows, at + n)
+
+    def read(self, index: Optional[torch.Tensor] = None, dtype=torch.complex64, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The stored states q (code * scale, exact in complex64; the gain is not applied): all written rows, or the rows
+        ``index`` (int64 on the GPU, any order, repeats allowed; a number outside the store gives a row of NaN)."""
+        index, out = from_dlpack(index), from_dlpack(out)
+        _one_device(self.codes, index, out)
+        if index is not None and (index.dtype != torch.int64 or index.dim() != 1 or not index.is_contiguous()):
+            raise ValueError("index must be a contiguous int64 vector")
+        n = self._rows if index is None else index.shape[0]
+        if out is None:
+            if dtype not in (torch.complex64, torch.complex128):
+                raise ValueError("dtype must be complex64 or complex128")
+            out = torch.empty((n, self.dim), dtype=dtype, device=self.device)
+        elif out.dtype not in (torch.complex64, torch.complex128) or out.shape != (n, self.dim) or not out.is_contiguous():
+            raise ValueError("out must be a contiguous complex64 / complex128 [rows, dim] tensor")
+        of = self._struct()
+        with _on(out):
+            _lib.check(_lib.load().qk_states8_read_dev(C.byref(of), self.dim, _dp(index), n, _dp(out),
+                                                       int(out.dtype == torch.complex64), self.dim, _stream_ptr()))
+        return out
+
+
+_K8_FLAGS = {torch.float32: 0, torch.float16: _lib.QK_GRAM8_F16, torch.float64: _lib.QK_GRAM8_F64}
+
+
+def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
+    """Fidelity kernels of several pairs of 8-bit stores in one call (one launch for up to 24 of them), every job with its
+    own rows and its own dim: the kernels of a population.  Each job: dict(A=, B=None, K=None, KT=None) with A, B
+    :class:`States8`; B is None: the symmetric kernel of A with an exact unit diagonal.  K (allocated as ``dtype`` if not
+    given) and KT, the transposed copy (not for symmetric jobs): float32, float16 or float64 [len(A), len(B)] views with unit
+    column stride.  Returns the Ks."""
+    if not jobs:
+        return []
+    device = jobs[0]["A"].device
+    arr = (_lib.qk_gram8_job * len(jobs))()
+    Ks = []
+    for a, j in zip(arr, jobs):
+        A, B, K, KT = j["A"], j.get("B"), from_dlpack(j.get("K")), from_dlpack(j.get("KT"))
+        sym = B is None
+        if sym:
+            B = A
+        if not isinstance(A, States8) or not isinstance(B, States8):
+            raise ValueError("A and B must be States8 stores")
+        if A.dim != B.dim:
+            raise ValueError(f"stores of different dim: {A.dim} and {B.dim}")
+        m, n = len(A), len(B)
+        if K is None:
+            if dtype not in _K8_FLAGS:
+                raise ValueError("K must be float32, float16 or float64")
+            K = torch.empty((m, n), dtype=dtype, device=device)
+        elif K.dtype not in _K8_FLAGS or K.shape != (m, n) or (K.numel() and ((n > 1 and K.stride(1) != 1) or (m > 1 and K.stride(0) < n))):
+            raise ValueError("K must be float32, float16 or float64 [len(A), len(B)] with unit column stride")
+        if KT is not None and (sym or KT.dtype != K.dtype or KT.shape != (n, m)
+                               or (KT.numel() and ((m > 1 and KT.stride(1) != 1) or (n > 1 and KT.stride(0) < m)))):
+            raise ValueError("KT must be of K's type, [len(B), len(A)] with unit column stride, and not for a symmetric job")
+        _require_gpu(K, KT)
+        if not A.device == B.device == K.device == device or (KT is not None and KT.device != device):
+            raise ValueError("tensors are on different GPUs")
+        a.A, a.B, a.D = A._struct(), B._struct(), A.dim
+        a.K, a.ldk = K.data_ptr(), (K.stride(0) if m > 1 and n else max(n, 1))
+        if KT is not None:
+            a.KT, a.ldkt = KT.data_ptr(), (KT.stride(0) if n > 1 and m else max(m, 1))
+        a.flags = _K8_FLAGS[K.dtype] | (_lib.QK_GRAM_SYMMETRIC if sym else 0)
+        Ks.append(K)
+    lib = _lib.load()
+    need = C.c_size_t()
+    _lib.check(lib.qk_gram8_workspace(arr, len(jobs), C.byref(need)))
+    with _on(jobs[0]["A"].codes):
+        ws = _workspace(need.value, device)
+        _lib.check(lib.qk_gram8_jobs_dev(arr, len(jobs), _dp(ws), need.value, _stream_ptr()))
+    return Ks
+
+
+def gram8(x: States8, y: Optional[States8] = None, out: Optional[torch.Tensor] = None, dtype=torch.float32) -> torch.Tensor:
+    """K = gain gain |<x|y>|^2 of two 8-bit stores; ``y is None`` -> the symmetric kernel of x with an exact unit diagonal.
+    ``dtype`` (or the type of ``out``): float32, float16 or float64.  From one row (a kernel row for one sample) up."""
+    return gram8_jobs([dict(A=x, B=y, K=out)], dtype)[0]
+
+
+def decision8(x: States8, y: States8, coef: torch.Tensor, intercept: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What a kernel machine answers, out[m, c] = sum_j K(x_m, y_j) coef[j, c] + intercept[c], float32 [len(x), C], without K
+    in memory: ``SVC.decision_function`` on a precomputed kernel (``coef = dual_coef_.T``, y the support vectors), kernel
+    ridge predictions, or K times a vector inside an iterative solver.  coef: float32 [len(y), C] (or [len(y)] for C = 1) with
+    unit column stride, C up to 64.  The gradient of a loss by coef is ``decision8(y, x, dloss/dout)``, the one by the
+    intercept the sum over dloss/dout's rows."""
+    coef, intercept, out = from_dlpack(coef), from_dlpack(intercept), from_dlpack(out)
+    if not isinstance(x, States8) or not isinstance(y, States8):
+        raise ValueError("x and y must be States8 stores")
+    _one_device(x.codes, y.codes, coef, intercept, out)
+    if x.dim != y.dim:
+        raise ValueError(f"stores of different dim: {x.dim} and {y.dim}")
+    if coef.dim() == 1:
+        coef = coef.unsqueeze(1)
+    m, n, c = len(x), len(y), coef.shape[1] if coef.dim() == 2 else 0
+    if coef.dtype != torch.float32 or coef.shape != (n, c) or not 1 <= c <= _lib.QK_DECISION8_MAX_C or (n and c > 1 and coef.stride(1) != 1):
+        raise ValueError("coef must be float32 [len(y), C] with unit column stride and 1 <= C <= 64")
+    if intercept is not None and (intercept.dtype != torch.float32 or intercept.shape != (c,) or not intercept.is_contiguous()):
+        raise ValueError("intercept must be a contiguous float32 vector of C entries")
+    if out is None:
+        out = torch.empty((m, c), dtype=torch.float32, device=x.device)
+    elif out.dtype != torch.float32 or out.shape != (m, c) or (m and c > 1 and out.stride(1) != 1):
+        raise ValueError("out must be float32 [len(x), C] with unit column stride")
+    ldc, ldo = (coef.stride(0) if n > 1 else c), (out.stride(0) if m > 1 else c)
+    if ldc < c or ldo < c:
+        raise ValueError("the rows of coef or out overlap")
+    lib = _lib.load()
+    need = C.c_size_t()
+    _lib.check(lib.qk_decision8_workspace(m, n, x.dim, c, C.byref(need)))
+    sx, sy = x._struct(), y._struct()
+    with _on(x.codes):
+        ws = _workspace(need.value, x.device)
+        _lib.check(lib.qk_decision8_dev(C.byref(sx), C.byref(sy), x.dim, _dp(coef), ldc, c, _dp(intercept), _dp(out), ldo, _dp(ws),
+                                        need.value, _stream_ptr()))
     return out
 
 
