@@ -17,7 +17,9 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
+#include <vector>
 
 #include "qk_common.h"
 
@@ -188,7 +190,7 @@ struct Gram8JobDev {
     int32_t flags;
     int32_t chunks;            // chunks per row
     int32_t sb;                // scale bytes per row
-    int32_t tiles_n;           // tile columns
+    int32_t tiles_m, tiles_n;  // tile rows and columns
     int32_t slices;            // the row's chunks are cut into this many slices of `per` chunks
     int32_t per;
     uint32_t live;             // tiles that have to be computed
@@ -245,21 +247,34 @@ __device__ __forceinline__ void emit(const Gram8JobDev& J, int64_t row, int64_t 
     if (J.KT) store_k(J.KT, col * J.ldkt + row, k, J.flags);
 }
 
-// Tile t of a job: row-major over the tiles that have to be computed (symmetric: those on or above the diagonal).
+// Tile t of a job: the tiles that have to be computed, strip by strip (8 tile rows), column by column inside a strip, so
+// that neighbours in the list share rows of both operands in an XCD's L2.  Symmetric: those on or above the diagonal; a
+// full strip then starts with a triangle of 36.
 __device__ __forceinline__ void gram8_tile(const Gram8JobDev& J, uint32_t t, uint32_t& ti, uint32_t& tj) {
-    const uint32_t T = (uint32_t)J.tiles_n;
+    const uint32_t TM = (uint32_t)J.tiles_m, TN = (uint32_t)J.tiles_n;
     if (!(J.flags & QK_GRAM_SYMMETRIC)) {
-        ti = t / T;
-        tj = t - ti * T;
+        const uint32_t strip = t / (8u * TN), in = t - strip * 8u * TN, rows = min(8u, TM - 8u * strip);
+        tj = in / rows;
+        ti = 8u * strip + (in - tj * rows);
         return;
     }
-    uint32_t lo = 0, hi = T - 1;             // the last row whose first tile is at or before t
+    uint32_t lo = 0, hi = (TM + 7u) / 8u - 1u;             // the last strip that starts at or before t
     while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) / 2;
-        if ((uint64_t)mid * T - (uint64_t)mid * (mid - 1) / 2 <= t) lo = mid; else hi = mid - 1;
+        const uint32_t mid = (lo + hi + 1u) / 2u;
+        if (mid * (36u + 8u * (TM - 4u * mid - 4u)) <= t) lo = mid; else hi = mid - 1u;
     }
-    ti = lo;
-    tj = lo + (t - (uint32_t)((uint64_t)lo * T - (uint64_t)lo * (lo - 1) / 2));
+    uint32_t in = t - lo * (36u + 8u * (TM - 4u * lo - 4u));
+    const uint32_t r0 = 8u * lo, rows = min(8u, TM - r0), tri = rows * (rows + 1u) / 2u;
+    if (in < tri) {
+        uint32_t c = 0;
+        while (in > c) in -= ++c;                          // column c of the triangle has c + 1 tiles
+        tj = r0 + c;
+        ti = r0 + in;
+        return;
+    }
+    in -= tri;
+    tj = r0 + rows + in / rows;
+    ti = r0 + in % rows;
 }
 
 __device__ __forceinline__ int gram8_job(const Gram8Args& a, uint32_t item) {
@@ -340,9 +355,259 @@ __global__ __launch_bounds__(256) void gram8_wave_kernel(Gram8Args args) {
     }
 }
 
-// Adds the slices of every tile in order and finishes its entries: one thread per entry, four workgroups per tile.
+// ---- 128 x 128 tiles ---------------------------------------------------------------------------------------------------
+// Four waves of 64 x 64 (2 x 2 matrix tiles, real and imaginary part: 128 accumulator registers), two workgroups per CU.
+// A step is one chunk of 128 + 128 rows, 32 KiB, copied straight to LDS one step ahead of its use (two buffers).  Row r of a
+// buffer holds its 16-byte piece p at p ^ ((r >> 1) & 7): the 16 rows that a quarter of a wave reads at once then lie in
+// different banks.
+constexpr int kTile = 128;
+constexpr int kStage = 2 * kTile * kChunkBytes;
+constexpr int kScales = 2 * kStage;                         // behind the two buffers: a dword of scales (8 chunks) per row, twice
+constexpr int kTileLds = kScales + 2 * 2 * kTile * 4;
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef const __attribute__((address_space(1))) void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+// NATIVE: products of the 8-bit codes on the matrix unit; else of their bf16 values.
+template <bool NATIVE>
+__device__ __forceinline__ void tile_product(uint8_t* lds, const Rows8& A, int64_t row_a, const Rows8& B, int64_t row_b, int chunks, int sb,
+                                             int c0, int c1, v16f (&re)[2][2], v16f (&im)[2][2]) {
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, h = lane >> 5;
+    const int64_t cb = (int64_t)chunks * kChunkBytes;
+    // copies: waves 0 and 1 bring A, 2 and 3 bring B, eight pieces of 8 rows each
+    const uint8_t* src = wave < 2 ? A.codes + row_a * cb : B.codes + row_b * cb;
+    const int last = (int)min((int64_t)kTile, (wave < 2 ? A.n - row_a : B.n - row_b)) - 1;
+    uint32_t vo[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int row = (wave & 1) * 64 + e * 8 + (lane >> 3);
+        vo[e] = (uint32_t)min(row, last) * (uint32_t)cb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+    const uint8_t* scale_src = wave < 2 ? A.scales + row_a * sb : B.scales + row_b * sb;
+    const uint32_t scale_vo = (uint32_t)min((wave & 1) * 64 + lane, last) * (uint32_t)sb;
+    auto stage = [&](int c, int buf) {
+        if (!(c & 7))
+            __builtin_amdgcn_global_load_lds((gptr_t)(scale_src + (c >> 3) * 4 + (uint64_t)scale_vo),
+                                             (lptr_t)(lds + kScales + (c >> 3 & 1) * 1024 + wave * 256), 4, 0, 0);
+        const uint8_t* at = src + (int64_t)c * kChunkBytes;
+        uint8_t* to = lds + buf * kStage + wave * 8192;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            __builtin_amdgcn_global_load_lds((gptr_t)(at + (uint64_t)vo[e]), (lptr_t)(to + e * 1024), 16, 0, 0);
+    };
+    // fragments: this lane's row of a 32-row tile, pieces 2 h and 2 h + 1 of either part (which codes of a chunk meet in one
+    // instruction is free as long as both operands agree)
+    const int fa = ((wave >> 1) * 64 + r) * kChunkBytes, fb = kTile * kChunkBytes + ((wave & 1) * 64 + r) * kChunkBytes;
+    const int key = (r >> 1) & 7;
+    int piece[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) piece[p] = (((p >> 1) * 4 + 2 * h + (p & 1)) ^ key) << 4;
+    auto compute = [&](int c, int buf) {
+        const uint8_t* base = lds + buf * kStage;
+        const int shift = (c >> 1 & 3) * 8;
+        uint32_t sa[2], sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint8_t* scale = lds + kScales + (c >> 3 & 1) * 1024 + r * 4 + t * 128;
+            sa[t] = *(const uint32_t*)(scale + (wave >> 1) * 256);
+            sc[t] = *(const uint32_t*)(scale + 512 + (wave & 1) * 256);
+        }
+        if constexpr (NATIVE) {
+            union F { v4u q[2]; v8i v; };
+            F ar[2], ai[2], br[2], bi[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    ar[t].q[s] = *(const v4u*)(base + fa + t * 4096 + piece[s]);
+                    ai[t].q[s] = *(const v4u*)(base + fa + t * 4096 + piece[2 + s]);
+                    br[t].q[s] = *(const v4u*)(base + fb + t * 4096 + piece[s]);
+                    bi[t].q[s] = *(const v4u*)(base + fb + t * 4096 + piece[2 + s]);
+                }
+            const int ea[2] = {(int)(sa[0] >> shift), (int)(sa[1] >> shift)}, eb[2] = {(int)(sc[0] >> shift), (int)(sc[1] >> shift)};
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    re[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ar[i].v, br[j].v, re[i][j], 0, 0, 0, ea[i], 0, eb[j]);
+                    im[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ar[i].v, bi[j].v, im[i][j], 0, 0, 0, ea[i], 0, eb[j]);
+                }
+            F na[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) na[i].q[s] = ai[i].q[s] ^ 0x80808080u;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    re[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ai[i].v, bi[j].v, re[i][j], 0, 0, 0, ea[i], 0, eb[j]);
+                    im[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(na[i].v, br[j].v, im[i][j], 0, 0, 0, ea[i], 0, eb[j]);
+                }
+        } else {
+            const float ea[2] = {scale_value((sa[0] >> shift) & 255u), scale_value((sa[1] >> shift) & 255u)};
+            const float eb[2] = {scale_value((sc[0] >> shift) & 255u), scale_value((sc[1] >> shift) & 255u)};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                v4u ar[2], ai[2], br[2], bi[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    ar[t] = *(const v4u*)(base + fa + t * 4096 + piece[s]);
+                    ai[t] = *(const v4u*)(base + fa + t * 4096 + piece[2 + s]);
+                    br[t] = *(const v4u*)(base + fb + t * 4096 + piece[s]);
+                    bi[t] = *(const v4u*)(base + fb + t * 4096 + piece[2 + s]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; q += 2) {
+                    v8b xr[2], xi[2], xn[2], yr[2], yi[2];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        xr[t] = widen8(ar[t][q], ar[t][q + 1], ea[t]);
+                        xi[t] = widen8(ai[t][q], ai[t][q + 1], ea[t]);
+                        yr[t] = widen8(br[t][q], br[t][q + 1], eb[t]);
+                        yi[t] = widen8(bi[t][q], bi[t][q + 1], eb[t]);
+                        xn[t] = negated(xi[t]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            re[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr[i], yr[j], re[i][j], 0, 0, 0);
+                            im[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr[i], yi[j], im[i][j], 0, 0, 0);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            re[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xi[i], yi[j], re[i][j], 0, 0, 0);
+                            im[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xn[i], yr[j], im[i][j], 0, 0, 0);
+                        }
+                }
+            }
+        }
+    };
+    // the copies of this chunk have landed, and every wave is done with the buffer that is filled next
+    auto meet = [] { asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory"); };
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) re[i][j][k] = im[i][j][k] = 0.f;
+    stage(c0, 0);                                       // c0 is a multiple of 8
+    for (int c = c0; c < c1; c += 2) {
+        meet();
+        if (c + 1 < c1) stage(c + 1, 1);
+        compute(c, 0);
+        if (c + 1 >= c1) break;
+        meet();
+        if (c + 2 < c1) stage(c + 2, 0);
+        compute(c + 1, 1);
+    }
+}
+
+// Position of a workgroup -> item of the launch: groups of 64 consecutive items (what an XCD runs at a time: 8 x 8 tiles of a
+// strip) are dealt to the eight XCDs in turn, the rest of the list evenly.
+__device__ __forceinline__ bool gram8_item(uint32_t total, uint32_t& item) {
+    const uint32_t xcd = blockIdx.x & 7u, seq = blockIdx.x >> 3, full = total >> 9;
+    if ((seq >> 6) < full) {
+        item = ((((seq >> 6) << 3) + xcd) << 6) + (seq & 63u);
+        return true;
+    }
+    const uint32_t rest = total - (full << 9), share = (rest + 7u) >> 3, in = seq - (full << 6);
+    item = (full << 9) + xcd * share + in;
+    return in < share && item < total;
+}
+
+template <typename T> __device__ __forceinline__ T k_as(float k) { return (T)k; }
+
+// T: the type of K
+template <bool NATIVE, typename T>
+__global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
+    extern __shared__ uint8_t lds[];
+    uint32_t item;
+    if (!gram8_item(args.total, item)) return;
+    const Gram8JobDev& J = args.job[gram8_job(args, item)];
+    const uint32_t in = item - J.begin, slice = in / J.live, t = in - slice * J.live;
+    uint32_t ti, tj;
+    gram8_tile(J, t, ti, tj);
+    v16f re[2][2], im[2][2];
+    const int c0 = (int)slice * J.per, c1 = min(J.chunks, c0 + J.per);
+    tile_product<NATIVE>(lds, J.A, (int64_t)ti * kTile, J.B, (int64_t)tj * kTile, J.chunks, J.sb, c0, c1, re, im);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, h = lane >> 5;
+    if (J.slices > 1) {
+        float2* ws = (float2*)(args.ws + J.ws) + (((int64_t)t * J.slices + slice) * 16 + wave * 4) * 1024 + lane;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) ws[(i * 2 + j) * 1024 + k * 64] = make_float2(re[i][j][k], im[i][j][k]);
+        return;
+    }
+    // Every 32 x 32 tile goes through a piece of LDS of its wave, [column][row], rows of 36 floats.  A tile whose entries all
+    // exist stores K from the registers (whole lines: a register holds 32 neighbours of two rows) and the mirror from LDS, 16
+    // bytes a lane; the others are stored entry by entry.
+    const bool sym = J.flags & QK_GRAM_SYMMETRIC;
+    const int64_t row_t = (int64_t)ti * kTile + (wave >> 1) * 64, col_t = (int64_t)tj * kTile + (wave & 1) * 64;
+    T* const M = (T*)(sym ? J.K : J.KT);
+    const int64_t ldm = sym ? J.ldk : J.ldkt;
+    const bool whole = (int64_t)(ti + 1) * kTile <= J.A.n && (int64_t)(tj + 1) * kTile <= J.B.n && !(sym && ti == tj) &&
+                       (((uintptr_t)M | (uint64_t)(ldm * (int64_t)sizeof(T))) & 15) == 0;
+    __syncthreads();                                        // the buffers are free
+    float* const piece = (float*)lds + wave * (32 * 36);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float ga[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) ga[k] = J.A.gains[min(row_t + i * 32 + acc_row(lane, k), J.A.n - 1)];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int64_t row0 = row_t + i * 32, col0 = col_t + j * 32;
+            const float gb = J.B.gains[min(col0 + r, J.B.n - 1)];
+            float k[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) k[q] = (re[i][j][q] * re[i][j][q] + im[i][j][q] * im[i][j][q]) * (ga[q] * gb);
+            if (M || !whole) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(float4*)(piece + r * 36 + 8 * q + 4 * h) = make_float4(k[4 * q], k[4 * q + 1], k[4 * q + 2], k[4 * q + 3]);
+            }
+            __builtin_amdgcn_wave_barrier();                // (a wave's LDS accesses stay in order)
+            if (whole) {
+                T* at = (T*)J.K + (row0 + 4 * h) * J.ldk + col0 + r;
+#pragma unroll
+                for (int q = 0; q < 16; ++q) at[(8 * (q >> 2) + (q & 3)) * J.ldk] = k_as<T>(k[q]);
+                if (M) {
+                    constexpr int E = 16 / sizeof(T), L = 32 / E;       // entries a lane stores, lanes a mirrored row takes
+#pragma unroll
+                    for (int c = lane / L; c < 32; c += 64 / L) {
+                        const float* from = piece + c * 36 + (lane % L) * E;
+                        T v[E] __attribute__((aligned(16)));
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[e] = k_as<T>(from[e]);
+                        *(uint4*)(M + (col0 + c) * ldm + row0 + (lane % L) * E) = *(const uint4*)v;
+                    }
+                }
+            } else {
+                for (int q = 0; q < 16; ++q) {
+                    const int rr = 2 * q + h;
+                    const int64_t row = row0 + rr, col = col0 + r;
+                    if (row >= J.A.n || col >= J.B.n || (sym && row > col)) continue;
+                    const float v = sym && row == col ? 1.f : piece[r * 36 + rr];
+                    ((T*)J.K)[row * J.ldk + col] = k_as<T>(v);
+                    if (M && !(sym && row == col)) M[col * ldm + row] = k_as<T>(v);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+}
+
+// Adds the slices of every tile in order and finishes its entries: one thread per entry.  SUB: matrix tiles per tile (1 or 16).
+template <int SUB>
 __global__ __launch_bounds__(256) void gram8_join_kernel(Gram8Args args) {
-    const uint32_t tile = blockIdx.x >> 2;
+    const uint32_t tile = blockIdx.x / (4 * SUB);
     uint32_t before = 0;
     int j = 0;
     for (; j + 1 < args.n_jobs; ++j) {
@@ -355,15 +620,18 @@ __global__ __launch_bounds__(256) void gram8_join_kernel(Gram8Args args) {
     if (J.slices <= 1 || t >= J.live) return;
     uint32_t ti, tj;
     gram8_tile(J, t, ti, tj);
-    const int e = (blockIdx.x & 3) * 256 + threadIdx.x, lane = e & 63, i = e >> 6;
-    const float2* ws = (const float2*)(args.ws + J.ws) + (int64_t)t * J.slices * 1024 + e;
+    const int in = (int)(blockIdx.x % (4 * SUB)) * 256 + threadIdx.x, sub = in >> 10, e = in & 1023, lane = e & 63, i = e >> 6;
+    const float2* ws = (const float2*)(args.ws + J.ws) + (int64_t)t * J.slices * SUB * 1024 + in;
     float x = 0.f, y = 0.f;
     for (int s = 0; s < J.slices; ++s) {
-        const float2 v = ws[(int64_t)s * 1024];
+        const float2 v = ws[(int64_t)s * SUB * 1024];
         x += v.x;
         y += v.y;
     }
-    emit(J, (int64_t)ti * 32 + acc_row(lane, i), (int64_t)tj * 32 + (lane & 31), x, y);
+    // matrix tile of the wave (sub >> 2), then of its 2 x 2
+    const int64_t row = SUB == 1 ? (int64_t)ti * 32 : (int64_t)ti * kTile + (sub >> 3) * 64 + ((sub >> 1) & 1) * 32;
+    const int64_t col = SUB == 1 ? (int64_t)tj * 32 : (int64_t)tj * kTile + ((sub >> 2) & 1) * 64 + (sub & 1) * 32;
+    emit(J, row + acc_row(lane, i), col + (lane & 31), x, y);
 }
 
 // ---- decision values -----------------------------------------------------------------------------------------------------
@@ -377,61 +645,46 @@ struct Decision8Args {
     int32_t C, chunks, sb, splits, per;      // per: tile columns of one split
 };
 
-// Sum of v[0..15] over the 32 lanes of a half; lane gets the sum of register `row_of(lane)`: halving exchanges, so every
-// step moves half of what is left.
-__device__ __forceinline__ float half_reduce(float* v, int lane) {
-#pragma unroll
-    for (int step = 0; step < 4; ++step) {
-        const int m = 16 >> step, n = 8 >> step;
-        const bool up = lane & m;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < n) {
-                const float send = up ? v[k] : v[k + n], keep = up ? v[k + n] : v[k];
-                v[k] = keep + __shfl_xor(send, m, 64);
-            }
-    }
-    return v[0] + __shfl_xor(v[0], 1, 64);
-}
-__device__ __forceinline__ int half_reduce_register(int lane) { return (lane >> 1) & 15; }
-
-// 32 rows of A against a range of B's rows: each of four waves takes every fourth tile of 32 of them, turns its K tile into
-// C partial sums per row at once and adds them up in LDS.
+// The product is taken the other way round (B's rows times A's), so a lane holds 16 of B's rows for ONE row of A: K times the
+// coefficients is then a sum over the lane's own registers, and only the two halves of the wave have to be added.  32 rows of A
+// per workgroup; each of four waves takes every fourth tile of 32 of B's rows in the workgroup's range.
 __global__ __launch_bounds__(256) void decision8_wave_kernel(Decision8Args a) {
     constexpr int W = 4;
-    extern __shared__ float acc[];            // [W][32][C]
+    extern __shared__ float acc[];            // [W][C][32]
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, h = lane >> 5;
     for (int k = tid; k < W * 32 * a.C; k += 256) acc[k] = 0.f;
     __syncthreads();
     const int64_t row0 = (int64_t)blockIdx.x * 32;
     const int64_t cb = (int64_t)a.chunks * kChunkBytes, ra = min(row0 + r, a.A.n - 1);
-    float ga[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ga[i] = a.A.gains[min(row0 + acc_row(lane, i), a.A.n - 1)];
+    const float ga = a.A.gains[ra];
     const int tiles = (int)((a.B.n + 31) / 32), t1 = min(tiles, ((int)blockIdx.y + 1) * a.per);
     for (int t = (int)blockIdx.y * a.per + wave; t < t1; t += W) {
-        const int64_t col = (int64_t)t * 32 + r, rb = min(col, a.B.n - 1);
+        const int64_t col0 = (int64_t)t * 32, rb = min(col0 + r, a.B.n - 1);
         v16f re, im;
 #pragma unroll
         for (int i = 0; i < 16; ++i) re[i] = im[i] = 0.f;
-        wave_product(a.A.codes + ra * cb + 16 * h, a.A.scales + ra * a.sb, a.B.codes + rb * cb + 16 * h, a.B.scales + rb * a.sb, 0, a.chunks,
+        wave_product(a.B.codes + rb * cb + 16 * h, a.B.scales + rb * a.sb, a.A.codes + ra * cb + 16 * h, a.A.scales + ra * a.sb, 0, a.chunks,
                      1, re, im);
-        const float gb = a.B.gains[rb];
         float k[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) k[i] = (re[i] * re[i] + im[i] * im[i]) * (ga[i] * gb);
+        for (int i = 0; i < 16; ++i) {
+            const int64_t col = col0 + acc_row(lane, i);
+            k[i] = col < a.B.n ? (re[i] * re[i] + im[i] * im[i]) * (ga * a.B.gains[col]) : 0.f;
+        }
         for (int c = 0; c < a.C; ++c) {
-            const float w = col < a.B.n ? a.coef[col * a.ldc + c] : 0.f;
-            float v[16];
+            float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = col < a.B.n ? k[i] * w : 0.f;
-            const float s = half_reduce(v, lane);
-            if (!(lane & 1)) acc[(wave * 32 + acc_row(lane, half_reduce_register(lane))) * a.C + c] += s;
+            for (int i = 0; i < 16; ++i) {
+                const int64_t col = col0 + acc_row(lane, i);
+                if (col < a.B.n) s += k[i] * a.coef[col * a.ldc + c];
+            }
+            s += __shfl_xor(s, 32, 64);
+            if (h == 0) acc[(wave * a.C + c) * 32 + r] += s;
         }
     }
     __syncthreads();
     for (int k = tid; k < 32 * a.C; k += 256) {
-        const int row = k / a.C, c = k - row * a.C;
+        const int row = k & 31, c = k >> 5;
         if (row0 + row >= a.A.n) continue;
         float s = 0.f;
 #pragma unroll
@@ -470,25 +723,41 @@ int check_dim(const char* who, int64_t D) {
 
 Rows8 rows8(const qk_states8& s) { return Rows8{(const uint8_t*)s.codes, (const uint8_t*)s.scales, s.gains, s.rows}; }
 
-// One launch's worth of jobs: tiles, slices, workspace.
+// Which kernel takes a job.  The 128 x 128 kernel reads every row from L2 once for 128 others and needs enough tile steps to
+// fill the chip; the 32 x 32 kernel starts at once, takes few rows without waste and spreads a small job over more
+// workgroups.
+enum Gram8Kind { GK_WAVE, GK_TILE, GK_TILE_F64, GK_TILE_NATIVE, GK_KINDS };
+std::atomic<int> g_path{0};      // development hook: 0 by rule, 1 always 32 x 32, 2 always 128 x 128
+
+int64_t live_tiles(const qk_gram8_job& j, int64_t tile) {
+    const int64_t tm = (j.A.rows + tile - 1) / tile, tn = (j.B.rows + tile - 1) / tile;
+    return (j.flags & QK_GRAM_SYMMETRIC) ? tm * (tm + 1) / 2 : tm * tn;
+}
+
+Gram8Kind kind_of(const qk_gram8_job& j) {
+    const int path = g_path.load(std::memory_order_relaxed);
+    const int64_t chunks = (j.D + kChunk - 1) / kChunk;
+    const bool fits = code_bytes(j.D) <= (int64_t)1 << 24;      // 32-bit offsets inside a tile
+    const bool tile = path == 2 || (path == 0 && std::min(j.A.rows, j.B.rows) >= 64 && live_tiles(j, kTile) * chunks >= 1024);
+    if (!tile || !fits) return GK_WAVE;
+    return j.flags & QK_GRAM8_F16 ? GK_TILE_NATIVE : j.flags & QK_GRAM8_F64 ? GK_TILE_F64 : GK_TILE;
+}
+
+// One launch's worth of jobs of one kind: tiles, slices, workspace.
 struct Gram8Plan {
     Gram8Args args;
     uint32_t join_tiles;
     size_t ws_floats;
 };
 
-int plan_gram8(const qk_gram8_job* jobs, int n, Gram8Plan& p) {
+int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind, Gram8Plan& p) {
     std::memset(&p, 0, sizeof(p));
+    const int64_t side = kind == GK_WAVE ? 32 : kTile;
     int64_t tiles = 0;
-    for (int k = 0; k < n; ++k) {
-        const qk_gram8_job& j = jobs[k];
-        const int64_t tm = (j.A.rows + 31) / 32, tn = (j.B.rows + 31) / 32;
-        tiles += (j.flags & QK_GRAM_SYMMETRIC) ? tm * (tm + 1) / 2 : tm * tn;
-    }
+    for (int k = 0; k < n; ++k) tiles += live_tiles(jobs[which[k]], side);
     int64_t items = 0;
     for (int k = 0; k < n; ++k) {
-        const qk_gram8_job& j = jobs[k];
-        if (!j.A.rows || !j.B.rows) continue;
+        const qk_gram8_job& j = jobs[which[k]];
         Gram8JobDev& d = p.args.job[p.args.n_jobs++];
         d.A = rows8(j.A);
         d.B = rows8(j.B);
@@ -499,12 +768,14 @@ int plan_gram8(const qk_gram8_job* jobs, int n, Gram8Plan& p) {
         d.flags = j.flags;
         d.chunks = (int32_t)((j.D + kChunk - 1) / kChunk);
         d.sb = (int32_t)scale_bytes(j.D);
-        const int64_t tm = (j.A.rows + 31) / 32, tn = (j.B.rows + 31) / 32;
-        d.tiles_n = (int32_t)tn;
-        const int64_t live = (j.flags & QK_GRAM_SYMMETRIC) ? tm * (tm + 1) / 2 : tm * tn;
-        // few tiles with long rows: slices of at least 16 chunks (four for each wave), enough for about 1024 workgroups
-        int64_t slices = std::max<int64_t>(1, std::min<int64_t>(d.chunks / 16, 1024 / std::max<int64_t>(tiles, 1)));
-        d.per = (int32_t)((d.chunks + slices - 1) / slices);
+        d.tiles_m = (int32_t)((j.A.rows + side - 1) / side);
+        d.tiles_n = (int32_t)((j.B.rows + side - 1) / side);
+        const int64_t live = live_tiles(j, side);
+        // few tiles with long rows: slices of at least 16 chunks (four for each wave) or 8, in whole groups of 8 (a dword
+        // of scales), enough for about 1024 or 512 workgroups
+        const int64_t least = kind == GK_WAVE ? 16 : 8, want = kind == GK_WAVE ? 1024 : 512;
+        const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(d.chunks / least, want / std::max<int64_t>(tiles, 1)));
+        d.per = (int32_t)(((d.chunks + slices - 1) / slices + 7) / 8 * 8);
         d.slices = (d.chunks + d.per - 1) / d.per;
         if (items + live * d.slices > 0x7fffffffLL) return fail(QK_ERR_UNSUPPORTED, "qk_gram8_jobs_dev: too many tiles; split the call");
         d.live = (uint32_t)live;
@@ -512,11 +783,27 @@ int plan_gram8(const qk_gram8_job* jobs, int n, Gram8Plan& p) {
         items += live * d.slices;
         if (d.slices > 1) {
             d.ws = (int64_t)p.ws_floats;
-            p.ws_floats += (size_t)live * d.slices * 2048;
+            p.ws_floats += (size_t)live * d.slices * 2 * side * side;
             p.join_tiles += (uint32_t)live;
         }
     }
     p.args.total = (uint32_t)items;
+    return QK_OK;
+}
+
+// The launches of a call, in order: `each(plan, kind)`.  Jobs with long rows go first, so that a launch does not end on them.
+template <typename F> int gram8_launches(const qk_gram8_job* jobs, int n, F each) {
+    std::vector<int> by[GK_KINDS];
+    for (int k = 0; k < n; ++k)
+        if (jobs[k].A.rows && jobs[k].B.rows) by[kind_of(jobs[k])].push_back(k);
+    for (int kind = GK_KINDS - 1; kind >= 0; --kind) {
+        std::stable_sort(by[kind].begin(), by[kind].end(), [&](int a, int b) { return jobs[a].D > jobs[b].D; });
+        for (size_t k = 0; k < by[kind].size(); k += kGram8Jobs) {
+            Gram8Plan p;
+            int rc = plan_gram8(jobs, by[kind].data() + k, (int)std::min<size_t>(kGram8Jobs, by[kind].size() - k), (Gram8Kind)kind, p);
+            if (rc || (rc = each(p, (Gram8Kind)kind))) return rc;
+        }
+    }
     return QK_OK;
 }
 
@@ -621,36 +908,58 @@ extern "C" int qk_states8_read_dev(const qk_states8* from, int64_t D, const int6
 extern "C" int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* bytes) {
     if (!bytes) return fail(QK_ERR_INVALID, "qk_gram8_workspace: null pointer");
     *bytes = 0;
-    int rc = check_gram8(jobs, n_jobs);
+    const int rc = check_gram8(jobs, n_jobs);
     if (rc) return rc;
-    size_t most = 0;
-    for (int k = 0; k < n_jobs; k += kGram8Jobs) {
-        Gram8Plan p;
-        if ((rc = plan_gram8(jobs + k, std::min(kGram8Jobs, n_jobs - k), p))) return rc;
-        most = std::max(most, p.ws_floats * sizeof(float));
-    }
-    *bytes = most;
-    return QK_OK;
+    return gram8_launches(jobs, n_jobs, [&](const Gram8Plan& p, Gram8Kind) {
+        *bytes = std::max(*bytes, p.ws_floats * sizeof(float));      // the launches of a call use it one after the other
+        return QK_OK;
+    });
 }
+
+#define QK_TILE8(NATIVE, T)                                                                                         \
+    do {                                                                                                            \
+        static DeviceOnce attr;                                                                                     \
+        if (attr.pending()) {                                                                                       \
+            QK_HIP(hipFuncSetAttribute((const void*)gram8_tile_kernel<NATIVE, T>, hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds)); \
+            attr.done();                                                                                            \
+        }                                                                                                           \
+        hipLaunchKernelGGL((gram8_tile_kernel<NATIVE, T>), dealt, dim3(256), kTileLds, s, p.args);                  \
+    } while (0)
 
 extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream) {
     int rc = check_gram8(jobs, n_jobs);
     if (rc) return rc;
-    for (int k = 0; k < n_jobs; k += kGram8Jobs) {
-        Gram8Plan p;
-        if ((rc = plan_gram8(jobs + k, std::min(kGram8Jobs, n_jobs - k), p))) return rc;
-        if (p.args.n_jobs == 0) continue;
-        if (p.ws_floats * sizeof(float) > ws_bytes || (p.ws_floats && !ws))
-            return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: workspace smaller than qk_gram8_workspace asks for");
-        if ((uintptr_t)ws & 15) return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: the workspace needs 16-byte alignment");
+    if ((uintptr_t)ws & 15) return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: the workspace needs 16-byte alignment");
+    size_t need = 0;
+    if ((rc = qk_gram8_workspace(jobs, n_jobs, &need))) return rc;
+    if (need > ws_bytes || (need && !ws))
+        return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: workspace smaller than qk_gram8_workspace asks for");
+    const hipStream_t s = (hipStream_t)stream;
+    return gram8_launches(jobs, n_jobs, [&](Gram8Plan& p, Gram8Kind kind) {
         p.args.ws = (float*)ws;
-        hipLaunchKernelGGL(gram8_wave_kernel, dim3(p.args.total), dim3(256), 0, (hipStream_t)stream, p.args);
+        const uint32_t total = p.args.total, full = total >> 9;
+        const dim3 dealt((full << 9) + 8 * ((total - (full << 9) + 7) >> 3));
+        if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, dim3(total), dim3(256), 0, s, p.args);
+        else if (kind == GK_TILE) QK_TILE8(false, float);
+        else if (kind == GK_TILE_F64) QK_TILE8(false, double);
+        else QK_TILE8(true, _Float16);
         QK_HIP(hipGetLastError());
         if (p.join_tiles) {
-            hipLaunchKernelGGL(gram8_join_kernel, dim3(p.join_tiles * 4), dim3(256), 0, (hipStream_t)stream, p.args);
+            if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_join_kernel<1>, dim3(p.join_tiles * 4), dim3(256), 0, s, p.args);
+            else hipLaunchKernelGGL(gram8_join_kernel<16>, dim3(p.join_tiles * 64), dim3(256), 0, s, p.args);
             QK_HIP(hipGetLastError());
         }
-    }
+        return (int)QK_OK;
+    });
+}
+
+// Development hook (not in the public header): which kernel the products of 8-bit stores use, whatever the rule says.
+extern "C" int qk_gram8_set_path(const char* name) {
+    const std::string s = name ? name : "";
+    if (s == "auto") g_path = 0;
+    else if (s == "wave") g_path = 1;
+    else if (s == "tile") g_path = 2;
+    else return fail(QK_ERR_INVALID, "qk_gram8_set_path: auto, wave or tile");
     return QK_OK;
 }
 

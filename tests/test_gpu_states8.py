@@ -1,4 +1,6 @@
 """8-bit state stores on the GPU against tests/_states8.py (float64 numpy)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -8,6 +10,16 @@ from tests import _states8 as S8
 
 pytestmark = pytest.mark.gpu
 NP = {torch.float32: S8.U32, torch.float16: S8.U16, torch.float64: 0.0}
+
+
+@pytest.fixture(params=["auto", "wave", "tile"])
+def path(request):
+    """The kernel that takes the products: by the library's rule, always 32 x 32 tiles, always 128 x 128."""
+    fn = _lib.load().qk_gram8_set_path
+    fn.restype, fn.argtypes = C.c_int, [C.c_char_p]
+    _lib.check(fn(request.param.encode()))
+    yield request.param
+    fn(b"auto")
 
 
 def put(psi, single=False):
@@ -89,7 +101,7 @@ def test_scale_borders_and_tiny_blocks():
     assert (np.abs(g - gains) <= 2 * S8.U32 * gains).all() and g[9] == 0 and (scales[:, 1] == 127).all()
 
 
-def test_values_that_are_not_finite():
+def test_values_that_are_not_finite(path):
     psi = S8.states(np.random.default_rng(4), 6, 300)
     psi[1, 10], psi[2, 200], psi[3, 299], psi[4, 0] = np.nan, np.inf, 1j * -np.inf, 1e39
     store, q, g = fill(psi)
@@ -134,7 +146,7 @@ SHAPES = [(1, 1, 1), (2, 3, 2), (31, 33, 16), (100, 64, 16), (1, 500, 64), (32, 
 
 @pytest.mark.parametrize("dtype", list(NP))
 @pytest.mark.parametrize("M,N,D", SHAPES)
-def test_gram8_cross(M, N, D, dtype):
+def test_gram8_cross(M, N, D, dtype, path):
     rng = np.random.default_rng(M * 7 + N * 13 + D)
     x, a, ga = fill(S8.states(rng, M, D, "product" if D > 1 else "spread"))
     y, b, gb = fill(S8.states(rng, N, D, "product" if M % 2 else "spread"))
@@ -143,14 +155,14 @@ def test_gram8_cross(M, N, D, dtype):
 
 @pytest.mark.parametrize("dtype", list(NP))
 @pytest.mark.parametrize("N,D", [(1, 2), (2, 16), (31, 64), (100, 16), (129, 32), (64, 300), (257, 128), (300, 1024), (513, 256), (40, 65536), (200, 4096)])
-def test_gram8_symmetric(N, D, dtype):
+def test_gram8_symmetric(N, D, dtype, path):
     x, a, ga = fill(S8.states(np.random.default_rng(N + D), N, D, "product"))
     check_k(qdev.gram8(x, dtype=dtype), a, ga, a, ga, symmetric=True)
 
 
 @pytest.mark.parametrize("M,N,D", [(1500, 1100, 512), (1, 5000, 1024), (2, 3000, 4096), (33, 2000, 2048), (700, 700, 16384)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
-def test_gram8_larger(M, N, D, dtype):
+def test_gram8_larger(M, N, D, dtype, path):
     rng = np.random.default_rng(D + M)
     x, a, ga = fill(S8.states(rng, M, D, "product"))
     y, b, gb = fill(S8.states(rng, N, D, "spread"))
@@ -160,7 +172,7 @@ def test_gram8_larger(M, N, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(NP))
-def test_gram8_writes_its_block_only(dtype):
+def test_gram8_writes_its_block_only(dtype, path):
     rng = np.random.default_rng(8)
     x, a, ga = fill(S8.states(rng, 150, 256))
     y, b, gb = fill(S8.states(rng, 141, 256))
@@ -205,7 +217,7 @@ def test_gram8_zero_rows_and_unnormalised_rows():
     assert ga[3] == 0 and abs(ga[7] * np.sum(np.abs(a[7]) ** 2) - 1e-12) < 1e-18      # the gain keeps ||psi||^2
 
 
-def test_population_of_ragged_sizes():
+def test_population_of_ragged_sizes(path):
     rng = np.random.default_rng(12)
     shapes = [(1, 2), (100, 16), (33, 1024), (257, 64), (2, 65536), (500, 200), (64, 32), (31, 8), (129, 4096), (100, 512), (3, 3)] * 3
     held = [fill(S8.states(rng, n, d, "product")) for n, d in shapes]
