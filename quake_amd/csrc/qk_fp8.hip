@@ -694,6 +694,67 @@ __global__ __launch_bounds__(256) void decision8_wave_kernel(Decision8Args a) {
     }
 }
 
+// The same over 128 x 128 tiles: a workgroup keeps 128 rows of A and walks B's tiles of its range; the sums of its C columns
+// wait in LDS behind the tile buffers, [C][128], where the two waves that share rows of A add one after the other.  The
+// coefficients of a tile pass through the buffers, [C][128]: a lane reads four of them at once, the same for its whole half.
+__global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a) {
+    extern __shared__ uint8_t lds[];
+    float* const acc = (float*)(lds + kTileLds);
+    float* const coef = (float*)lds;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, h = lane >> 5;
+    const int xs = (wave & 1) * 64 + r, ys = (wave >> 1) * 64;
+    const int64_t row0 = (int64_t)blockIdx.x * kTile;
+    for (int k = tid; k < kTile * a.C; k += 256) acc[k] = 0.f;
+    float gx[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) gx[j] = a.A.gains[min(row0 + xs + j * 32, a.A.n - 1)];
+    const int tiles = (int)((a.B.n + kTile - 1) / kTile), t1 = min(tiles, ((int)blockIdx.y + 1) * a.per);
+    for (int t = (int)blockIdx.y * a.per; t < t1; ++t) {
+        const int64_t col0 = (int64_t)t * kTile;
+        v16f re[2][2], im[2][2];
+        tile_product<false>(lds, a.B, col0, a.A, row0, a.chunks, a.sb, 0, a.chunks, re, im);
+        __syncthreads();
+        for (int k = tid; k < kTile * a.C; k += 256) {
+            const int row = (int)((unsigned)k / (unsigned)a.C), c = k - row * a.C;
+            coef[c * kTile + row] = col0 + row < a.B.n ? a.coef[(col0 + row) * a.ldc + c] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const float gy = a.B.gains[min(col0 + ys + i * 32 + acc_row(lane, q), a.B.n - 1)];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) re[i][j][q] = (re[i][j][q] * re[i][j][q] + im[i][j][q] * im[i][j][q]) * (gx[j] * gy);
+            }
+        __syncthreads();
+        for (int half = 0; half < 2; ++half) {
+            if ((wave >> 1) == half)
+                for (int c = 0; c < a.C; ++c) {
+                    float s[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float4 w = *(const float4*)(coef + c * kTile + ys + i * 32 + 8 * q + 4 * h);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                s[j] += re[i][j][4 * q] * w.x + re[i][j][4 * q + 1] * w.y + re[i][j][4 * q + 2] * w.z + re[i][j][4 * q + 3] * w.w;
+                        }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) s[j] += __shfl_xor(s[j], 32, 64);
+                    acc[c * kTile + xs + h * 32] += h ? s[1] : s[0];      // lane half h adds the rows of tile j = h
+                }
+            __syncthreads();
+        }
+    }
+    for (int k = tid; k < kTile * a.C; k += 256) {
+        const int c = k >> 7, row = k & (kTile - 1);
+        if (row0 + row >= a.A.n) continue;
+        if (a.splits == 1) a.out[(row0 + row) * a.ldo + c] = acc[k] + (a.intercept ? a.intercept[c] : 0.f);
+        else a.ws[((int64_t)blockIdx.y * a.A.n + row0 + row) * a.C + c] = acc[k];
+    }
+}
+
 __global__ __launch_bounds__(256) void decision8_join_kernel(Decision8Args a) {
     const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (k >= a.A.n * a.C) return;
@@ -828,15 +889,20 @@ int check_gram8(const qk_gram8_job* jobs, int n) {
     return QK_OK;
 }
 
-int plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
+// -> whether the 128 x 128 kernel takes it (gram8's rule)
+bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
     a.C = C;
     a.chunks = (int32_t)((D + kChunk - 1) / kChunk);
     a.sb = (int32_t)scale_bytes(D);
-    const int64_t tm = (M + 31) / 32, tn = (N + 31) / 32;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((tn + 3) / 4, 1024 / std::max<int64_t>(tm, 1)));
+    const int path = g_path.load(std::memory_order_relaxed);
+    const bool tile = code_bytes(D) <= (int64_t)1 << 24 &&
+                      (path == 2 || (path == 0 && std::min(M, N) >= 64 && (M + kTile - 1) / kTile * ((N + kTile - 1) / kTile) * a.chunks >= 1024));
+    const int64_t side = tile ? kTile : 32, tm = (M + side - 1) / side, tn = (N + side - 1) / side;
+    const int64_t want = tile ? std::max<int64_t>(1, std::min<int64_t>(tn, 512 / std::max<int64_t>(tm, 1)))
+                              : std::max<int64_t>(1, std::min<int64_t>((tn + 3) / 4, 1024 / std::max<int64_t>(tm, 1)));
     a.per = (int32_t)std::max<int64_t>(1, (tn + want - 1) / want);
     a.splits = (int32_t)std::max<int64_t>(1, (tn + a.per - 1) / a.per);
-    return QK_OK;
+    return tile;
 }
 }  // namespace
 }  // namespace qk
@@ -1001,7 +1067,7 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
     a.ws = (float*)ws;
     a.ldc = ldc;
     a.ldo = ldo;
-    plan_decision8(x->rows, y->rows, D, C, a);
+    const bool tile = plan_decision8(x->rows, y->rows, D, C, a);
     const hipStream_t s = (hipStream_t)stream;
     const unsigned joins = (unsigned)((x->rows * C + 255) / 256);
     if (y->rows == 0) {
@@ -1010,8 +1076,19 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
         QK_HIP(hipGetLastError());
         return QK_OK;
     }
-    hipLaunchKernelGGL(decision8_wave_kernel, dim3((unsigned)((x->rows + 31) / 32), (unsigned)a.splits), dim3(256),
-                       (size_t)4 * 32 * C * sizeof(float), s, a);
+    if (tile) {
+        static DeviceOnce attr;
+        if (attr.pending()) {
+            QK_HIP(hipFuncSetAttribute((const void*)decision8_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       kTileLds + QK_DECISION8_MAX_C * kTile * 4));
+            attr.done();
+        }
+        hipLaunchKernelGGL(decision8_tile_kernel, dim3((unsigned)((x->rows + kTile - 1) / kTile), (unsigned)a.splits), dim3(256),
+                           (size_t)kTileLds + (size_t)C * kTile * sizeof(float), s, a);
+    } else {
+        hipLaunchKernelGGL(decision8_wave_kernel, dim3((unsigned)((x->rows + 31) / 32), (unsigned)a.splits), dim3(256),
+                           (size_t)4 * 32 * C * sizeof(float), s, a);
+    }
     QK_HIP(hipGetLastError());
     if (a.splits > 1) {
         hipLaunchKernelGGL(decision8_join_kernel, dim3(joins), dim3(256), 0, s, a);

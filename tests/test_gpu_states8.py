@@ -249,7 +249,7 @@ def check_decision(out, x, y, coef, intercept):
 @pytest.mark.parametrize("M,N,D,C", [(1, 1, 2, 1), (1, 1000, 1024, 1), (1, 33, 65536, 3), (33, 31, 16, 2), (100, 100, 16, 1), (257, 300, 200, 45),
                                      (129, 1000, 64, 64), (500, 700, 1024, 1), (1, 5000, 256, 10), (64, 128, 128, 33), (1300, 400, 512, 7),
                                      (2, 257, 4096, 5), (40, 2000, 100, 16)])
-def test_decision8(M, N, D, C):
+def test_decision8(M, N, D, C, path):
     rng = np.random.default_rng(M + N + D + C)
     x, y = fill(S8.states(rng, M, D, "product")), fill(S8.states(rng, N, D, "spread"))
     coef = (rng.normal(size=(N, C)) * rng.choice([0, 1, 100], size=(N, 1))).astype(np.float32)
