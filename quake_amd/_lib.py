@@ -6,6 +6,7 @@ the first call that needs it raises.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -55,6 +56,9 @@ class qk_gram8_job(C.Structure):
     ]
 
 
+GRAM8_JOB = struct.Struct("@13q2i")     # qk_gram8_job as its fields in order
+assert GRAM8_JOB.size == C.sizeof(qk_gram8_job)
+
 STATS_LEN = 8
 STATS_WS = 1024 * 8
 NOISE_NONE, NOISE_GAUSSIAN, NOISE_SHOTS = 0, 1, 2
@@ -85,8 +89,8 @@ SIGNATURES = {
     "qk_states8_layout": (C.c_int, [_I64, C.POINTER(_I64), C.POINTER(_I64)]),
     "qk_states8_write_dev": (C.c_int, [_P, C.c_int, _I64, _I64, C.POINTER(qk_states8), _P]),
     "qk_states8_read_dev": (C.c_int, [C.POINTER(qk_states8), _I64, _P, _I64, _P, C.c_int, _I64, _P]),
-    "qk_gram8_workspace": (C.c_int, [C.POINTER(qk_gram8_job), C.c_int, C.POINTER(C.c_size_t)]),
-    "qk_gram8_jobs_dev": (C.c_int, [C.POINTER(qk_gram8_job), C.c_int, _P, C.c_size_t, _P]),
+    "qk_gram8_workspace": (C.c_int, [_P, C.c_int, C.POINTER(C.c_size_t)]),
+    "qk_gram8_jobs_dev": (C.c_int, [_P, C.c_int, _P, C.c_size_t, _P]),
     "qk_decision8_workspace": (C.c_int, [_I64, _I64, _I64, C.c_int, C.POINTER(C.c_size_t)]),
     "qk_decision8_dev": (C.c_int, [C.POINTER(qk_states8), C.POINTER(qk_states8), _I64, _P, _I64, C.c_int, _P, _P, _I64, _P,
                                    C.c_size_t, _P]),

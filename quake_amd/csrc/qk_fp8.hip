@@ -356,59 +356,92 @@ __global__ __launch_bounds__(256) void gram8_wave_kernel(Gram8Args args) {
 }
 
 // ---- 128 x 128 tiles ---------------------------------------------------------------------------------------------------
-// Four waves of 64 x 64 (2 x 2 matrix tiles, real and imaginary part: 128 accumulator registers), two workgroups per CU.
-// A step is one chunk of 128 + 128 rows, 32 KiB, copied straight to LDS one step ahead of its use (two buffers).  Row r of a
-// buffer holds its 16-byte piece p at p ^ ((r >> 1) & 7): the 16 rows that a quarter of a wave reads at once then lie in
-// different banks.
+// Four waves of 64 x 64 (2 x 2 matrix tiles, real and imaginary part: 128 accumulator registers), two workgroups per CU that
+// stay and walk the list of tiles.  A step is one chunk of 128 + 128 rows, 32 KiB, copied straight to LDS one step ahead of
+// its use (two buffers); the first chunk of the next tile is on its way while a tile is finished, so that rows of a few chunks
+// do not pay the latency of memory once per tile.  Row r of a buffer holds its 16-byte piece p at p ^ ((r >> 1) & 7): the 16
+// rows that a quarter of a wave reads at once then lie in different banks.
 constexpr int kTile = 128;
 constexpr int kStage = 2 * kTile * kChunkBytes;
-constexpr int kScales = 2 * kStage;                         // behind the two buffers: a dword of scales (8 chunks) per row, twice
-constexpr int kTileLds = kScales + 2 * 2 * kTile * 4;
+constexpr int kScales = 2 * kStage;                         // a dword of scales (8 chunks) per row, twice
+constexpr int kGains = kScales + 2 * 2 * kTile * 4;         // the rows' gains, twice
+constexpr int kPipeLds = kGains + 2 * 2 * kTile * 4;
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef const __attribute__((address_space(1))) void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 
-// NATIVE: products of the 8-bit codes on the matrix unit; else of their bf16 values.
-template <bool NATIVE>
-__device__ __forceinline__ void tile_product(uint8_t* lds, const Rows8& A, int64_t row_a, const Rows8& B, int64_t row_b, int chunks, int sb,
-                                             int c0, int c1, v16f (&re)[2][2], v16f (&im)[2][2]) {
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, h = lane >> 5;
-    const int64_t cb = (int64_t)chunks * kChunkBytes;
-    // copies: waves 0 and 1 bring A, 2 and 3 bring B, eight pieces of 8 rows each
-    const uint8_t* src = wave < 2 ? A.codes + row_a * cb : B.codes + row_b * cb;
-    const int last = (int)min((int64_t)kTile, (wave < 2 ? A.n - row_a : B.n - row_b)) - 1;
-    uint32_t vo[8];
+struct TileWork {              // what one pass of the pipeline computes; the same for the whole workgroup
+    Rows8 A, B;
+    int64_t row_a, row_b;
+    int chunks, sb, c0, c1;    // c0: a multiple of 8
+};
+
+template <bool NATIVE> struct TilePipe {
+    uint8_t* lds;
+    int wave, lane, r, h;
+    const uint8_t* src;        // copies: waves 0 and 1 bring A, 2 and 3 bring B, eight pieces of 8 rows each
+    const uint8_t* scale_src;
+    uint32_t vo[8], scale_vo;
+    int fa, fb, piece[4];
+    int buf = 0, area = 0;     // of the step that is computed next
+    int next_area = 0;         // of the scales that were copied last
+
+    __device__ __forceinline__ TilePipe(uint8_t* lds_) : lds(lds_) {
+        const int tid = threadIdx.x;
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        lane = tid & 63;
+        r = lane & 31;
+        h = lane >> 5;
+        // fragments: this lane's row of a 32-row tile, pieces 2 h and 2 h + 1 of either part (which codes of a chunk meet in
+        // one instruction is free as long as both operands agree)
+        fa = ((wave >> 1) * 64 + r) * kChunkBytes;
+        fb = kTile * kChunkBytes + ((wave & 1) * 64 + r) * kChunkBytes;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int row = (wave & 1) * 64 + e * 8 + (lane >> 3);
-        vo[e] = (uint32_t)min(row, last) * (uint32_t)cb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+        for (int p = 0; p < 4; ++p) piece[p] = (((p >> 1) * 4 + 2 * h + (p & 1)) ^ ((r >> 1) & 7)) << 4;
     }
-    const uint8_t* scale_src = wave < 2 ? A.scales + row_a * sb : B.scales + row_b * sb;
-    const uint32_t scale_vo = (uint32_t)min((wave & 1) * 64 + lane, last) * (uint32_t)sb;
-    auto stage = [&](int c, int buf) {
-        if (!(c & 7))
+
+    __device__ __forceinline__ void stage(int c, int to_buf) {
+        if (!(c & 7)) {
+            next_area ^= 1;
+            asm volatile("" : "+v"(scale_vo));
             __builtin_amdgcn_global_load_lds((gptr_t)(scale_src + (c >> 3) * 4 + (uint64_t)scale_vo),
-                                             (lptr_t)(lds + kScales + (c >> 3 & 1) * 1024 + wave * 256), 4, 0, 0);
+                                             (lptr_t)(lds + kScales + next_area * 1024 + wave * 256), 4, 0, 0);
+        }
         const uint8_t* at = src + (int64_t)c * kChunkBytes;
-        uint8_t* to = lds + buf * kStage + wave * 8192;
+        uint8_t* to = lds + to_buf * kStage + wave * 8192;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 8; ++e) {
+            asm volatile("" : "+v"(vo[e]));      // the sum stays base + 32-bit offset, the instruction's own form
             __builtin_amdgcn_global_load_lds((gptr_t)(at + (uint64_t)vo[e]), (lptr_t)(to + e * 1024), 16, 0, 0);
-    };
-    // fragments: this lane's row of a 32-row tile, pieces 2 h and 2 h + 1 of either part (which codes of a chunk meet in one
-    // instruction is free as long as both operands agree)
-    const int fa = ((wave >> 1) * 64 + r) * kChunkBytes, fb = kTile * kChunkBytes + ((wave & 1) * 64 + r) * kChunkBytes;
-    const int key = (r >> 1) & 7;
-    int piece[4];
+        }
+    }
+
+    // a tile's first chunk, and its gains into half `g` of their area
+    __device__ __forceinline__ void open(const TileWork& w, int to_buf, int g) {
+        const int64_t cb = (int64_t)w.chunks * kChunkBytes;
+        const Rows8 S = wave < 2 ? w.A : w.B;
+        const int64_t row0 = wave < 2 ? w.row_a : w.row_b;
+        const int last = (int)min((int64_t)kTile, S.n - row0) - 1;      // rows behind the last repeat it
+        src = S.codes + row0 * cb;
+        scale_src = S.scales + row0 * w.sb;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) piece[p] = (((p >> 1) * 4 + 2 * h + (p & 1)) ^ key) << 4;
-    auto compute = [&](int c, int buf) {
+        for (int e = 0; e < 8; ++e) {
+            const int row = (wave & 1) * 64 + e * 8 + (lane >> 3);
+            vo[e] = (uint32_t)min(row, last) * (uint32_t)cb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+        }
+        const uint32_t row = (uint32_t)min((wave & 1) * 64 + lane, last);
+        scale_vo = row * (uint32_t)w.sb;
+        __builtin_amdgcn_global_load_lds((gptr_t)(S.gains + row0 + (uint64_t)row), (lptr_t)(lds + kGains + g * 1024 + wave * 256), 4, 0, 0);
+        stage(w.c0, to_buf);
+    }
+
+    __device__ __forceinline__ void compute(int c, v16f (&re)[2][2], v16f (&im)[2][2]) {
         const uint8_t* base = lds + buf * kStage;
         const int shift = (c >> 1 & 3) * 8;
         uint32_t sa[2], sc[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const uint8_t* scale = lds + kScales + (c >> 3 & 1) * 1024 + r * 4 + t * 128;
+            const uint8_t* scale = lds + kScales + area * 1024 + r * 4 + t * 128;
             sa[t] = *(const uint32_t*)(scale + (wave >> 1) * 256);
             sc[t] = *(const uint32_t*)(scale + 512 + (wave & 1) * 256);
         }
@@ -485,31 +518,53 @@ __device__ __forceinline__ void tile_product(uint8_t* lds, const Rows8& A, int64
                 }
             }
         }
-    };
-    // the copies of this chunk have landed, and every wave is done with the buffer that is filled next
-    auto meet = [] { asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory"); };
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) re[i][j][k] = im[i][j][k] = 0.f;
-    stage(c0, 0);                                       // c0 is a multiple of 8
-    for (int c = c0; c < c1; c += 2) {
-        meet();
-        if (c + 1 < c1) stage(c + 1, 1);
-        compute(c, 0);
-        if (c + 1 >= c1) break;
-        meet();
-        if (c + 2 < c1) stage(c + 2, 0);
-        compute(c + 1, 1);
     }
-}
 
-// Position of a workgroup -> item of the launch: groups of 64 consecutive items (what an XCD runs at a time: 8 x 8 tiles of a
-// strip) are dealt to the eight XCDs in turn, the rest of the list evenly.
-__device__ __forceinline__ bool gram8_item(uint32_t total, uint32_t& item) {
-    const uint32_t xcd = blockIdx.x & 7u, seq = blockIdx.x >> 3, full = total >> 9;
+    // work(k, w): the k-th piece of this workgroup's work, false behind the last.  finish(k, more, gains, room, re, im): more: the next
+    // one is open; room: 8 KiB of LDS for this wave, the buffer of the last chunk.  STORES: finish issues at least 63 memory
+    // instructions.
+    template <bool STORES, typename Work, typename Finish> __device__ __forceinline__ void run(Work work, Finish finish) {
+        TileWork w;
+        if (!work(0, w)) return;
+        open(w, 0, 0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int k = 0;; ++k) {
+            v16f re[2][2], im[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) re[i][j][q] = im[i][j][q] = 0.f;
+            int c = w.c0;
+            const int c1 = w.c1;
+            area = next_area;
+            for (; c + 1 < c1; ++c) {
+                stage(c + 1, buf ^ 1);
+                compute(c, re, im);
+                buf ^= 1;
+                // the copies of the next chunk have landed, and every wave has read the buffer that is filled after it
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                area = (c + 1) & 7 ? area : next_area;
+            }
+            const bool more = work(k + 1, w);
+            if (more) open(w, buf ^ 1, (k + 1) & 1);
+            compute(c, re, im);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            finish(k, more, (const float*)(lds + kGains + (k & 1) * 1024), lds + buf * kStage + wave * 8192, re, im);
+            if (!more) return;
+            buf ^= 1;
+            // memory instructions end in order: behind a tile's stores it is enough that all but the youngest 63 have
+            if constexpr (STORES) asm volatile("s_waitcnt vmcnt(63) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+    }
+};
+
+// Position in a launch -> item: groups of 64 consecutive items (what an XCD runs at a time: 8 x 8 tiles of a strip) are dealt to
+// the eight XCDs in turn, the rest of the list evenly.
+__device__ __forceinline__ bool gram8_item(uint32_t total, uint32_t position, uint32_t& item) {
+    const uint32_t xcd = position & 7u, seq = position >> 3, full = total >> 9;
     if ((seq >> 6) < full) {
         item = ((((seq >> 6) << 3) + xcd) << 6) + (seq & 63u);
         return true;
@@ -519,89 +574,150 @@ __device__ __forceinline__ bool gram8_item(uint32_t total, uint32_t& item) {
     return in < share && item < total;
 }
 
-template <typename T> __device__ __forceinline__ T k_as(float k) { return (T)k; }
+// Stores through a buffer: the offset -1 is dropped.  The range covers a tile of any row stride the host lets through.
+constexpr int kRange = 0x7ffffffe, kRsrc = 0x00027000;
+template <typename T> __device__ __forceinline__ void put(T v, __amdgpu_buffer_rsrc_t to, int off, int soff) {
+    if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), to, off, soff, 0);
+    else if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), to, off, soff, 0);
+    else {
+        typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, v), to, off, soff, 0);
+    }
+}
+__device__ __forceinline__ void put16(uint4 v, __amdgpu_buffer_rsrc_t to, int off, int soff) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), to, off, soff, 0);
+}
+
+// The same in every lane, and known to be: addresses and descriptors made from it stay in scalar registers.
+template <typename I> __device__ __forceinline__ I uniform(I v) { return (I)__builtin_amdgcn_readfirstlane((int)v); }
 
 // T: the type of K
 template <bool NATIVE, typename T>
 __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
     extern __shared__ uint8_t lds[];
-    uint32_t item;
-    if (!gram8_item(args.total, item)) return;
-    const Gram8JobDev& J = args.job[gram8_job(args, item)];
-    const uint32_t in = item - J.begin, slice = in / J.live, t = in - slice * J.live;
-    uint32_t ti, tj;
-    gram8_tile(J, t, ti, tj);
-    v16f re[2][2], im[2][2];
-    const int c0 = (int)slice * J.per, c1 = min(J.chunks, c0 + J.per);
-    tile_product<NATIVE>(lds, J.A, (int64_t)ti * kTile, J.B, (int64_t)tj * kTile, J.chunks, J.sb, c0, c1, re, im);
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, h = lane >> 5;
-    if (J.slices > 1) {
-        float2* ws = (float2*)(args.ws + J.ws) + (((int64_t)t * J.slices + slice) * 16 + wave * 4) * 1024 + lane;
+    TilePipe<NATIVE> pipe(lds);
+    const int wave = pipe.wave, lane = pipe.lane, r = pipe.r, h = pipe.h;
+    struct Where { int job; uint32_t ti, tj, slice, t; } now{}, before{};      // of the tile that was opened last and the one before
+    auto work = [&](int k, TileWork& w) {
+        uint32_t item;
+        if (!gram8_item(args.total, blockIdx.x + (uint32_t)k * gridDim.x, item)) return false;
+        before = now;
+        Where& p = now;
+        p.job = uniform(gram8_job(args, item));
+        const Gram8JobDev& J = args.job[p.job];
+        const uint32_t in = item - J.begin;
+        p.slice = uniform(in / J.live);
+        p.t = uniform(in - p.slice * J.live);
+        gram8_tile(J, p.t, p.ti, p.tj);
+        p.ti = uniform(p.ti);
+        p.tj = uniform(p.tj);
+        w.A = J.A;
+        w.B = J.B;
+        w.row_a = (int64_t)p.ti * kTile;
+        w.row_b = (int64_t)p.tj * kTile;
+        w.chunks = J.chunks;
+        w.sb = J.sb;
+        w.c0 = (int)p.slice * J.per;
+        w.c1 = min(J.chunks, w.c0 + J.per);
+        return true;
+    };
+    auto finish = [&](int, bool more, const float* gains, uint8_t* room, v16f (&re)[2][2], v16f (&im)[2][2]) {
+        const Where w = more ? before : now, p = {uniform(w.job), uniform(w.ti), uniform(w.tj), uniform(w.slice), uniform(w.t)};
+        const Gram8JobDev& J = args.job[p.job];
+        if (J.slices > 1) {
+            float2* ws = (float2*)(args.ws + J.ws) + (((int64_t)p.t * J.slices + p.slice) * 16 + wave * 4) * 1024 + lane;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) ws[(i * 2 + j) * 1024 + q * 64] = make_float2(re[i][j][q], im[i][j][q]);
+            return;
+        }
+        // K from the registers: one of them holds 32 neighbours of two rows.  Entries outside the matrix (symmetric: on or below
+        // the diagonal) get an offset that the buffer's range check drops, so the stores have no branches.
+        const int S = sizeof(T);
+        const bool sym = J.flags & QK_GRAM_SYMMETRIC, diagonal = sym && p.ti == p.tj;
+        const int64_t row_t = (int64_t)p.ti * kTile + (wave >> 1) * 64, col_t = (int64_t)p.tj * kTile + (wave & 1) * 64;
+        const int rows = (int)min((int64_t)64, J.A.n - row_t), cols = (int)min((int64_t)64, J.B.n - col_t);     // (may be negative)
+        const int step = (int)J.ldk * S, ahead = (int)(col_t - row_t);
+        const __amdgpu_buffer_rsrc_t K = __builtin_amdgcn_make_buffer_rsrc((char*)J.K + (row_t * J.ldk + col_t) * S, 0, kRange, kRsrc);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j) {
+                const int col = j * 32 + r, off = 4 * h * step + col * S;
+                const float gb = gains[kTile + (wave & 1) * 64 + col];
+                // rows i * 32 + 4 h + n with n < limit
+                int limit = rows - i * 32 - 4 * h;
+                if (diagonal) limit = min(limit, col + ahead - i * 32 - 4 * h);
+                if (col >= cols) limit = 0;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) ws[(i * 2 + j) * 1024 + k * 64] = make_float2(re[i][j][k], im[i][j][k]);
-        return;
-    }
-    // Every 32 x 32 tile goes through a piece of LDS of its wave, [column][row], rows of 36 floats.  A tile whose entries all
-    // exist stores K from the registers (whole lines: a register holds 32 neighbours of two rows) and the mirror from LDS, 16
-    // bytes a lane; the others are stored entry by entry.
-    const bool sym = J.flags & QK_GRAM_SYMMETRIC;
-    const int64_t row_t = (int64_t)ti * kTile + (wave >> 1) * 64, col_t = (int64_t)tj * kTile + (wave & 1) * 64;
-    T* const M = (T*)(sym ? J.K : J.KT);
-    const int64_t ldm = sym ? J.ldk : J.ldkt;
-    const bool whole = (int64_t)(ti + 1) * kTile <= J.A.n && (int64_t)(tj + 1) * kTile <= J.B.n && !(sym && ti == tj) &&
-                       (((uintptr_t)M | (uint64_t)(ldm * (int64_t)sizeof(T))) & 15) == 0;
-    __syncthreads();                                        // the buffers are free
-    float* const piece = (float*)lds + wave * (32 * 36);
+                for (int q = 0; q < 16; q += 4) {
+                    const float4 ga = *(const float4*)(gains + (wave >> 1) * 64 + i * 32 + 2 * q + 4 * h);
+                    const float g[4] = {ga.x, ga.y, ga.z, ga.w};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        float ga[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) ga[k] = J.A.gains[min(row_t + i * 32 + acc_row(lane, k), J.A.n - 1)];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int64_t row0 = row_t + i * 32, col0 = col_t + j * 32;
-            const float gb = J.B.gains[min(col0 + r, J.B.n - 1)];
-            float k[16];
-#pragma unroll
-            for (int q = 0; q < 16; ++q) k[q] = (re[i][j][q] * re[i][j][q] + im[i][j][q] * im[i][j][q]) * (ga[q] * gb);
-            if (M || !whole) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *(float4*)(piece + r * 36 + 8 * q + 4 * h) = make_float4(k[4 * q], k[4 * q + 1], k[4 * q + 2], k[4 * q + 3]);
-            }
-            __builtin_amdgcn_wave_barrier();                // (a wave's LDS accesses stay in order)
-            if (whole) {
-                T* at = (T*)J.K + (row0 + 4 * h) * J.ldk + col0 + r;
-#pragma unroll
-                for (int q = 0; q < 16; ++q) at[(8 * (q >> 2) + (q & 3)) * J.ldk] = k_as<T>(k[q]);
-                if (M) {
-                    constexpr int E = 16 / sizeof(T), L = 32 / E;       // entries a lane stores, lanes a mirrored row takes
-#pragma unroll
-                    for (int c = lane / L; c < 32; c += 64 / L) {
-                        const float* from = piece + c * 36 + (lane % L) * E;
-                        T v[E] __attribute__((aligned(16)));
-#pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] = k_as<T>(from[e]);
-                        *(uint4*)(M + (col0 + c) * ldm + row0 + (lane % L) * E) = *(const uint4*)v;
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = re[i][j][q + e], y = im[i][j][q + e];
+                        re[i][j][q + e] = (x * x + y * y) * (g[e] * gb);
+                        const int n = 2 * q + e;
+                        put<T>((T)re[i][j][q + e], K, n < limit ? off : -1, (i * 32 + n) * step);
                     }
                 }
-            } else {
-                for (int q = 0; q < 16; ++q) {
-                    const int rr = 2 * q + h;
-                    const int64_t row = row0 + rr, col = col0 + r;
-                    if (row >= J.A.n || col >= J.B.n || (sym && row > col)) continue;
-                    const float v = sym && row == col ? 1.f : piece[r * 36 + rr];
-                    ((T*)J.K)[row * J.ldk + col] = k_as<T>(v);
-                    if (M && !(sym && row == col)) M[col * ldm + row] = k_as<T>(v);
-                }
             }
-            __builtin_amdgcn_wave_barrier();
-        }
-    }
+        if (diagonal && ahead == 0) put<T>((T)1.f, K, lane < min(rows, cols) ? lane * (step + S) : -1, 0);
+        T* const mirror = (T*)(sym ? J.K : J.KT);
+        if (!mirror) return;
+        // The mirror through LDS, [column][its rows], 16-byte pieces of a column at piece ^ key(column); out in whole lines where the
+        // rows allow it.
+        const int64_t ldm = sym ? J.ldk : J.ldkt;
+        const int mstep = (int)ldm * S;
+        const bool whole = rows == 64 && cols == 64 && !diagonal && !(((uintptr_t)mirror | (uint32_t)mstep) & 15);
+        const __amdgpu_buffer_rsrc_t M = __builtin_amdgcn_make_buffer_rsrc((char*)mirror + (col_t * ldm + row_t) * S, 0, kRange, kRsrc);
+        constexpr int E = 16 / sizeof(T), IP = sizeof(T) == 8 ? 1 : 2, JP = sizeof(T) == 2 ? 2 : 1;      // matrix tiles that 8 KiB hold
+        constexpr int RB = IP * 32 * sizeof(T), L = RB / 16;                                             // bytes and pieces of a column
+#pragma unroll
+        for (int j0 = 0; j0 < 2; j0 += JP)
+#pragma unroll
+            for (int i0 = 0; i0 < 2; i0 += IP) {
+#pragma unroll
+                for (int j = 0; j < JP; ++j)
+#pragma unroll
+                    for (int i = 0; i < IP; ++i)
+#pragma unroll
+                        for (int q = 0; q < 16; q += 4) {
+                            uint8_t* const at = room + (j * 32 + r) * RB;
+                            const int key = sizeof(T) == 2 ? (r >> 1) & 7 : r & 15, byte = (i * 32 + 2 * q + 4 * h) * (int)sizeof(T);
+                            T u[4] __attribute__((aligned(16)));
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) u[e] = (T)re[i0 + i][j0 + j][q + e];
+                            if constexpr (sizeof(T) == 2) *(uint2*)(at + (((byte >> 4) ^ key) << 4) + (byte & 8)) = *(const uint2*)u;
+                            else
+#pragma unroll
+                                for (int e = 0; e < 4; e += E) *(uint4*)(at + (((byte >> 4) + e / E) ^ key) * 16) = *(const uint4*)(u + e);
+                        }
+                __builtin_amdgcn_wave_barrier();                // (a wave's LDS accesses stay in order)
+                const int s = lane % L;
+#pragma unroll 4
+                for (int n = 0; n < JP * L / 2; ++n) {
+                    const int c = n * (64 / L) + lane / L, key = sizeof(T) == 2 ? (c >> 1) & 7 : c & 15, col = j0 * 32 + c;
+                    const uint4 u = *(const uint4*)(room + c * RB + ((s ^ key) << 4));
+                    const int off = c * mstep + s * 16, so = j0 * 32 * mstep + i0 * 32 * S;
+                    if (whole) put16(u, M, off, so);
+                    else {
+                        int limit = rows;
+                        if (diagonal) limit = min(limit, col + ahead);
+                        if (col >= cols) limit = 0;
+                        T v[E] __attribute__((aligned(16)));
+                        *(uint4*)v = u;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) put<T>(v[e], M, i0 * 32 + s * E + e < limit ? off + e * S : -1, so);
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+    };
+    pipe.template run<true>(work, finish);
 }
 
 // Adds the slices of every tile in order and finishes its entries: one thread per entry.  SUB: matrix tiles per tile (1 or 16).
@@ -640,9 +756,9 @@ struct Decision8Args {
     const float* coef;
     const float* intercept;
     float* out;
-    float* ws;             // splits x M x C partial sums when splits > 1
-    int64_t ldc, ldo;
-    int32_t C, chunks, sb, splits, per;      // per: tile columns of one split
+    float* ws;             // [parts][C][stride] partial sums
+    int64_t ldc, ldo, stride;
+    int32_t C, chunks, sb, splits, per, parts;      // per: tile columns of one split; parts: what is left to be joined, 0: out is written at once
 };
 
 // The product is taken the other way round (B's rows times A's), so a lane holds 16 of B's rows for ONE row of A: K times the
@@ -689,79 +805,101 @@ __global__ __launch_bounds__(256) void decision8_wave_kernel(Decision8Args a) {
         float s = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) s += acc[w * 32 * a.C + k];
-        if (a.splits == 1) a.out[(row0 + row) * a.ldo + c] = s + (a.intercept ? a.intercept[c] : 0.f);
-        else a.ws[((int64_t)blockIdx.y * a.A.n + row0 + row) * a.C + c] = s;
+        if (a.parts == 0) a.out[(row0 + row) * a.ldo + c] = s + (a.intercept ? a.intercept[c] : 0.f);
+        else a.ws[((int64_t)blockIdx.y * a.C + c) * a.stride + row0 + row] = s;
     }
 }
 
-// The same over 128 x 128 tiles: a workgroup keeps 128 rows of A and walks B's tiles of its range; the sums of its C columns
-// wait in LDS behind the tile buffers, [C][128], where the two waves that share rows of A add one after the other.  The
-// coefficients of a tile pass through the buffers, [C][128]: a lane reads four of them at once, the same for its whole half.
+// The same over 128 x 128 tiles: a workgroup keeps 128 rows of A and walks B's tiles of its range.  Each of the two waves that
+// share rows of A keeps its own sums of the C columns: in LDS up to eight columns, in the workspace (which stays in L2) above, where
+// every lane adds to entries that no other lane touches.  A wave brings the coefficients of its 64 rows of B through its part of the free buffer,
+// [32 columns][64]; a lane reads four at once, the same for its whole half.
+constexpr int kLdsColumns = 8;
+constexpr int kDecisionLds = kPipeLds + 2 * kLdsColumns * kTile * 4;
+static_assert(2 * kDecisionLds <= 160 * 1024, "two workgroups per CU");
+
 __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a) {
     extern __shared__ uint8_t lds[];
-    float* const acc = (float*)(lds + kTileLds);
-    float* const coef = (float*)lds;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, h = lane >> 5;
-    const int xs = (wave & 1) * 64 + r, ys = (wave >> 1) * 64;
-    const int64_t row0 = (int64_t)blockIdx.x * kTile;
-    for (int k = tid; k < kTile * a.C; k += 256) acc[k] = 0.f;
-    float gx[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) gx[j] = a.A.gains[min(row0 + xs + j * 32, a.A.n - 1)];
-    const int tiles = (int)((a.B.n + kTile - 1) / kTile), t1 = min(tiles, ((int)blockIdx.y + 1) * a.per);
-    for (int t = (int)blockIdx.y * a.per; t < t1; ++t) {
-        const int64_t col0 = (int64_t)t * kTile;
-        v16f re[2][2], im[2][2];
-        tile_product<false>(lds, a.B, col0, a.A, row0, a.chunks, a.sb, 0, a.chunks, re, im);
-        __syncthreads();
-        for (int k = tid; k < kTile * a.C; k += 256) {
-            const int row = (int)((unsigned)k / (unsigned)a.C), c = k - row * a.C;
-            coef[c * kTile + row] = col0 + row < a.B.n ? a.coef[(col0 + row) * a.ldc + c] : 0.f;
-        }
+    TilePipe<false> pipe(lds);
+    const int tid = threadIdx.x, wave = pipe.wave, lane = pipe.lane, r = pipe.r, h = pipe.h;
+    const int xs = (wave & 1) * 64, ys = (wave >> 1) * 64;
+    const int64_t row0 = (int64_t)blockIdx.x * kTile, mp = (int64_t)gridDim.x * kTile;
+    float* const sums = (float*)(lds + kPipeLds);
+    const bool in_lds = a.C <= kLdsColumns;
+    const int tiles = (int)((a.B.n + kTile - 1) / kTile), t0 = (int)blockIdx.y * a.per, t1 = min(tiles, t0 + a.per);
+    auto work = [&](int k, TileWork& w) {
+        if (t0 + k >= t1) return false;
+        w.A = a.B;
+        w.B = a.A;
+        w.row_a = (int64_t)(t0 + k) * kTile;
+        w.row_b = row0;
+        w.chunks = a.chunks;
+        w.sb = a.sb;
+        w.c0 = 0;
+        w.c1 = a.chunks;
+        return true;
+    };
+    auto finish = [&](int k, bool, const float* gains, uint8_t* room, v16f (&re)[2][2], v16f (&im)[2][2]) {
+        float* const coef = (float*)room;
+        const int64_t y = (int64_t)(t0 + k) * kTile + ys + lane;
+        const float* from = a.coef + min(y, a.B.n - 1) * a.ldc;
+        const float gx[2] = {gains[kTile + xs + r], gains[kTile + xs + 32 + r]};
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const float gy = a.B.gains[min(col0 + ys + i * 32 + acc_row(lane, q), a.B.n - 1)];
+            for (int q = 0; q < 16; q += 4) {
+                const float4 gy = *(const float4*)(gains + ys + i * 32 + 2 * q + 4 * h);
+                const float g[4] = {gy.x, gy.y, gy.z, gy.w};
 #pragma unroll
-                for (int j = 0; j < 2; ++j) re[i][j][q] = (re[i][j][q] * re[i][j][q] + im[i][j][q] * im[i][j][q]) * (gx[j] * gy);
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        re[i][j][q + e] = (re[i][j][q + e] * re[i][j][q + e] + im[i][j][q + e] * im[i][j][q + e]) * (gx[j] * g[e]);
             }
-        __syncthreads();
-        for (int half = 0; half < 2; ++half) {
-            if ((wave >> 1) == half)
-                for (int c = 0; c < a.C; ++c) {
-                    float s[2] = {0.f, 0.f};
+        for (int c0 = 0; c0 < a.C; c0 += 32) {
+            const int n = min(32, a.C - c0);
+            for (int c = 0; c < n; ++c) coef[c * 64 + lane] = y < a.B.n ? from[c0 + c] : 0.f;
+            __builtin_amdgcn_wave_barrier();
+            for (int c = 0; c < n; ++c) {
+                float s[2] = {0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const float4 w = *(const float4*)(coef + c * kTile + ys + i * 32 + 8 * q + 4 * h);
+                    for (int q = 0; q < 16; q += 4) {
+                        const float4 w = *(const float4*)(coef + c * 64 + i * 32 + 2 * q + 4 * h);
 #pragma unroll
-                            for (int j = 0; j < 2; ++j)
-                                s[j] += re[i][j][4 * q] * w.x + re[i][j][4 * q + 1] * w.y + re[i][j][4 * q + 2] * w.z + re[i][j][4 * q + 3] * w.w;
-                        }
+                        for (int j = 0; j < 2; ++j)
+                            s[j] += re[i][j][q] * w.x + re[i][j][q + 1] * w.y + re[i][j][q + 2] * w.z + re[i][j][q + 3] * w.w;
+                    }
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) s[j] += __shfl_xor(s[j], 32, 64);
-                    acc[c * kTile + xs + h * 32] += h ? s[1] : s[0];      // lane half h adds the rows of tile j = h
-                }
-            __syncthreads();
+                for (int j = 0; j < 2; ++j) s[j] += __shfl_xor(s[j], 32, 64);
+                const float mine = h ? s[1] : s[0];                  // lane half h keeps the rows of matrix tile j = h
+                float* const to = in_lds ? sums + ((wave >> 1) * kLdsColumns + c) * kTile + xs + lane
+                                         : a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + c) * mp + row0 + xs + lane;
+                *to = k ? *to + mine : mine;
+            }
+            __builtin_amdgcn_wave_barrier();
         }
-    }
+    };
+    pipe.run<false>(work, finish);
+    if (!in_lds) return;
+    __syncthreads();
     for (int k = tid; k < kTile * a.C; k += 256) {
-        const int c = k >> 7, row = k & (kTile - 1);
+        const int row = k & (kTile - 1), c = k >> 7;
         if (row0 + row >= a.A.n) continue;
-        if (a.splits == 1) a.out[(row0 + row) * a.ldo + c] = acc[k] + (a.intercept ? a.intercept[c] : 0.f);
-        else a.ws[((int64_t)blockIdx.y * a.A.n + row0 + row) * a.C + c] = acc[k];
+        const float s = sums[c * kTile + row] + sums[(kLdsColumns + c) * kTile + row];
+        if (a.parts == 0) a.out[(row0 + row) * a.ldo + c] = s + (a.intercept ? a.intercept[c] : 0.f);
+        else a.ws[((int64_t)blockIdx.y * a.C + c) * mp + row0 + row] = s;
     }
 }
 
+// Adds the parts in order: ws[part][C][stride], parts == 0: only the intercept.
 __global__ __launch_bounds__(256) void decision8_join_kernel(Decision8Args a) {
-    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (k >= a.A.n * a.C) return;
-    const int64_t row = k / a.C;
-    const int c = (int)(k - row * a.C);
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int c = blockIdx.y;
+    if (row >= a.A.n) return;
     double s = 0.0;
-    for (int p = 0; p < a.splits; ++p) s += (double)a.ws[(int64_t)p * a.A.n * a.C + k];
+    for (int p = 0; p < a.parts; ++p) s += (double)a.ws[((int64_t)p * a.C + c) * a.stride + row];
     a.out[row * a.ldo + c] = (float)(s + (a.intercept ? (double)a.intercept[c] : 0.0));
 }
 
@@ -788,6 +926,7 @@ Rows8 rows8(const qk_states8& s) { return Rows8{(const uint8_t*)s.codes, (const 
 // fill the chip; the 32 x 32 kernel starts at once, takes few rows without waste and spreads a small job over more
 // workgroups.
 enum Gram8Kind { GK_WAVE, GK_TILE, GK_TILE_F64, GK_TILE_NATIVE, GK_KINDS };
+constexpr double g_tiles = 96, g_steps = 1024;
 std::atomic<int> g_path{0};      // development hook: 0 by rule, 1 always 32 x 32, 2 always 128 x 128
 
 int64_t live_tiles(const qk_gram8_job& j, int64_t tile) {
@@ -795,12 +934,19 @@ int64_t live_tiles(const qk_gram8_job& j, int64_t tile) {
     return (j.flags & QK_GRAM_SYMMETRIC) ? tm * (tm + 1) / 2 : tm * tn;
 }
 
-Gram8Kind kind_of(const qk_gram8_job& j) {
+// 128 x 128 tiles that a job fills (its parts of tiles added up); 0: too few rows, or rows so long or so far apart that 32 bits
+// do not hold the offsets inside a tile
+double tiles_of(const qk_gram8_job& j) {
+    const int64_t m = std::min(j.A.rows, j.B.rows), n = std::max(j.A.rows, j.B.rows);
+    if (m < (g_path.load(std::memory_order_relaxed) == 2 ? 1 : 33) || code_bytes(j.D) > (int64_t)1 << 24) return 0;
+    if (std::max(j.ldk, j.KT ? j.ldkt : 0) * 8 > (int64_t)1 << 23) return 0;
+    return (double)std::max<int64_t>(m, 64) * (double)n / (kTile * kTile) * (j.flags & QK_GRAM_SYMMETRIC ? 0.5 : 1.0);
+}
+
+// tiles, steps (tiles times chunks): of all jobs of the call
+Gram8Kind kind_of(const qk_gram8_job& j, double tiles, double steps) {
     const int path = g_path.load(std::memory_order_relaxed);
-    const int64_t chunks = (j.D + kChunk - 1) / kChunk;
-    const bool fits = code_bytes(j.D) <= (int64_t)1 << 24;      // 32-bit offsets inside a tile
-    const bool tile = path == 2 || (path == 0 && std::min(j.A.rows, j.B.rows) >= 64 && live_tiles(j, kTile) * chunks >= 1024);
-    if (!tile || !fits) return GK_WAVE;
+    if (path == 1 || tiles_of(j) == 0 || (path == 0 && tiles < g_tiles && steps < g_steps)) return GK_WAVE;
     return j.flags & QK_GRAM8_F16 ? GK_TILE_NATIVE : j.flags & QK_GRAM8_F64 ? GK_TILE_F64 : GK_TILE;
 }
 
@@ -855,8 +1001,14 @@ int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind
 // The launches of a call, in order: `each(plan, kind)`.  Jobs with long rows go first, so that a launch does not end on them.
 template <typename F> int gram8_launches(const qk_gram8_job* jobs, int n, F each) {
     std::vector<int> by[GK_KINDS];
+    double tiles = 0, steps = 0;
+    for (int k = 0; k < n; ++k) {
+        const double t = tiles_of(jobs[k]);
+        tiles += t;
+        steps += t * (double)((jobs[k].D + kChunk - 1) / kChunk);
+    }
     for (int k = 0; k < n; ++k)
-        if (jobs[k].A.rows && jobs[k].B.rows) by[kind_of(jobs[k])].push_back(k);
+        if (jobs[k].A.rows && jobs[k].B.rows) by[kind_of(jobs[k], tiles, steps)].push_back(k);
     for (int kind = GK_KINDS - 1; kind >= 0; --kind) {
         std::stable_sort(by[kind].begin(), by[kind].end(), [&](int a, int b) { return jobs[a].D > jobs[b].D; });
         for (size_t k = 0; k < by[kind].size(); k += kGram8Jobs) {
@@ -895,13 +1047,16 @@ bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
     a.chunks = (int32_t)((D + kChunk - 1) / kChunk);
     a.sb = (int32_t)scale_bytes(D);
     const int path = g_path.load(std::memory_order_relaxed);
+    const double area = (double)std::max<int64_t>(M, 64) * (double)std::max<int64_t>(N, 64) / (kTile * kTile);
     const bool tile = code_bytes(D) <= (int64_t)1 << 24 &&
-                      (path == 2 || (path == 0 && std::min(M, N) >= 64 && (M + kTile - 1) / kTile * ((N + kTile - 1) / kTile) * a.chunks >= 1024));
+                      (path == 2 || (path == 0 && M > 32 && (area >= g_tiles || area * a.chunks >= g_steps)));
     const int64_t side = tile ? kTile : 32, tm = (M + side - 1) / side, tn = (N + side - 1) / side;
     const int64_t want = tile ? std::max<int64_t>(1, std::min<int64_t>(tn, 512 / std::max<int64_t>(tm, 1)))
                               : std::max<int64_t>(1, std::min<int64_t>((tn + 3) / 4, 1024 / std::max<int64_t>(tm, 1)));
     a.per = (int32_t)std::max<int64_t>(1, (tn + want - 1) / want);
     a.splits = (int32_t)std::max<int64_t>(1, (tn + a.per - 1) / a.per);
+    a.stride = tm * side;
+    a.parts = tile && C > kLdsColumns ? 2 * a.splits : a.splits > 1 ? a.splits : 0;
     return tile;
 }
 }  // namespace
@@ -986,25 +1141,27 @@ extern "C" int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* 
     do {                                                                                                            \
         static DeviceOnce attr;                                                                                     \
         if (attr.pending()) {                                                                                       \
-            QK_HIP(hipFuncSetAttribute((const void*)gram8_tile_kernel<NATIVE, T>, hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds)); \
+            QK_HIP(hipFuncSetAttribute((const void*)gram8_tile_kernel<NATIVE, T>, hipFuncAttributeMaxDynamicSharedMemorySize, kPipeLds)); \
             attr.done();                                                                                            \
         }                                                                                                           \
-        hipLaunchKernelGGL((gram8_tile_kernel<NATIVE, T>), dealt, dim3(256), kTileLds, s, p.args);                  \
+        hipLaunchKernelGGL((gram8_tile_kernel<NATIVE, T>), dealt, dim3(256), kPipeLds, s, p.args);                  \
     } while (0)
 
 extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream) {
     int rc = check_gram8(jobs, n_jobs);
     if (rc) return rc;
     if ((uintptr_t)ws & 15) return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: the workspace needs 16-byte alignment");
-    size_t need = 0;
-    if ((rc = qk_gram8_workspace(jobs, n_jobs, &need))) return rc;
-    if (need > ws_bytes || (need && !ws))
-        return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: workspace smaller than qk_gram8_workspace asks for");
+    rc = gram8_launches(jobs, n_jobs, [&](const Gram8Plan& p, Gram8Kind) {      // all of it is checked before any of it runs
+        if (p.ws_floats * sizeof(float) > ws_bytes || (p.ws_floats && !ws))
+            return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: workspace smaller than qk_gram8_workspace asks for");
+        return (int)QK_OK;
+    });
+    if (rc) return rc;
     const hipStream_t s = (hipStream_t)stream;
     return gram8_launches(jobs, n_jobs, [&](Gram8Plan& p, Gram8Kind kind) {
         p.args.ws = (float*)ws;
         const uint32_t total = p.args.total, full = total >> 9;
-        const dim3 dealt((full << 9) + 8 * ((total - (full << 9) + 7) >> 3));
+        const dim3 dealt(std::min<uint32_t>(512, (full << 9) + 8 * ((total - (full << 9) + 7) >> 3)));      // two workgroups per CU
         if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, dim3(total), dim3(256), 0, s, p.args);
         else if (kind == GK_TILE) QK_TILE8(false, float);
         else if (kind == GK_TILE_F64) QK_TILE8(false, double);
@@ -1041,7 +1198,7 @@ extern "C" int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, si
     Decision8Args a;
     std::memset(&a, 0, sizeof(a));
     plan_decision8(M, N, D, C, a);
-    if (a.splits > 1) *bytes = (size_t)a.splits * M * C * sizeof(float);
+    *bytes = (size_t)a.parts * C * a.stride * sizeof(float);
     return QK_OK;
 }
 
@@ -1069,10 +1226,10 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
     a.ldo = ldo;
     const bool tile = plan_decision8(x->rows, y->rows, D, C, a);
     const hipStream_t s = (hipStream_t)stream;
-    const unsigned joins = (unsigned)((x->rows * C + 255) / 256);
+    const dim3 joins((unsigned)((x->rows + 255) / 256), (unsigned)C);
     if (y->rows == 0) {
-        a.splits = 0;
-        hipLaunchKernelGGL(decision8_join_kernel, dim3(joins), dim3(256), 0, s, a);
+        a.parts = 0;
+        hipLaunchKernelGGL(decision8_join_kernel, joins, dim3(256), 0, s, a);
         QK_HIP(hipGetLastError());
         return QK_OK;
     }
@@ -1080,18 +1237,18 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
         static DeviceOnce attr;
         if (attr.pending()) {
             QK_HIP(hipFuncSetAttribute((const void*)decision8_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       kTileLds + QK_DECISION8_MAX_C * kTile * 4));
+                                       kDecisionLds));
             attr.done();
         }
         hipLaunchKernelGGL(decision8_tile_kernel, dim3((unsigned)((x->rows + kTile - 1) / kTile), (unsigned)a.splits), dim3(256),
-                           (size_t)kTileLds + (size_t)C * kTile * sizeof(float), s, a);
+                           kDecisionLds, s, a);
     } else {
         hipLaunchKernelGGL(decision8_wave_kernel, dim3((unsigned)((x->rows + 31) / 32), (unsigned)a.splits), dim3(256),
                            (size_t)4 * 32 * C * sizeof(float), s, a);
     }
     QK_HIP(hipGetLastError());
-    if (a.splits > 1) {
-        hipLaunchKernelGGL(decision8_join_kernel, dim3(joins), dim3(256), 0, s, a);
+    if (a.parts) {
+        hipLaunchKernelGGL(decision8_join_kernel, joins, dim3(256), 0, s, a);
         QK_HIP(hipGetLastError());
     }
     return QK_OK;

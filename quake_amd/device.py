@@ -205,15 +205,19 @@ def pqk(rdm_x: torch.Tensor, rdm_y: Optional[torch.Tensor], gamma: float,
 _NO_GUARD = contextlib.nullcontext()
 
 
-def _on(t: torch.Tensor):
-    """Makes the tensor's GPU the current one for a launch (kernels run on the current stream of that GPU)."""
-    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _on(gpu: int):
+    """Makes a GPU the current one for a launch (kernels run on that GPU's current stream)."""
+    return _NO_GUARD if gpu == torch.cuda.current_device() else torch.cuda.device(gpu)
 
 
-def _one_device(*tensors) -> None:
-    _require_gpu(*tensors)
-    if len({t.device for t in tensors if t is not None}) > 1:
-        raise ValueError("tensors are on different GPUs")
+def _stream_on(gpu: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(gpu)
+
+
+def _same_gpu(gpu: int, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != gpu:
+            raise ValueError("device entry points need tensors in GPU memory, all on one GPU")
 
 
 class States8:
@@ -245,16 +249,19 @@ class States8:
 
     def _set(self, codes, scales, gains, dim, rows):
         self.codes, self.scales, self.gains, self.dim, self._rows = codes, scales, gains, dim, rows
+        self._gpu = gpu = codes.get_device()
+        if gpu < 0 or scales.get_device() != gpu or gains.get_device() != gpu:
+            raise ValueError("device entry points need tensors in GPU memory, all on one GPU")
+        self._at = codes.data_ptr(), scales.data_ptr(), gains.data_ptr()
 
     @classmethod
     def from_arrays(cls, codes: torch.Tensor, scales: torch.Tensor, gains: torch.Tensor, dim: int) -> "States8":
         """A store over arrays that hold written rows already (a saved store, a selection ``codes[rows], scales[rows],
         gains[rows]`` of another one's); the arrays are used, not copied."""
         code, scale = cls._layout(dim)
-        _one_device(codes, scales, gains)
-        rows = gains.shape[0] if gains.dim() == 1 else -1
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or gains.dtype != torch.float32 \
-                or codes.shape != (rows, code) or scales.shape != (rows, scale) \
+        rows = gains.numel()
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or gains.dtype is not torch.float32 \
+                or gains.shape != (rows,) or codes.shape != (rows, code) or scales.shape != (rows, scale) \
                 or not (codes.is_contiguous() and scales.is_contiguous() and gains.is_contiguous()):
             raise ValueError("need contiguous codes uint8 [rows, 128 ceil(dim / 64)], scales uint8 [rows, 4 ceil(dim / 512)], "
                              "gains float32 [rows]")
@@ -286,15 +293,16 @@ class States8:
         self._rows = 0
 
     def _struct(self, start: int = 0, rows: Optional[int] = None) -> "_lib.qk_states8":
-        rows = self._rows if rows is None else rows
-        return _lib.qk_states8(self.codes.data_ptr() + start * self.codes.shape[1],
-                               self.scales.data_ptr() + start * self.scales.shape[1], self.gains.data_ptr() + 4 * start, rows)
+        codes, scales, gains = self._at
+        if start:
+            codes, scales, gains = codes + start * self.codes.shape[1], scales + start * self.scales.shape[1], gains + 4 * start
+        return _lib.qk_states8(codes, scales, gains, self._rows if rows is None else rows)
 
     def write(self, psi: torch.Tensor, at: Optional[int] = None) -> None:
         """Quantises psi [rows, dim] (complex128 or complex64, unit column stride) behind the rows written so far, or from row
         ``at`` on (overwriting; ``at`` may be at most the number of rows written so far)."""
         psi = from_dlpack(psi)
-        _one_device(psi, self.codes)
+        _same_gpu(self._gpu, psi)
         if psi.dtype not in (torch.complex128, torch.complex64) or psi.dim() != 2 or psi.shape[1] != self.dim \
                 or (psi.shape[0] and self.dim > 1 and psi.stride(1) != 1) or psi.is_conj():
             raise ValueError("psi must be a complex128 / complex64 [rows, dim] tensor with unit column stride")
@@ -307,16 +315,16 @@ class States8:
         if ld < self.dim:
             raise ValueError("the rows of psi overlap")
         to = self._struct(at, n)
-        with _on(psi):
+        with _on(self._gpu):
             _lib.check(_lib.load().qk_states8_write_dev(_dp(psi), int(psi.dtype == torch.complex64), ld, self.dim, C.byref(to),
-                                                        _stream_ptr()))
+                                                        _stream_on(self._gpu)))
         self._rows = max(self._rows, at + n)
 
     def read(self, index: Optional[torch.Tensor] = None, dtype=torch.complex64, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The stored states q (code * scale, exact in complex64; the gain is not applied): all written rows, or the rows
         ``index`` (int64 on the GPU, any order, repeats allowed; a number outside the store gives a row of NaN)."""
         index, out = from_dlpack(index), from_dlpack(out)
-        _one_device(self.codes, index, out)
+        _same_gpu(self._gpu, index, out)
         if index is not None and (index.dtype != torch.int64 or index.dim() != 1 or not index.is_contiguous()):
             raise ValueError("index must be a contiguous int64 vector")
         n = self._rows if index is None else index.shape[0]
@@ -327,13 +335,17 @@ class States8:
         elif out.dtype not in (torch.complex64, torch.complex128) or out.shape != (n, self.dim) or not out.is_contiguous():
             raise ValueError("out must be a contiguous complex64 / complex128 [rows, dim] tensor")
         of = self._struct()
-        with _on(out):
+        with _on(self._gpu):
             _lib.check(_lib.load().qk_states8_read_dev(C.byref(of), self.dim, _dp(index), n, _dp(out),
-                                                       int(out.dtype == torch.complex64), self.dim, _stream_ptr()))
+                                                       int(out.dtype == torch.complex64), self.dim, _stream_on(self._gpu)))
         return out
 
 
 _K8_FLAGS = {torch.float32: 0, torch.float16: _lib.QK_GRAM8_F16, torch.float64: _lib.QK_GRAM8_F64}
+
+
+def _padded(entries: int) -> int:
+    return (entries + 127) & ~127
 
 
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
@@ -344,47 +356,60 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
     """Fidelity kernels of several pairs of 8-bit stores in one call (one launch for up to 24 of them), every job with its
     own rows and its own dim: the kernels of a population.  Each job: dict(A=, B=None, K=None, KT=None) with A, B
     :class:`States8`; B is None: the symmetric kernel of A with an exact unit diagonal.  K (allocated as ``dtype`` if not
-    given) and KT, the transposed copy (not for symmetric jobs): float32, float16 or float64 [len(A), len(B)] views with unit
+    given, several of them in one allocation) and KT, the transposed copy (not for symmetric jobs): float32, float16 or float64 [len(A), len(B)] views with unit
     column stride.  Returns the Ks."""
     if not jobs:
         return []
-    device = jobs[0]["A"].device
-    arr = (_lib.qk_gram8_job * len(jobs))()
-    Ks = []
-    for a, j in zip(arr, jobs):
-        A, B, K, KT = j["A"], j.get("B"), from_dlpack(j.get("K")), from_dlpack(j.get("KT"))
+    if dtype not in _K8_FLAGS:
+        raise ValueError("K must be float32, float16 or float64")
+    packed, Ks, gpu, device, flat, used = [], [], None, None, None, 0
+    for j in jobs:
+        A, B, K, KT = j["A"], j.get("B"), j.get("K"), j.get("KT")
         sym = B is None
         if sym:
             B = A
-        if not isinstance(A, States8) or not isinstance(B, States8):
+        if not isinstance(A, States8) or not (sym or isinstance(B, States8)):
             raise ValueError("A and B must be States8 stores")
-        if A.dim != B.dim:
+        if not sym and A.dim != B.dim:
             raise ValueError(f"stores of different dim: {A.dim} and {B.dim}")
-        m, n = len(A), len(B)
+        if gpu is None:
+            gpu, device = A._gpu, A.codes.device
+        if A._gpu != gpu or B._gpu != gpu:
+            raise ValueError("stores on different GPUs")
+        m, n = A._rows, B._rows
         if K is None:
-            if dtype not in _K8_FLAGS:
-                raise ValueError("K must be float32, float16 or float64")
-            K = torch.empty((m, n), dtype=dtype, device=device)
-        elif K.dtype not in _K8_FLAGS or K.shape != (m, n) or (K.numel() and ((n > 1 and K.stride(1) != 1) or (m > 1 and K.stride(0) < n))):
-            raise ValueError("K must be float32, float16 or float64 [len(A), len(B)] with unit column stride")
-        if KT is not None and (sym or KT.dtype != K.dtype or KT.shape != (n, m)
-                               or (KT.numel() and ((m > 1 and KT.stride(1) != 1) or (n > 1 and KT.stride(0) < m)))):
-            raise ValueError("KT must be of K's type, [len(B), len(A)] with unit column stride, and not for a symmetric job")
-        _require_gpu(K, KT)
-        if not A.device == B.device == K.device == device or (KT is not None and KT.device != device):
-            raise ValueError("tensors are on different GPUs")
-        a.A, a.B, a.D = A._struct(), B._struct(), A.dim
-        a.K, a.ldk = K.data_ptr(), (K.stride(0) if m > 1 and n else max(n, 1))
+            if len(jobs) == 1:
+                K = torch.empty((m, n), dtype=dtype, device=device)
+            else:                       # views of one allocation, which lives as long as any of them
+                if flat is None:
+                    flat = torch.empty(sum(_padded(len(j["A"]) * len(j["A" if j.get("B") is None else "B"])) for j in jobs
+                                           if j.get("K") is None), dtype=dtype, device=device)
+                K = flat.as_strided((m, n), (n or 1, 1), used)
+                used += _padded(m * n)
+            ldk = n or 1
+        else:
+            K = from_dlpack(K)
+            if K.dtype not in _K8_FLAGS or K.shape != (m, n) or (K.numel() and ((n > 1 and K.stride(1) != 1) or (m > 1 and K.stride(0) < n))):
+                raise ValueError("K must be float32, float16 or float64 [len(A), len(B)] with unit column stride")
+            _same_gpu(gpu, K)
+            ldk = K.stride(0) if m > 1 and n else max(n, 1)
+        kt = ldkt = 0
         if KT is not None:
-            a.KT, a.ldkt = KT.data_ptr(), (KT.stride(0) if n > 1 and m else max(m, 1))
-        a.flags = _K8_FLAGS[K.dtype] | (_lib.QK_GRAM_SYMMETRIC if sym else 0)
+            KT = from_dlpack(KT)
+            if sym or KT.dtype != K.dtype or KT.shape != (n, m) \
+                    or (KT.numel() and ((m > 1 and KT.stride(1) != 1) or (n > 1 and KT.stride(0) < m))):
+                raise ValueError("KT must be of K's type, [len(B), len(A)] with unit column stride, and not for a symmetric job")
+            _same_gpu(gpu, KT)
+            kt, ldkt = KT.data_ptr(), (KT.stride(0) if n > 1 and m else max(m, 1))
+        packed.append(_lib.GRAM8_JOB.pack(*A._at, m, *B._at, n, A.dim, K.data_ptr(), kt, ldk, ldkt,
+                                          _K8_FLAGS[K.dtype] | (_lib.QK_GRAM_SYMMETRIC if sym else 0), 0))
         Ks.append(K)
-    lib = _lib.load()
+    lib, arr = _lib.load(), b"".join(packed)
     need = C.c_size_t()
     _lib.check(lib.qk_gram8_workspace(arr, len(jobs), C.byref(need)))
-    with _on(jobs[0]["A"].codes):
+    with _on(gpu):
         ws = _workspace(need.value, device)
-        _lib.check(lib.qk_gram8_jobs_dev(arr, len(jobs), _dp(ws), need.value, _stream_ptr()))
+        _lib.check(lib.qk_gram8_jobs_dev(arr, len(jobs), _dp(ws), need.value, _stream_on(gpu)))
     return Ks
 
 
@@ -404,12 +429,12 @@ def decision8(x: States8, y: States8, coef: torch.Tensor, intercept: Optional[to
     coef, intercept, out = from_dlpack(coef), from_dlpack(intercept), from_dlpack(out)
     if not isinstance(x, States8) or not isinstance(y, States8):
         raise ValueError("x and y must be States8 stores")
-    _one_device(x.codes, y.codes, coef, intercept, out)
+    _same_gpu(x._gpu, y.codes, coef, intercept, out)
     if x.dim != y.dim:
         raise ValueError(f"stores of different dim: {x.dim} and {y.dim}")
     if coef.dim() == 1:
         coef = coef.unsqueeze(1)
-    m, n, c = len(x), len(y), coef.shape[1] if coef.dim() == 2 else 0
+    m, n, c = x._rows, y._rows, coef.shape[1] if coef.dim() == 2 else 0
     if coef.dtype != torch.float32 or coef.shape != (n, c) or not 1 <= c <= _lib.QK_DECISION8_MAX_C or (n and c > 1 and coef.stride(1) != 1):
         raise ValueError("coef must be float32 [len(y), C] with unit column stride and 1 <= C <= 64")
     if intercept is not None and (intercept.dtype != torch.float32 or intercept.shape != (c,) or not intercept.is_contiguous()):
@@ -425,10 +450,10 @@ def decision8(x: States8, y: States8, coef: torch.Tensor, intercept: Optional[to
     need = C.c_size_t()
     _lib.check(lib.qk_decision8_workspace(m, n, x.dim, c, C.byref(need)))
     sx, sy = x._struct(), y._struct()
-    with _on(x.codes):
+    with _on(x._gpu):
         ws = _workspace(need.value, x.device)
         _lib.check(lib.qk_decision8_dev(C.byref(sx), C.byref(sy), x.dim, _dp(coef), ldc, c, _dp(intercept), _dp(out), ldo, _dp(ws),
-                                        need.value, _stream_ptr()))
+                                        need.value, _stream_on(x._gpu)))
     return out
 
 
