@@ -191,10 +191,11 @@ struct Gram8JobDev {
     int32_t chunks;            // chunks per row
     int32_t sb;                // scale bytes per row
     int32_t tiles_m, tiles_n;  // tile rows and columns
-    int32_t slices;            // the row's chunks are cut into this many slices of `per` chunks
+    int32_t slices;            // the tiles behind the first `whole` are cut into this many slices of `per` chunks
     int32_t per;
     uint32_t live;             // tiles that have to be computed
-    uint32_t begin;            // items (tile x slice) of the jobs before
+    uint32_t whole;
+    uint32_t begin;            // items of the jobs before; a job's: its whole tiles, then slice by slice the others
 };
 
 struct Gram8Args {
@@ -277,6 +278,17 @@ __device__ __forceinline__ void gram8_tile(const Gram8JobDev& J, uint32_t t, uin
     ti = r0 + in % rows;
 }
 
+// Item `in` of a job -> tile t, slice (-1: the whole tile)
+__device__ __forceinline__ void gram8_part(const Gram8JobDev& J, uint32_t in, uint32_t& t, int& slice) {
+    t = in;
+    slice = -1;
+    if (in >= J.whole) {
+        const uint32_t cut = J.live - J.whole, k = in - J.whole;
+        slice = (int)(k / cut);
+        t = J.whole + (k - (uint32_t)slice * cut);
+    }
+}
+
 __device__ __forceinline__ int gram8_job(const Gram8Args& a, uint32_t item) {
     int j = 0;
     while (j + 1 < a.n_jobs && a.job[j + 1].begin <= item) ++j;
@@ -320,15 +332,16 @@ __global__ __launch_bounds__(256) void gram8_wave_kernel(Gram8Args args) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, h = lane >> 5;
     const uint32_t item = blockIdx.x;
     const Gram8JobDev& J = args.job[gram8_job(args, item)];
-    const uint32_t in = item - J.begin, slice = in / J.live, t = in - slice * J.live;
-    uint32_t ti, tj;
+    uint32_t t, ti, tj;
+    int slice;
+    gram8_part(J, item - J.begin, t, slice);
     gram8_tile(J, t, ti, tj);
     const int64_t cb = (int64_t)J.chunks * kChunkBytes;
     const int64_t ra = min((int64_t)ti * 32 + r, J.A.n - 1), rb = min((int64_t)tj * 32 + r, J.B.n - 1);
     v16f re, im;
 #pragma unroll
     for (int i = 0; i < 16; ++i) re[i] = im[i] = 0.f;
-    const int c0 = (int)slice * J.per, c1 = min(J.chunks, c0 + J.per);
+    const int c0 = max(slice, 0) * J.per, c1 = slice < 0 ? J.chunks : min(J.chunks, c0 + J.per);
     wave_product(J.A.codes + ra * cb + 16 * h, J.A.scales + ra * J.sb, J.B.codes + rb * cb + 16 * h, J.B.scales + rb * J.sb, c0 + wave,
                  c1, W, re, im);
 #pragma unroll
@@ -346,10 +359,10 @@ __global__ __launch_bounds__(256) void gram8_wave_kernel(Gram8Args args) {
             x += part[w][i][lane];
             y += part[w][16 + i][lane];
         }
-        if (J.slices == 1) {
+        if (slice < 0) {
             emit(J, (int64_t)ti * 32 + acc_row(lane, i), (int64_t)tj * 32 + r, x, y);
         } else {
-            float2* ws = (float2*)(args.ws + J.ws) + ((int64_t)t * J.slices + slice) * 1024;
+            float2* ws = (float2*)(args.ws + J.ws) + ((int64_t)(t - J.whole) * J.slices + slice) * 1024;
             ws[i * 64 + lane] = make_float2(x, y);
         }
     }
@@ -373,7 +386,7 @@ typedef __attribute__((address_space(3))) void* lptr_t;
 struct TileWork {              // what one pass of the pipeline computes; the same for the whole workgroup
     Rows8 A, B;
     int64_t row_a, row_b;
-    int chunks, sb, c0, c1;    // c0: a multiple of 8
+    int chunks, sb, c0, c1;
 };
 
 template <bool NATIVE> struct TilePipe {
@@ -400,8 +413,8 @@ template <bool NATIVE> struct TilePipe {
         for (int p = 0; p < 4; ++p) piece[p] = (((p >> 1) * 4 + 2 * h + (p & 1)) ^ ((r >> 1) & 7)) << 4;
     }
 
-    __device__ __forceinline__ void stage(int c, int to_buf) {
-        if (!(c & 7)) {
+    __device__ __forceinline__ void stage(int c, int to_buf, bool first = false) {
+        if (first || !(c & 7)) {
             next_area ^= 1;
             asm volatile("" : "+v"(scale_vo));
             __builtin_amdgcn_global_load_lds((gptr_t)(scale_src + (c >> 3) * 4 + (uint64_t)scale_vo),
@@ -432,7 +445,7 @@ template <bool NATIVE> struct TilePipe {
         const uint32_t row = (uint32_t)min((wave & 1) * 64 + lane, last);
         scale_vo = row * (uint32_t)w.sb;
         __builtin_amdgcn_global_load_lds((gptr_t)(S.gains + row0 + (uint64_t)row), (lptr_t)(lds + kGains + g * 1024 + wave * 256), 4, 0, 0);
-        stage(w.c0, to_buf);
+        stage(w.c0, to_buf, true);
     }
 
     __device__ __forceinline__ void compute(int c, v16f (&re)[2][2], v16f (&im)[2][2]) {
@@ -597,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
     extern __shared__ uint8_t lds[];
     TilePipe<NATIVE> pipe(lds);
     const int wave = pipe.wave, lane = pipe.lane, r = pipe.r, h = pipe.h;
-    struct Where { int job; uint32_t ti, tj, slice, t; } now{}, before{};      // of the tile that was opened last and the one before
+    struct Where { int job; uint32_t t, ti, tj; int slice; } now{}, before{};      // of the tile that was opened last and the one before
     auto work = [&](int k, TileWork& w) {
         uint32_t item;
         if (!gram8_item(args.total, blockIdx.x + (uint32_t)k * gridDim.x, item)) return false;
@@ -605,10 +618,10 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
         Where& p = now;
         p.job = uniform(gram8_job(args, item));
         const Gram8JobDev& J = args.job[p.job];
-        const uint32_t in = item - J.begin;
-        p.slice = uniform(in / J.live);
-        p.t = uniform(in - p.slice * J.live);
+        gram8_part(J, item - J.begin, p.t, p.slice);
         gram8_tile(J, p.t, p.ti, p.tj);
+        p.t = uniform(p.t);
+        p.slice = uniform(p.slice);
         p.ti = uniform(p.ti);
         p.tj = uniform(p.tj);
         w.A = J.A;
@@ -617,15 +630,15 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
         w.row_b = (int64_t)p.tj * kTile;
         w.chunks = J.chunks;
         w.sb = J.sb;
-        w.c0 = (int)p.slice * J.per;
-        w.c1 = min(J.chunks, w.c0 + J.per);
+        w.c0 = max(p.slice, 0) * J.per;
+        w.c1 = p.slice < 0 ? J.chunks : min(J.chunks, w.c0 + J.per);
         return true;
     };
     auto finish = [&](int, bool more, const float* gains, uint8_t* room, v16f (&re)[2][2], v16f (&im)[2][2]) {
-        const Where w = more ? before : now, p = {uniform(w.job), uniform(w.ti), uniform(w.tj), uniform(w.slice), uniform(w.t)};
+        const Where w = more ? before : now, p = {uniform(w.job), uniform(w.t), uniform(w.ti), uniform(w.tj), uniform(w.slice)};
         const Gram8JobDev& J = args.job[p.job];
-        if (J.slices > 1) {
-            float2* ws = (float2*)(args.ws + J.ws) + (((int64_t)p.t * J.slices + p.slice) * 16 + wave * 4) * 1024 + lane;
+        if (p.slice >= 0) {
+            float2* ws = (float2*)(args.ws + J.ws) + (((int64_t)(p.t - J.whole) * J.slices + p.slice) * 16 + wave * 4) * 1024 + lane;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -727,18 +740,19 @@ __global__ __launch_bounds__(256) void gram8_join_kernel(Gram8Args args) {
     uint32_t before = 0;
     int j = 0;
     for (; j + 1 < args.n_jobs; ++j) {
-        const uint32_t here = args.job[j].slices > 1 ? args.job[j].live : 0;
+        const uint32_t here = args.job[j].live - args.job[j].whole;
         if (tile < before + here) break;
         before += here;
     }
     const Gram8JobDev& J = args.job[j];
-    const uint32_t t = tile - before;
-    if (J.slices <= 1 || t >= J.live) return;
+    const uint32_t t = J.whole + (tile - before);
+    if (t >= J.live) return;
     uint32_t ti, tj;
     gram8_tile(J, t, ti, tj);
     const int in = (int)(blockIdx.x % (4 * SUB)) * 256 + threadIdx.x, sub = in >> 10, e = in & 1023, lane = e & 63, i = e >> 6;
-    const float2* ws = (const float2*)(args.ws + J.ws) + (int64_t)t * J.slices * SUB * 1024 + in;
+    const float2* ws = (const float2*)(args.ws + J.ws) + (int64_t)(t - J.whole) * J.slices * SUB * 1024 + in;
     float x = 0.f, y = 0.f;
+#pragma unroll 8
     for (int s = 0; s < J.slices; ++s) {
         const float2 v = ws[(int64_t)s * SUB * 1024];
         x += v.x;
@@ -957,11 +971,37 @@ struct Gram8Plan {
     size_t ws_floats;
 };
 
+// Workgroups that run at a time
+constexpr int64_t slots(Gram8Kind kind) { return kind == GK_WAVE ? 1024 : 512; }
+
+// Which of a job's tiles are cut into slices of their rows, and into how many: those of the last round over the chip's slots,
+// where cutting brings more than it costs.  Measured: a step (a chunk of a tile) takes 3.0 us with all slots busy (fp8 1.7;
+// 32 x 32 tiles 0.4), joining a call's slices 5 us and what writing and reading them takes at 5 TB/s.
+void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double rest, Gram8JobDev& d) {
+    const int64_t all = slots(kind), side = kind == GK_WAVE ? 32 : kTile, last = (taken + live) % all, tail = std::min(live, last);
+    const double step = kind == GK_WAVE ? 0.4 : kind == GK_TILE_NATIVE ? 1.7 : 3.0;
+    d.whole = (uint32_t)live;
+    d.slices = 1;
+    d.per = chunks;
+    if (tail == 0 || rest >= 0.5 * (double)((all - last) * chunks)) return;      // the jobs behind it fill the round
+    double best = (double)chunks * step;
+    const int most = std::min(kind == GK_WAVE ? chunks / 16 : chunks / 4, 256);
+    for (int n = 2; n <= most; ++n) {
+        const int per = (chunks + n - 1) / n;
+        if ((chunks + per - 1) / per != n) continue;
+        const double cost = (double)((tail * n + all - 1) / all) * per * step + 5.0 + (double)(tail * n * side * side * 16) / 5e6;
+        if (cost < best) {
+            best = cost;
+            d.slices = n;
+            d.per = per;
+            d.whole = (uint32_t)(live - tail);
+        }
+    }
+}
+
 int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind, Gram8Plan& p) {
     std::memset(&p, 0, sizeof(p));
     const int64_t side = kind == GK_WAVE ? 32 : kTile;
-    int64_t tiles = 0;
-    for (int k = 0; k < n; ++k) tiles += live_tiles(jobs[which[k]], side);
     int64_t items = 0;
     for (int k = 0; k < n; ++k) {
         const qk_gram8_job& j = jobs[which[k]];
@@ -978,20 +1018,18 @@ int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind
         d.tiles_m = (int32_t)((j.A.rows + side - 1) / side);
         d.tiles_n = (int32_t)((j.B.rows + side - 1) / side);
         const int64_t live = live_tiles(j, side);
-        // few tiles with long rows: slices of at least 16 chunks (four for each wave) or 8, in whole groups of 8 (a dword
-        // of scales), enough for about 1024 or 512 workgroups
-        const int64_t least = kind == GK_WAVE ? 16 : 8, want = kind == GK_WAVE ? 1024 : 512;
-        const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(d.chunks / least, want / std::max<int64_t>(tiles, 1)));
-        d.per = (int32_t)(((d.chunks + slices - 1) / slices + 7) / 8 * 8);
-        d.slices = (d.chunks + d.per - 1) / d.per;
+        // what the jobs behind this one (shorter rows) bring to the slots that its last tiles leave free, in steps
+        double rest = 0;
+        for (int l = k + 1; l < n; ++l) rest += (double)live_tiles(jobs[which[l]], side) * (double)((jobs[which[l]].D + kChunk - 1) / kChunk);
+        cut(kind, live, d.chunks, items % slots(kind), rest, d);
         if (items + live * d.slices > 0x7fffffffLL) return fail(QK_ERR_UNSUPPORTED, "qk_gram8_jobs_dev: too many tiles; split the call");
         d.live = (uint32_t)live;
         d.begin = (uint32_t)items;
-        items += live * d.slices;
-        if (d.slices > 1) {
+        items += d.whole + (live - d.whole) * d.slices;
+        if (d.whole < live) {
             d.ws = (int64_t)p.ws_floats;
-            p.ws_floats += (size_t)live * d.slices * 2 * side * side;
-            p.join_tiles += (uint32_t)live;
+            p.ws_floats += (size_t)(live - d.whole) * d.slices * 2 * side * side;
+            p.join_tiles += (uint32_t)(live - d.whole);
         }
     }
     p.args.total = (uint32_t)items;
@@ -1161,7 +1199,10 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
     return gram8_launches(jobs, n_jobs, [&](Gram8Plan& p, Gram8Kind kind) {
         p.args.ws = (float*)ws;
         const uint32_t total = p.args.total, full = total >> 9;
-        const dim3 dealt(std::min<uint32_t>(512, (full << 9) + 8 * ((total - (full << 9) + 7) >> 3)));      // two workgroups per CU
+        // two workgroups per CU that stay, or, for long rows, one for each item: the hardware then starts neighbours together, and they
+        // keep sharing rows in L2 (12000 rows: 16384 amplitudes 4.37 against 4.12 ms, 65536 20.3 against 17.3; 4096 rows of 4096
+        // amplitudes the same; 256 amplitudes 27.5 against 28.4 us)
+        const dim3 dealt(std::min<uint32_t>(p.args.job[0].chunks > 64 ? 0x7fffffffu : 512u, (full << 9) + 8 * ((total - (full << 9) + 7) >> 3)));      // two workgroups per CU
         if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, dim3(total), dim3(256), 0, s, p.args);
         else if (kind == GK_TILE) QK_TILE8(false, float);
         else if (kind == GK_TILE_F64) QK_TILE8(false, double);
