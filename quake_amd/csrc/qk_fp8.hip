@@ -296,37 +296,56 @@ __device__ __forceinline__ int gram8_job(const Gram8Args& a, uint32_t item) {
 }
 
 // re += conj(a) c, im of the same, over chunks c0, c0 + step, ... < c1 of two 32-row operands (pa, pb: this lane's rows,
-// offset by its half).  The matrix instruction sums 8 codes of either half of the wave; which 8 is free as long as both
-// operands agree, so a lane takes whole 16-byte pieces.
+// offset by its half), the next chunk's loads in flight while one is multiplied.  The matrix instruction sums 8 codes of
+// either half of the wave; which 8 is free as long as both operands agree, so a lane takes whole 16-byte pieces.
+struct WaveChunk {
+    v4u ar[2], ai[2], br[2], bi[2];
+    uint32_t ea, eb;
+};
+__device__ __forceinline__ void wave_load(WaveChunk& f, const uint8_t* pa, const uint8_t* sa, const uint8_t* pb, const uint8_t* sb, int c) {
+    const uint8_t *a = pa + (int64_t)c * kChunkBytes, *b = pb + (int64_t)c * kChunkBytes;
+    f.ea = sa[c >> 1];
+    f.eb = sb[c >> 1];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        f.ar[s] = *(const v4u*)(a + 32 * s);
+        f.ai[s] = *(const v4u*)(a + 64 + 32 * s);
+        f.br[s] = *(const v4u*)(b + 32 * s);
+        f.bi[s] = *(const v4u*)(b + 64 + 32 * s);
+    }
+}
+__device__ __forceinline__ void wave_multiply(const WaveChunk& f, v16f& re, v16f& im) {
+    const float ea = scale_value(f.ea), eb = scale_value(f.eb);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+            const v8b xr = widen8(f.ar[s][q], f.ar[s][q + 1], ea), xi = widen8(f.ai[s][q], f.ai[s][q + 1], ea);
+            const v8b yr = widen8(f.br[s][q], f.br[s][q + 1], eb), yi = widen8(f.bi[s][q], f.bi[s][q + 1], eb);
+            re = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr, yr, re, 0, 0, 0);
+            im = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr, yi, im, 0, 0, 0);
+            re = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xi, yi, re, 0, 0, 0);
+            im = __builtin_amdgcn_mfma_f32_32x32x16_bf16(negated(xi), yr, im, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);      // (widening all codes first would take twice the registers)
+        }
+}
 __device__ __forceinline__ void wave_product(const uint8_t* pa, const uint8_t* sa, const uint8_t* pb, const uint8_t* sb, int c0,
                                              int c1, int step, v16f& re, v16f& im) {
-    for (int c = c0; c < c1; c += step) {
-        const float fa = scale_value(sa[c >> 1]), fb = scale_value(sb[c >> 1]);
-        const uint8_t *a = pa + (int64_t)c * kChunkBytes, *b = pb + (int64_t)c * kChunkBytes;
-        v4u ar[2], ai[2], br[2], bi[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            ar[s] = *(const v4u*)(a + 32 * s);
-            ai[s] = *(const v4u*)(a + 64 + 32 * s);
-            br[s] = *(const v4u*)(b + 32 * s);
-            bi[s] = *(const v4u*)(b + 64 + 32 * s);
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int q = 0; q < 4; q += 2) {
-                const v8b xr = widen8(ar[s][q], ar[s][q + 1], fa), xi = widen8(ai[s][q], ai[s][q + 1], fa);
-                const v8b yr = widen8(br[s][q], br[s][q + 1], fb), yi = widen8(bi[s][q], bi[s][q + 1], fb);
-                re = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr, yr, re, 0, 0, 0);
-                re = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xi, yi, re, 0, 0, 0);
-                im = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr, yi, im, 0, 0, 0);
-                im = __builtin_amdgcn_mfma_f32_32x32x16_bf16(negated(xi), yr, im, 0, 0, 0);
-            }
+    if (c0 >= c1) return;
+    WaveChunk f, g;
+    wave_load(f, pa, sa, pb, sb, c0);
+    for (int c = c0;;) {
+        if ((c += step) < c1) wave_load(g, pa, sa, pb, sb, c);
+        wave_multiply(f, re, im);
+        if (c >= c1) return;
+        if ((c += step) < c1) wave_load(f, pa, sa, pb, sb, c);
+        wave_multiply(g, re, im);
+        if (c >= c1) return;
     }
 }
 
 // A 32 x 32 tile per workgroup, the chunks of its slice dealt to four waves, their sums joined in LDS.
-__global__ __launch_bounds__(256) void gram8_wave_kernel(Gram8Args args) {
+__global__ __launch_bounds__(256, 3) void gram8_wave_kernel(Gram8Args args) {
     constexpr int W = 4;
     __shared__ float part[W][32][64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, h = lane >> 5;
@@ -368,6 +387,144 @@ __global__ __launch_bounds__(256) void gram8_wave_kernel(Gram8Args args) {
     }
 }
 
+// ---- few rows against many ---------------------------------------------------------------------------------------------
+// Up to 32 rows of A against rows of B that are read once: memory bound.  Every wave copies whole lines of 32 rows of B (and of
+// A, from L2) into a ring of S chunks of its own in LDS, S - 1 of them on their way while one is multiplied; no wave waits for
+// another before the end.  (Loading the fragments to registers directly touches every line four times, 32 bytes of 32
+// lines per instruction: 3.96 TB/s at one row against 65536 of 4096 amplitudes.)  Pieces lie as in the 128 x 128 tiles.
+// AR: rows of A that are copied (8 or 32); those behind the last repeat it.
+typedef const __attribute__((address_space(1))) void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+template <int AR, int S> struct ThinPipe {
+    static constexpr int kBytes = 4096 + AR * kChunkBytes + 256, kLoads = 4 + AR / 8 + 1;
+    uint8_t* ring;
+    int lane, r, h;
+    uint32_t vb[4], va[AR / 8];
+    const uint8_t* scale;        // lanes 0 .. 31: of B's rows, 32 .. 63: of A's
+
+    __device__ __forceinline__ ThinPipe(uint8_t* ring_) : ring(ring_) {
+        lane = threadIdx.x & 63;
+        r = lane & 31;
+        h = lane >> 5;
+    }
+    __device__ __forceinline__ void rows(const Rows8& A, int64_t row_a, const Rows8& B, int64_t row_b, int64_t cb, int sb) {
+        const int la = (int)min((int64_t)32, A.n - row_a) - 1, lb = (int)min((int64_t)32, B.n - row_b) - 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = e * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
+            vb[e] = (uint32_t)min(row, lb) * (uint32_t)cb + piece * 16;
+            if (e < AR / 8) va[e] = (uint32_t)min(row, la) * (uint32_t)cb + piece * 16;
+        }
+        scale = h ? A.scales + (row_a + min(r, la)) * sb : B.scales + (row_b + min(r, lb)) * sb;
+    }
+    __device__ __forceinline__ void stage(const uint8_t* a, const uint8_t* b, int c, int slot) {
+        uint8_t* to = ring + slot * kBytes;
+        const int64_t at = (int64_t)c * kChunkBytes;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            __builtin_amdgcn_global_load_lds((gptr_t)(b + at + (uint64_t)vb[e]), (lptr_t)(to + e * 1024), 16, 0, 0);
+#pragma unroll
+        for (int e = 0; e < AR / 8; ++e)
+            __builtin_amdgcn_global_load_lds((gptr_t)(a + at + (uint64_t)va[e]), (lptr_t)(to + 4096 + e * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t)(scale + (c >> 3) * 4), (lptr_t)(to + 4096 + AR * kChunkBytes), 4, 0, 0);
+    }
+    // SWAP: B's rows are the accumulator's rows (else A's)
+    template <bool SWAP> __device__ __forceinline__ void multiply(int c, int slot, v16f& re, v16f& im) {
+        const uint8_t* const at = ring + slot * kBytes;
+        const int shift = (c >> 1 & 3) * 8, ra = r & (AR - 1);
+        const float eb = scale_value((*(const uint32_t*)(at + 4096 + AR * kChunkBytes + r * 4) >> shift) & 255u);
+        const float ea = scale_value((*(const uint32_t*)(at + 4096 + AR * kChunkBytes + 128 + r * 4) >> shift) & 255u);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int key = (r >> 1) & 7, keya = (ra >> 1) & 7, pr = 2 * h + s, pi = 4 + 2 * h + s;
+            const v4u br = *(const v4u*)(at + r * kChunkBytes + ((pr ^ key) << 4)), bi = *(const v4u*)(at + r * kChunkBytes + ((pi ^ key) << 4));
+            const v4u ar = *(const v4u*)(at + 4096 + ra * kChunkBytes + ((pr ^ keya) << 4)), ai = *(const v4u*)(at + 4096 + ra * kChunkBytes + ((pi ^ keya) << 4));
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+                v8b xr = widen8(ar[q], ar[q + 1], ea), xi = widen8(ai[q], ai[q + 1], ea);
+                v8b yr = widen8(br[q], br[q + 1], eb), yi = widen8(bi[q], bi[q + 1], eb);
+                if (SWAP) {
+                    const v8b tr = xr, ti = xi;
+                    xr = yr; xi = yi; yr = tr; yi = ti;
+                }
+                re = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr, yr, re, 0, 0, 0);
+                im = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr, yi, im, 0, 0, 0);
+                re = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xi, yi, re, 0, 0, 0);
+                im = __builtin_amdgcn_mfma_f32_32x32x16_bf16(negated(xi), yr, im, 0, 0, 0);
+            }
+        }
+    }
+    // re, im += over chunks c0 .. c1 - 1 of the rows a, b point at
+    template <bool SWAP> __device__ __forceinline__ void run(const uint8_t* a, const uint8_t* b, int c0, int c1, v16f& re, v16f& im) {
+#pragma unroll
+        for (int k = 0; k < S - 1; ++k)
+            if (c0 + k < c1) stage(a, b, c0 + k, k);
+        int slot = 0;
+        for (int c = c0; c < c1; ++c) {
+            const int next = slot ? slot - 1 : S - 1;      // the slot that was read in the round before
+            if (c + S - 1 < c1) stage(a, b, c + S - 1, next);
+            const int behind = min(S - 1, c1 - 1 - c);     // chunks that may still be on their way
+            if (behind == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * kLoads) : "memory");
+            else if (behind == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+            else if (behind == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            multiply<SWAP>(c, slot, re, im);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (read before the slot is filled again)
+            slot = slot + 1 == S ? 0 : slot + 1;
+        }
+    }
+};
+constexpr int kThinLds8 = 4 * 3 * ThinPipe<8, 3>::kBytes, kThinLds32 = 4 * 4 * ThinPipe<32, 4>::kBytes;
+static_assert(2 * kThinLds8 <= 160 * 1024 && kThinLds32 <= 160 * 1024 && kThinLds8 >= 4 * 32 * 64 * 4, "LDS");
+
+// K of up to 32 rows (the smaller side of a job, J.A or, if SWAP, J.B) against 32 rows of the other: the four waves split the
+// chunks of the item's slice and join their sums in LDS.
+template <int AR, bool SWAP> __global__ __launch_bounds__(256) void gram8_thin_kernel(Gram8Args args) {
+    constexpr int W = 4, S = AR == 8 ? 3 : 4;
+    extern __shared__ uint8_t lds[];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    ThinPipe<AR, S> pipe(lds + wave * S * ThinPipe<AR, S>::kBytes);
+    const int lane = pipe.lane, r = pipe.r;
+    const uint32_t item = blockIdx.x;
+    const Gram8JobDev& J = args.job[gram8_job(args, item)];
+    uint32_t t, ti, tj;
+    int slice;
+    gram8_part(J, item - J.begin, t, slice);
+    gram8_tile(J, t, ti, tj);
+    const Rows8 A = SWAP ? J.B : J.A, B = SWAP ? J.A : J.B;
+    const int64_t cb = (int64_t)J.chunks * kChunkBytes, row_a = (int64_t)(SWAP ? tj : ti) * 32, row_b = (int64_t)(SWAP ? ti : tj) * 32;
+    v16f re, im;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) re[i] = im[i] = 0.f;
+    const int c0 = max(slice, 0) * J.per, c1 = slice < 0 ? J.chunks : min(J.chunks, c0 + J.per), n = c1 - c0;
+    pipe.rows(A, row_a, B, row_b, cb, J.sb);
+    pipe.template run<SWAP>(A.codes + row_a * cb, B.codes + row_b * cb, c0 + n * wave / W, c0 + n * (wave + 1) / W, re, im);
+    __syncthreads();
+    float (*part)[32][64] = (float (*)[32][64])lds;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        part[wave][i][lane] = re[i];
+        part[wave][16 + i][lane] = im[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16 / W; ++k) {
+        const int i = wave * (16 / W) + k;
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            x += part[w][i][lane];
+            y += part[w][16 + i][lane];
+        }
+        if (slice < 0) {
+            emit(J, (int64_t)ti * 32 + acc_row(lane, i), (int64_t)tj * 32 + r, x, y);
+        } else {
+            float2* ws = (float2*)(args.ws + J.ws) + ((int64_t)(t - J.whole) * J.slices + slice) * 1024;
+            ws[i * 64 + lane] = make_float2(x, y);
+        }
+    }
+}
+
 // ---- 128 x 128 tiles ---------------------------------------------------------------------------------------------------
 // Four waves of 64 x 64 (2 x 2 matrix tiles, real and imaginary part: 128 accumulator registers), two workgroups per CU that
 // stay and walk the list of tiles.  A step is one chunk of 128 + 128 rows, 32 KiB, copied straight to LDS one step ahead of
@@ -380,8 +537,6 @@ constexpr int kScales = 2 * kStage;                         // a dword of scales
 constexpr int kGains = kScales + 2 * 2 * kTile * 4;         // the rows' gains, twice
 constexpr int kPipeLds = kGains + 2 * 2 * kTile * 4;
 typedef int v8i __attribute__((ext_vector_type(8)));
-typedef const __attribute__((address_space(1))) void* gptr_t;
-typedef __attribute__((address_space(3))) void* lptr_t;
 
 struct TileWork {              // what one pass of the pipeline computes; the same for the whole workgroup
     Rows8 A, B;
@@ -448,7 +603,9 @@ template <bool NATIVE> struct TilePipe {
         stage(w.c0, to_buf, true);
     }
 
-    __device__ __forceinline__ void compute(int c, v16f (&re)[2][2], v16f (&im)[2][2]) {
+    // One step.  STAGE: the copies of the next chunk are issued in its middle, behind the first matrix instructions (12000 rows
+    // of 16384 amplitudes, half K: 4.13 ms with the copies first, 4.03 in the middle).
+    template <bool STAGE> __device__ __forceinline__ void compute(int c, v16f (&re)[2][2], v16f (&im)[2][2]) {
         const uint8_t* base = lds + buf * kStage;
         const int shift = (c >> 1 & 3) * 8;
         uint32_t sa[2], sc[2];
@@ -478,6 +635,11 @@ template <bool NATIVE> struct TilePipe {
                     re[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ar[i].v, br[j].v, re[i][j], 0, 0, 0, ea[i], 0, eb[j]);
                     im[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ar[i].v, bi[j].v, im[i][j], 0, 0, 0, ea[i], 0, eb[j]);
                 }
+            if constexpr (STAGE) {
+                __builtin_amdgcn_sched_barrier(0);
+                stage(c + 1, buf ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             F na[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -495,6 +657,7 @@ template <bool NATIVE> struct TilePipe {
             const float eb[2] = {scale_value((sc[0] >> shift) & 255u), scale_value((sc[1] >> shift) & 255u)};
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
+                if (STAGE && s == 1) stage(c + 1, buf ^ 1);
                 v4u ar[2], ai[2], br[2], bi[2];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
@@ -553,16 +716,16 @@ template <bool NATIVE> struct TilePipe {
             const int c1 = w.c1;
             area = next_area;
             for (; c + 1 < c1; ++c) {
-                stage(c + 1, buf ^ 1);
-                compute(c, re, im);
+                compute<true>(c, re, im);
                 buf ^= 1;
+                __builtin_amdgcn_sched_barrier(0);      // (matrix instructions that sink behind the barrier would not hide it)
                 // the copies of the next chunk have landed, and every wave has read the buffer that is filled after it
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 area = (c + 1) & 7 ? area : next_area;
             }
             const bool more = work(k + 1, w);
             if (more) open(w, buf ^ 1, (k + 1) & 1);
-            compute(c, re, im);
+            compute<false>(c, re, im);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             finish(k, more, (const float*)(lds + kGains + (k & 1) * 1024), lds + buf * kStage + wave * 8192, re, im);
             if (!more) return;
@@ -777,37 +940,72 @@ struct Decision8Args {
 
 // The product is taken the other way round (B's rows times A's), so a lane holds 16 of B's rows for ONE row of A: K times the
 // coefficients is then a sum over the lane's own registers, and only the two halves of the wave have to be added.  32 rows of A
-// per workgroup; each of four waves takes every fourth tile of 32 of B's rows in the workgroup's range.
-__global__ __launch_bounds__(256) void decision8_wave_kernel(Decision8Args a) {
-    constexpr int W = 4;
-    extern __shared__ float acc[];            // [W][C][32]
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, h = lane >> 5;
+// (8 with AR = 8) per workgroup against a range of B's.  SPLIT (rows of 8 chunks or more): the four waves share every tile of 32 of
+// B's rows, each multiplies a quarter of the chunks and then finishes a quarter of the tile's rows; else every wave has a tile of
+// its own.
+template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_thin_kernel(Decision8Args a) {
+    constexpr int W = 4, R = SPLIT ? 16 / W : 16, S = 3;      // R: accumulator registers that a wave finishes
+    extern __shared__ uint8_t lds[];
+    float* const acc = (float*)(lds + W * S * ThinPipe<AR, S>::kBytes);   // [W][C][32]
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    ThinPipe<AR, S> pipe(lds + wave * S * ThinPipe<AR, S>::kBytes);
+    const int lane = pipe.lane, r = pipe.r, h = pipe.h;
     for (int k = tid; k < W * 32 * a.C; k += 256) acc[k] = 0.f;
-    __syncthreads();
-    const int64_t row0 = (int64_t)blockIdx.x * 32;
-    const int64_t cb = (int64_t)a.chunks * kChunkBytes, ra = min(row0 + r, a.A.n - 1);
-    const float ga = a.A.gains[ra];
+    const int64_t row0 = (int64_t)blockIdx.x * AR;
+    const int64_t cb = (int64_t)a.chunks * kChunkBytes;
+    const float ga = a.A.gains[min(row0 + r, a.A.n - 1)];
     const int tiles = (int)((a.B.n + 31) / 32), t1 = min(tiles, ((int)blockIdx.y + 1) * a.per);
-    for (int t = (int)blockIdx.y * a.per + wave; t < t1; t += W) {
-        const int64_t col0 = (int64_t)t * 32, rb = min(col0 + r, a.B.n - 1);
+    for (int t = (int)blockIdx.y * a.per + (SPLIT ? 0 : wave); t < t1; t += SPLIT ? 1 : W) {
+        const int64_t col0 = (int64_t)t * 32;
+        // of this lane's rows of B: gains and the first column's coefficients, on their way while the product is taken
+        float gb[R], w[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t col = min(col0 + acc_row(lane, SPLIT ? wave * R + i : i), a.B.n - 1);
+            gb[i] = a.B.gains[col];
+            w[i] = a.coef[col * a.ldc];
+        }
         v16f re, im;
 #pragma unroll
         for (int i = 0; i < 16; ++i) re[i] = im[i] = 0.f;
-        wave_product(a.B.codes + rb * cb + 16 * h, a.B.scales + rb * a.sb, a.A.codes + ra * cb + 16 * h, a.A.scales + ra * a.sb, 0, a.chunks,
-                     1, re, im);
-        float k[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int64_t col = col0 + acc_row(lane, i);
-            k[i] = col < a.B.n ? (re[i] * re[i] + im[i] * im[i]) * (ga * a.B.gains[col]) : 0.f;
-        }
-        for (int c = 0; c < a.C; ++c) {
-            float s = 0.f;
+        pipe.rows(a.A, row0, a.B, col0, cb, a.sb);
+        pipe.template run<true>(a.A.codes + row0 * cb, a.B.codes + col0 * cb, SPLIT ? a.chunks * wave / W : 0,
+                                SPLIT ? a.chunks * (wave + 1) / W : a.chunks, re, im);
+        float k[R];
+        if constexpr (SPLIT) {
+            float (*part)[32][64] = (float (*)[32][64])lds;
+            __syncthreads();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int64_t col = col0 + acc_row(lane, i);
-                if (col < a.B.n) s += k[i] * a.coef[col * a.ldc + c];
+                part[wave][i][lane] = re[i];
+                part[wave][16 + i][lane] = im[i];
             }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                float x = 0.f, y = 0.f;
+#pragma unroll
+                for (int v = 0; v < W; ++v) {
+                    x += part[v][wave * R + i][lane];
+                    y += part[v][16 + wave * R + i][lane];
+                }
+                k[i] = x * x + y * y;
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; ++i) k[i] = re[i] * re[i] + im[i] * im[i];
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) k[i] = col0 + acc_row(lane, SPLIT ? wave * R + i : i) < a.B.n ? k[i] * (ga * gb[i]) : 0.f;
+        for (int c = 0; c < a.C; ++c) {
+            if (c) {
+#pragma unroll
+                for (int i = 0; i < R; ++i) w[i] = a.coef[min(col0 + acc_row(lane, SPLIT ? wave * R + i : i), a.B.n - 1) * a.ldc + c];
+            }
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < R; ++i) s += col0 + acc_row(lane, SPLIT ? wave * R + i : i) < a.B.n ? k[i] * w[i] : 0.f;
             s += __shfl_xor(s, 32, 64);
             if (h == 0) acc[(wave * a.C + c) * 32 + r] += s;
         }
@@ -815,10 +1013,10 @@ __global__ __launch_bounds__(256) void decision8_wave_kernel(Decision8Args a) {
     __syncthreads();
     for (int k = tid; k < 32 * a.C; k += 256) {
         const int row = k & 31, c = k >> 5;
-        if (row0 + row >= a.A.n) continue;
+        if (row >= AR || row0 + row >= a.A.n) continue;
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) s += acc[w * 32 * a.C + k];
+        for (int v = 0; v < W; ++v) s += acc[v * 32 * a.C + k];
         if (a.parts == 0) a.out[(row0 + row) * a.ldo + c] = s + (a.intercept ? a.intercept[c] : 0.f);
         else a.ws[((int64_t)blockIdx.y * a.C + c) * a.stride + row0 + row] = s;
     }
@@ -874,23 +1072,34 @@ __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a)
             const int n = min(32, a.C - c0);
             for (int c = 0; c < n; ++c) coef[c * 64 + lane] = y < a.B.n ? from[c0 + c] : 0.f;
             __builtin_amdgcn_wave_barrier();
-            for (int c = 0; c < n; ++c) {
-                float s[2] = {0.f, 0.f};
+            for (int b = 0; b < n; b += 8) {
+                // eight columns at a time, the sums so far on their way while the new ones are formed
+                float* at[8];
+                float old[8];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int e = 0; e < 8; ++e) {
+                    const int c = min(b + e, n - 1);
+                    at[e] = in_lds ? sums + ((wave >> 1) * kLdsColumns + c) * kTile + xs + lane
+                                   : a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + c) * mp + row0 + xs + lane;
+                    old[e] = k ? *at[e] : 0.f;
+                }
 #pragma unroll
-                    for (int q = 0; q < 16; q += 4) {
-                        const float4 w = *(const float4*)(coef + c * 64 + i * 32 + 2 * q + 4 * h);
+                for (int e = 0; e < 8; ++e) {
+                    if (b + e >= n) break;
+                    float s[2] = {0.f, 0.f};
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            s[j] += re[i][j][q] * w.x + re[i][j][q + 1] * w.y + re[i][j][q + 2] * w.z + re[i][j][q + 3] * w.w;
-                    }
+                    for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) s[j] += __shfl_xor(s[j], 32, 64);
-                const float mine = h ? s[1] : s[0];                  // lane half h keeps the rows of matrix tile j = h
-                float* const to = in_lds ? sums + ((wave >> 1) * kLdsColumns + c) * kTile + xs + lane
-                                         : a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + c) * mp + row0 + xs + lane;
-                *to = k ? *to + mine : mine;
+                        for (int q = 0; q < 16; q += 4) {
+                            const float4 w = *(const float4*)(coef + (b + e) * 64 + i * 32 + 2 * q + 4 * h);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                s[j] += re[i][j][q] * w.x + re[i][j][q + 1] * w.y + re[i][j][q + 2] * w.z + re[i][j][q + 3] * w.w;
+                        }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) s[j] += __shfl_xor(s[j], 32, 64);
+                    *at[e] = old[e] + (h ? s[1] : s[0]);             // lane half h keeps the rows of matrix tile j = h
+                }
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -907,14 +1116,24 @@ __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a)
     }
 }
 
-// Adds the parts in order: ws[part][C][stride], parts == 0: only the intercept.
+// Adds the parts, ws[part][C][stride], in a fixed order: 16 rows per workgroup, each by 16 threads that take every 16th part.
+// parts == 0: only the intercept.
 __global__ __launch_bounds__(256) void decision8_join_kernel(Decision8Args a) {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int c = blockIdx.y;
-    if (row >= a.A.n) return;
+    __shared__ double sum[16][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.y;
+    const int64_t row = (int64_t)blockIdx.x * 16 + x;
     double s = 0.0;
-    for (int p = 0; p < a.parts; ++p) s += (double)a.ws[((int64_t)p * a.C + c) * a.stride + row];
-    a.out[row * a.ldo + c] = (float)(s + (a.intercept ? (double)a.intercept[c] : 0.0));
+    if (row < a.A.n) {
+#pragma unroll 4
+        for (int p = y; p < a.parts; p += 16) s += (double)a.ws[((int64_t)p * a.C + c) * a.stride + row];
+    }
+    sum[y][x] = s;
+    __syncthreads();
+    if (y || row >= a.A.n) return;
+    s = a.intercept ? (double)a.intercept[c] : 0.0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += sum[k][x];
+    a.out[row * a.ldo + c] = (float)s;
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
@@ -939,9 +1158,9 @@ Rows8 rows8(const qk_states8& s) { return Rows8{(const uint8_t*)s.codes, (const 
 // Which kernel takes a job.  The 128 x 128 kernel reads every row from L2 once for 128 others and needs enough tile steps to
 // fill the chip; the 32 x 32 kernel starts at once, takes few rows without waste and spreads a small job over more
 // workgroups.
-enum Gram8Kind { GK_WAVE, GK_TILE, GK_TILE_F64, GK_TILE_NATIVE, GK_KINDS };
+enum Gram8Kind { GK_WAVE, GK_THIN8, GK_THIN32, GK_THIN8_SWAP, GK_THIN32_SWAP, GK_TILE, GK_TILE_F64, GK_TILE_NATIVE, GK_KINDS };
 constexpr double g_tiles = 96, g_steps = 1024;
-std::atomic<int> g_path{0};      // development hook: 0 by rule, 1 always 32 x 32, 2 always 128 x 128
+std::atomic<int> g_path{0};      // development hook: 0 by rule, 1 always 32 x 32, 2 always 128 x 128, 3 the kernels for few rows where they can
 
 int64_t live_tiles(const qk_gram8_job& j, int64_t tile) {
     const int64_t tm = (j.A.rows + tile - 1) / tile, tn = (j.B.rows + tile - 1) / tile;
@@ -960,7 +1179,14 @@ double tiles_of(const qk_gram8_job& j) {
 // tiles, steps (tiles times chunks): of all jobs of the call
 Gram8Kind kind_of(const qk_gram8_job& j, double tiles, double steps) {
     const int path = g_path.load(std::memory_order_relaxed);
-    if (path == 1 || tiles_of(j) == 0 || (path == 0 && tiles < g_tiles && steps < g_steps)) return GK_WAVE;
+    // up to 32 rows against more than 2 MiB of codes: memory bound
+    const int64_t few = std::min(j.A.rows, j.B.rows), many = std::max(j.A.rows, j.B.rows);
+    if (!(j.flags & QK_GRAM_SYMMETRIC) && few <= 32 && code_bytes(j.D) <= (int64_t)1 << 26 &&
+        (path == 3 || (path == 0 && many * code_bytes(j.D) > (int64_t)1 << 21))) {
+        const bool swap = j.B.rows < j.A.rows;
+        return few <= 8 ? (swap ? GK_THIN8_SWAP : GK_THIN8) : (swap ? GK_THIN32_SWAP : GK_THIN32);
+    }
+    if (path == 1 || path == 3 || tiles_of(j) == 0 || (path == 0 && tiles < g_tiles && steps < g_steps)) return GK_WAVE;
     return j.flags & QK_GRAM8_F16 ? GK_TILE_NATIVE : j.flags & QK_GRAM8_F64 ? GK_TILE_F64 : GK_TILE;
 }
 
@@ -972,20 +1198,20 @@ struct Gram8Plan {
 };
 
 // Workgroups that run at a time
-constexpr int64_t slots(Gram8Kind kind) { return kind == GK_WAVE ? 1024 : 512; }
+constexpr int64_t slots(Gram8Kind kind) { return kind == GK_WAVE ? 1024 : kind == GK_THIN32 || kind == GK_THIN32_SWAP ? 256 : 512; }
 
 // Which of a job's tiles are cut into slices of their rows, and into how many: those of the last round over the chip's slots,
 // where cutting brings more than it costs.  Measured: a step (a chunk of a tile) takes 3.0 us with all slots busy (fp8 1.7;
 // 32 x 32 tiles 0.4), joining a call's slices 5 us and what writing and reading them takes at 5 TB/s.
 void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double rest, Gram8JobDev& d) {
-    const int64_t all = slots(kind), side = kind == GK_WAVE ? 32 : kTile, last = (taken + live) % all, tail = std::min(live, last);
-    const double step = kind == GK_WAVE ? 0.4 : kind == GK_TILE_NATIVE ? 1.7 : 3.0;
+    const int64_t all = slots(kind), side = kind < GK_TILE ? 32 : kTile, last = (taken + live) % all, tail = std::min(live, last);
+    const double step = kind < GK_TILE ? 0.4 : kind == GK_TILE_NATIVE ? 1.7 : 3.0;
     d.whole = (uint32_t)live;
     d.slices = 1;
     d.per = chunks;
     if (tail == 0 || rest >= 0.5 * (double)((all - last) * chunks)) return;      // the jobs behind it fill the round
     double best = (double)chunks * step;
-    const int most = std::min(kind == GK_WAVE ? chunks / 16 : chunks / 4, 256);
+    const int most = std::min(kind < GK_TILE ? chunks / 16 : chunks / 4, 256);
     for (int n = 2; n <= most; ++n) {
         const int per = (chunks + n - 1) / n;
         if ((chunks + per - 1) / per != n) continue;
@@ -1001,7 +1227,7 @@ void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double rest, G
 
 int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind, Gram8Plan& p) {
     std::memset(&p, 0, sizeof(p));
-    const int64_t side = kind == GK_WAVE ? 32 : kTile;
+    const int64_t side = kind < GK_TILE ? 32 : kTile;
     int64_t items = 0;
     for (int k = 0; k < n; ++k) {
         const qk_gram8_job& j = jobs[which[k]];
@@ -1088,9 +1314,9 @@ bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
     const double area = (double)std::max<int64_t>(M, 64) * (double)std::max<int64_t>(N, 64) / (kTile * kTile);
     const bool tile = code_bytes(D) <= (int64_t)1 << 24 &&
                       (path == 2 || (path == 0 && M > 32 && (area >= g_tiles || area * a.chunks >= g_steps)));
-    const int64_t side = tile ? kTile : 32, tm = (M + side - 1) / side, tn = (N + side - 1) / side;
+    const int64_t side = tile ? kTile : M <= 8 ? 8 : 32, tm = (M + side - 1) / side, tn = (N + (tile ? kTile : 32) - 1) / (tile ? kTile : 32);
     const int64_t want = tile ? std::max<int64_t>(1, std::min<int64_t>(tn, 512 / std::max<int64_t>(tm, 1)))
-                              : std::max<int64_t>(1, std::min<int64_t>((tn + 3) / 4, 1024 / std::max<int64_t>(tm, 1)));
+                              : std::max<int64_t>(1, std::min<int64_t>(a.chunks >= 8 ? tn : (tn + 3) / 4, 1024 / std::max<int64_t>(tm, 1)));
     a.per = (int32_t)std::max<int64_t>(1, (tn + want - 1) / want);
     a.splits = (int32_t)std::max<int64_t>(1, (tn + a.per - 1) / a.per);
     a.stride = tm * side;
@@ -1175,14 +1401,28 @@ extern "C" int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* 
     });
 }
 
-#define QK_TILE8(NATIVE, T)                                                                                         \
-    do {                                                                                                            \
-        static DeviceOnce attr;                                                                                     \
-        if (attr.pending()) {                                                                                       \
-            QK_HIP(hipFuncSetAttribute((const void*)gram8_tile_kernel<NATIVE, T>, hipFuncAttributeMaxDynamicSharedMemorySize, kPipeLds)); \
-            attr.done();                                                                                            \
-        }                                                                                                           \
-        hipLaunchKernelGGL((gram8_tile_kernel<NATIVE, T>), dealt, dim3(256), kPipeLds, s, p.args);                  \
+// A launch with more LDS than a kernel may have unasked
+template <typename K, typename A> int launch8(K kernel, dim3 grid, int lds, hipStream_t s, const A& args, DeviceOnce& once, int most) {
+    if (once.pending()) {
+        QK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, most));
+        once.done();
+    }
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, args);
+    QK_HIP(hipGetLastError());
+    return QK_OK;
+}
+#define QK_TILE8(NATIVE, T)                                                                                          \
+    do {                                                                                                             \
+        static DeviceOnce once;                                                                                      \
+        const int rc8 = launch8(gram8_tile_kernel<NATIVE, T>, dealt, kPipeLds, s, p.args, once, kPipeLds);           \
+        if (rc8) return rc8;                                                                                         \
+    } while (0)
+#define QK_THIN8(AR, SWAP)                                                                                           \
+    do {                                                                                                             \
+        static DeviceOnce once;                                                                                      \
+        constexpr int lds8 = AR == 8 ? kThinLds8 : kThinLds32;                                                       \
+        const int rc8 = launch8(gram8_thin_kernel<AR, SWAP>, dim3(total), lds8, s, p.args, once, lds8);              \
+        if (rc8) return rc8;                                                                                         \
     } while (0)
 
 extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream) {
@@ -1204,12 +1444,16 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
         // amplitudes the same; 256 amplitudes 27.5 against 28.4 us)
         const dim3 dealt(std::min<uint32_t>(p.args.job[0].chunks > 64 ? 0x7fffffffu : 512u, (full << 9) + 8 * ((total - (full << 9) + 7) >> 3)));      // two workgroups per CU
         if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, dim3(total), dim3(256), 0, s, p.args);
+        else if (kind == GK_THIN8) QK_THIN8(8, false);
+        else if (kind == GK_THIN8_SWAP) QK_THIN8(8, true);
+        else if (kind == GK_THIN32) QK_THIN8(32, false);
+        else if (kind == GK_THIN32_SWAP) QK_THIN8(32, true);
         else if (kind == GK_TILE) QK_TILE8(false, float);
         else if (kind == GK_TILE_F64) QK_TILE8(false, double);
         else QK_TILE8(true, _Float16);
         QK_HIP(hipGetLastError());
         if (p.join_tiles) {
-            if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_join_kernel<1>, dim3(p.join_tiles * 4), dim3(256), 0, s, p.args);
+            if (kind < GK_TILE) hipLaunchKernelGGL(gram8_join_kernel<1>, dim3(p.join_tiles * 4), dim3(256), 0, s, p.args);
             else hipLaunchKernelGGL(gram8_join_kernel<16>, dim3(p.join_tiles * 64), dim3(256), 0, s, p.args);
             QK_HIP(hipGetLastError());
         }
@@ -1223,7 +1467,8 @@ extern "C" int qk_gram8_set_path(const char* name) {
     if (s == "auto") g_path = 0;
     else if (s == "wave") g_path = 1;
     else if (s == "tile") g_path = 2;
-    else return fail(QK_ERR_INVALID, "qk_gram8_set_path: auto, wave or tile");
+    else if (s == "thin") g_path = 3;
+    else return fail(QK_ERR_INVALID, "qk_gram8_set_path: auto, wave, tile or thin");
     return QK_OK;
 }
 
@@ -1267,7 +1512,7 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
     a.ldo = ldo;
     const bool tile = plan_decision8(x->rows, y->rows, D, C, a);
     const hipStream_t s = (hipStream_t)stream;
-    const dim3 joins((unsigned)((x->rows + 255) / 256), (unsigned)C);
+    const dim3 joins((unsigned)((x->rows + 15) / 16), (unsigned)C);
     if (y->rows == 0) {
         a.parts = 0;
         hipLaunchKernelGGL(decision8_join_kernel, joins, dim3(256), 0, s, a);
@@ -1275,19 +1520,22 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
         return QK_OK;
     }
     if (tile) {
-        static DeviceOnce attr;
-        if (attr.pending()) {
-            QK_HIP(hipFuncSetAttribute((const void*)decision8_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       kDecisionLds));
-            attr.done();
-        }
-        hipLaunchKernelGGL(decision8_tile_kernel, dim3((unsigned)((x->rows + kTile - 1) / kTile), (unsigned)a.splits), dim3(256),
-                           kDecisionLds, s, a);
+        static DeviceOnce once;
+        rc = launch8(decision8_tile_kernel, dim3((unsigned)((x->rows + kTile - 1) / kTile), (unsigned)a.splits), kDecisionLds, s, a, once, kDecisionLds);
     } else {
-        hipLaunchKernelGGL(decision8_wave_kernel, dim3((unsigned)((x->rows + 31) / 32), (unsigned)a.splits), dim3(256),
-                           (size_t)4 * 32 * C * sizeof(float), s, a);
+        const int side = x->rows <= 8 ? 8 : 32, sums = 4 * 32 * C * (int)sizeof(float);
+        constexpr int most = 4 * 32 * QK_DECISION8_MAX_C * (int)sizeof(float), ring8 = 4 * 3 * ThinPipe<8, 3>::kBytes, ring32 = 4 * 3 * ThinPipe<32, 3>::kBytes;
+        static_assert(ring32 + most <= 160 * 1024, "LDS");
+        const dim3 grid((unsigned)((x->rows + side - 1) / side), (unsigned)a.splits);
+        static DeviceOnce once[4];
+        if (side == 8)
+            rc = a.chunks >= 8 ? launch8(decision8_thin_kernel<8, true>, grid, ring8 + sums, s, a, once[0], ring8 + most)
+                               : launch8(decision8_thin_kernel<8, false>, grid, ring8 + sums, s, a, once[1], ring8 + most);
+        else
+            rc = a.chunks >= 8 ? launch8(decision8_thin_kernel<32, true>, grid, ring32 + sums, s, a, once[2], ring32 + most)
+                               : launch8(decision8_thin_kernel<32, false>, grid, ring32 + sums, s, a, once[3], ring32 + most);
     }
-    QK_HIP(hipGetLastError());
+    if (rc) return rc;
     if (a.parts) {
         hipLaunchKernelGGL(decision8_join_kernel, joins, dim3(256), 0, s, a);
         QK_HIP(hipGetLastError());

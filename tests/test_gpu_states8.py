@@ -12,9 +12,9 @@ pytestmark = pytest.mark.gpu
 NP = {torch.float32: S8.U32, torch.float16: S8.U16, torch.float64: 0.0}
 
 
-@pytest.fixture(params=["auto", "wave", "tile"])
+@pytest.fixture(params=["auto", "wave", "tile", "thin"])
 def path(request):
-    """The kernel that takes the products: by the library's rule, always 32 x 32 tiles, always 128 x 128."""
+    """The kernel that takes the products: by the library's rule, always 32 x 32 tiles, always 128 x 128, the ones for few rows."""
     fn = _lib.load().qk_gram8_set_path
     fn.restype, fn.argtypes = C.c_int, [C.c_char_p]
     _lib.check(fn(request.param.encode()))
@@ -141,7 +141,7 @@ def test_write_appends_overwrites_and_takes_strides():
 
 # ---- kernels -------------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (2, 3, 2), (31, 33, 16), (100, 64, 16), (1, 500, 64), (32, 129, 65), (257, 1, 100), (65, 70, 128), (130, 131, 256),
-          (200, 257, 1000), (3, 129, 4096), (129, 260, 2048), (1, 40, 65536), (70, 30, 16384), (40, 300, 8192)]
+          (200, 257, 1000), (3, 129, 4096), (129, 260, 2048), (1, 40, 65536), (70, 30, 16384), (40, 300, 8192), (8, 70, 300), (9, 33, 1025), (300, 2, 640), (65, 32, 100), (500, 5, 2048)]
 
 
 @pytest.mark.parametrize("dtype", list(NP))
@@ -248,7 +248,7 @@ def check_decision(out, x, y, coef, intercept):
 
 @pytest.mark.parametrize("M,N,D,C", [(1, 1, 2, 1), (1, 1000, 1024, 1), (1, 33, 65536, 3), (33, 31, 16, 2), (100, 100, 16, 1), (257, 300, 200, 45),
                                      (129, 1000, 64, 64), (500, 700, 1024, 1), (1, 5000, 256, 10), (64, 128, 128, 33), (1300, 400, 512, 7),
-                                     (2, 257, 4096, 5), (40, 2000, 100, 16)])
+                                     (2, 257, 4096, 5), (40, 2000, 100, 16), (8, 40, 1000, 64), (9, 300, 513, 2), (30, 65, 64, 64), (3, 2000, 16384, 4)])
 def test_decision8(M, N, D, C, path):
     rng = np.random.default_rng(M + N + D + C)
     x, y = fill(S8.states(rng, M, D, "product")), fill(S8.states(rng, N, D, "spread"))
