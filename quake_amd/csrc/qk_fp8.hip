@@ -64,8 +64,28 @@ template <typename T> struct Pair;
 template <> struct Pair<double> { typedef double2 type; };
 template <> struct Pair<float> { typedef float2 type; };
 
-// One half-wave (32 lanes) holds one block: lane i has amplitudes i, i + 32, i + 64, i + 96 (coalesced loads).  WPR waves
-// work on one row and its sums meet in LDS.
+// Largest of 32 lanes, in all of them
+__device__ __forceinline__ float half_max(float v) {
+#define QK_MAX_DPP(CTRL) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)))
+    QK_MAX_DPP(0xB1);      // neighbours in pairs,
+    QK_MAX_DPP(0x4E);      // pairs in fours,
+    QK_MAX_DPP(0x141);     // fours in eights (mirrored),
+    QK_MAX_DPP(0x140);     // eights in sixteens (mirrored)
+#undef QK_MAX_DPP
+    return fmaxf(v, __shfl_xor(v, 16, 64));
+}
+
+// Four lanes of a quad, byte k of lane l -> byte l of lane k
+__device__ __forceinline__ uint32_t quad_transpose(uint32_t v, int lane) {
+    const uint32_t x = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false);
+    v = __builtin_amdgcn_perm(x, v, lane & 1 ? 0x03070105u : 0x06020400u);      // bytes 0 .. 3: own, 4 .. 7: the neighbour's
+    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false);
+    return __builtin_amdgcn_perm(y, v, lane & 2 ? 0x03020706u : 0x05040100u);
+}
+
+// One half-wave (32 lanes) holds one block: lane i has amplitudes i, i + 32, i + 64, i + 96 (coalesced loads, the next
+// block's in flight while one is rounded) and, after a transpose in its quad, stores the codes of four neighbours at once.  WPR
+// waves work on one row and its sums meet in LDS.
 template <typename T, int WPR>
 __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void states8_write_kernel(const void* psi_, int64_t N, int64_t D, int64_t ld,
                                                                                 uint8_t* codes, uint8_t* scales, float* gains) {
@@ -82,23 +102,28 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void states8_write_kernel
         const P* src = (const P*)psi_ + row * ld;
         uint8_t* dst = codes + row * cb;
         uint8_t* sc = scales + row * sb;
+        P v[4];
+        auto load = [&](int64_t b) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t at = b * kBlock + 32 * k + i;
+                v[k].x = v[k].y = 0;
+                if (at < D) v[k] = src[at];
+            }
+        };
+        load(2 * sub + half);
         for (int64_t b0 = 2 * sub; b0 < sb; b0 += 2 * WPR) {
             const int64_t b = b0 + half;
             float re[4], im[4], top = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int64_t at = b * kBlock + 32 * k + i;
-                P v;
-                v.x = v.y = 0;
-                if (at < D) v = src[at];
-                norm += (double)v.x * (double)v.x + (double)v.y * (double)v.y;
-                re[k] = to_f32_odd(v.x);
-                im[k] = to_f32_odd(v.y);
+                norm += (double)v[k].x * (double)v[k].x + (double)v[k].y * (double)v[k].y;
+                re[k] = to_f32_odd(v[k].x);
+                im[k] = to_f32_odd(v[k].y);
                 top = fmaxf(top, fmaxf(fabsf(re[k]), fabsf(im[k])));      // (fmax drops NaN)
             }
-#pragma unroll
-            for (int m = 16; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 32));
-            const int e = scale_exponent(top);
+            if (b0 + 2 * WPR < sb) load(b + 2 * WPR);
+            const int e = scale_exponent(half_max(top));
             uint32_t wr = 0, wi = 0;      // byte k: the code of amplitude 32 k + i
             float sq = 0.f;
 #pragma unroll
@@ -112,16 +137,15 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void states8_write_kernel
                 sq += qa * qa + qc * qc;
             }
             kept += ldexp((double)sq, 2 * e);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int64_t at = b * kBlock + 32 * k + i;
-                const int64_t o = (at >> 6) * kChunkBytes + (at & 63);
-                if (o < cb) {
-                    dst[o] = (uint8_t)(wr >> (8 * k));
-                    dst[o + kChunk] = (uint8_t)(wi >> (8 * k));
-                }
+            wr = quad_transpose(wr, lane);
+            wi = quad_transpose(wi, lane);
+            const int64_t at = b * kBlock + 32 * (i & 3) + (i & ~3);      // four amplitudes from here on
+            const int64_t o = (at >> 6) * kChunkBytes + (at & 63);
+            if (o < cb) {
+                *(uint32_t*)(dst + o) = wr;
+                *(uint32_t*)(dst + o + kChunk) = wi;
             }
-            if (i == 0 && b < sb) sc[b] = (uint8_t)(b < blocks ? e + 127 : 127);
+            if (i == 0) sc[b] = (uint8_t)(b < blocks ? e + 127 : 127);
         }
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) {
@@ -145,31 +169,105 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void states8_write_kernel
 }
 
 // ---- read --------------------------------------------------------------------------------------------------------------
-// Two amplitudes per thread.  A row number outside 0 .. of - 1 gives a row of NaN.
-template <typename T>
+// Rows of 512 amplitudes or more: a wave takes 512 of them, whose codes are 1024 bytes in a row and whose scales are one
+// dword: one load of 16 bytes per lane, through LDS to pairs of amplitudes, four stores of whole lines.  A row number outside
+// 0 .. of - 1 gives a row of NaN.  VEC: rows of psi start on 16 bytes.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void states8_read_long_kernel(const uint8_t* codes, const uint8_t* scales, const int64_t* index,
+                                                                int64_t of, uint32_t items, int64_t D, void* out_, int64_t ldo,
+                                                                uint32_t segments) {
+    typedef typename Pair<T>::type P;
+    __shared__ uint4 room[4][64];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t item = blockIdx.x * 4 + wave;
+    if (item >= items) return;
+    const int64_t cb = (D + kChunk - 1) / kChunk * kChunkBytes, sb = ((D + kBlock - 1) / kBlock + 3) / 4 * 4;
+    const uint32_t n = item / segments, seg = item - n * segments;
+    const int64_t row = index ? index[n] : (int64_t)n;
+    const bool there = row >= 0 && row < of;
+    uint4 u = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+    uint32_t e4 = 0x7f7f7f7fu;
+    if (there) {
+        const int64_t o = (int64_t)seg * 1024 + lane * 16;
+        if (o < cb) u = *(const uint4*)(codes + row * cb + o);
+        e4 = *(const uint32_t*)(scales + row * sb + seg * 4);
+    }
+    room[wave][lane] = u;
+    __builtin_amdgcn_wave_barrier();      // (a wave's LDS accesses stay in order)
+    const uint8_t* const from = (const uint8_t*)room[wave];
+    P* const out = (P*)out_ + (int64_t)n * ldo + (int64_t)seg * 512;
+    if constexpr (sizeof(T) == 8) {      // 16 bytes are one amplitude
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int at = k * 64 + lane, e = (int)((e4 >> (8 * (k >> 1))) & 255u) - 127;
+            const int r = from[k * kChunkBytes + lane], s = from[k * kChunkBytes + kChunk + lane];
+            P v;
+            v.x = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(r, 0), e);
+            v.y = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(s, 0), e);
+            if (at < D - (int64_t)seg * 512) out[at] = v;
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int at = k * 128 + lane * 2, b = (at >> 6) * kChunkBytes + (at & 63), e = (int)((e4 >> (8 * k)) & 255u) - 127;
+        const int r = *(const uint16_t*)(from + b), s = *(const uint16_t*)(from + b + kChunk);
+        P v[2];
+        v[0].x = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(r, 0), e);
+        v[1].x = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(r, 1), e);
+        v[0].y = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(s, 0), e);
+        v[1].y = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(s, 1), e);
+        const int64_t left = D - (int64_t)seg * 512 - at;
+        if (VEC && sizeof(T) == 4 && left > 1) *(float4*)(out + at) = make_float4((float)v[0].x, (float)v[0].y, (float)v[1].x, (float)v[1].y);
+        else {
+            if (left > 0) out[at] = v[0];
+            if (left > 1) out[at + 1] = v[1];
+        }
+    }
+}
+
+// Shorter rows: a workgroup reads 2048 amplitudes (pairs of them, four pairs per thread, their loads all in flight) of as many whole rows as
+// that holds.
+constexpr int kReadPairs = 1024;
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void states8_read_kernel(const uint8_t* codes, const uint8_t* scales, const int64_t* index,
-                                                           int64_t of, int64_t N, int64_t D, void* out_, int64_t ldo) {
+                                                           int64_t of, int64_t N, int64_t D, void* out_, int64_t ldo, uint32_t rows) {
     typedef typename Pair<T>::type P;
     const int64_t cb = (D + kChunk - 1) / kChunk * kChunkBytes, sb = ((D + kBlock - 1) / kBlock + 3) / 4 * 4;
-    const int64_t per = (D + 1) / 2;
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < N * per; t += (int64_t)gridDim.x * 256) {
-        const int64_t n = t / per, at = 2 * (t - n * per);
-        const int64_t row = index ? index[n] : n;
-        P* out = (P*)out_ + n * ldo + at;
+    const uint32_t per = (uint32_t)((D + 1) / 2);
+    int64_t n[4], at[4], row[4];
+    int r[4], s[4], e[4];
+    bool live[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t p = k * 256 + threadIdx.x, in = p / per;
+        n[k] = (int64_t)blockIdx.x * rows + in;
+        at[k] = 2 * (int64_t)(p - in * per);
+        live[k] = in < rows && n[k] < N;
+        row[k] = live[k] ? (index ? index[n[k]] : n[k]) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const bool there = row[k] >= 0 && row[k] < of;
+        const uint8_t* c = codes + (there ? row[k] * cb + (at[k] >> 6) * kChunkBytes + (at[k] & 63) : 0);
+        e[k] = there ? (int)scales[row[k] * sb + (at[k] >> 7)] - 127 : 0;
+        r[k] = there ? *(const uint16_t*)c : 0x7f7f;
+        s[k] = there ? *(const uint16_t*)(c + kChunk) : 0x7f7f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (!live[k]) continue;
+        P* out = (P*)out_ + n[k] * ldo + at[k];
         P v[2];
-        if (row < 0 || row >= of) {
-            v[0].x = v[0].y = v[1].x = v[1].y = (T)__builtin_nanf("");
-        } else {
-            const uint8_t* c = codes + row * cb + (at >> 6) * kChunkBytes + (at & 63);
-            const int e = (int)scales[row * sb + (at >> 7)] - 127;
-            const int r = *(const uint16_t*)c, s = *(const uint16_t*)(c + kChunk);
-            v[0].x = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(r, 0), e);
-            v[1].x = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(r, 1), e);
-            v[0].y = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(s, 0), e);
-            v[1].y = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(s, 1), e);
+        v[0].x = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(r[k], 0), e[k]);
+        v[1].x = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(r[k], 1), e[k]);
+        v[0].y = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(s[k], 0), e[k]);
+        v[1].y = (T)ldexpf(__builtin_amdgcn_cvt_f32_fp8(s[k], 1), e[k]);
+        if (VEC && sizeof(T) == 4 && at[k] + 1 < D) *(float4*)out = make_float4((float)v[0].x, (float)v[0].y, (float)v[1].x, (float)v[1].y);
+        else {
+            out[0] = v[0];
+            if (at[k] + 1 < D) out[1] = v[1];
         }
-        out[0] = v[0];
-        if (at + 1 < D) out[1] = v[1];
     }
 }
 
@@ -1027,6 +1125,7 @@ template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_t
 // every lane adds to entries that no other lane touches.  A wave brings the coefficients of its 64 rows of B through its part of the free buffer,
 // [32 columns][64]; a lane reads four at once, the same for its whole half.
 constexpr int kLdsColumns = 8;
+constexpr int kMatrixColumns = 12;      // from here on FP32 matrix instructions for 32 columns (4096 clocks a tile and wave) beat 340 a column
 constexpr int kDecisionLds = kPipeLds + 2 * kLdsColumns * kTile * 4;
 static_assert(2 * kDecisionLds <= 160 * 1024, "two workgroups per CU");
 
@@ -1070,6 +1169,43 @@ __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a)
             }
         for (int c0 = 0; c0 < a.C; c0 += 32) {
             const int n = min(32, a.C - c0);
+            if (n >= kMatrixColumns) {
+                // out^T += coef^T K^T, two rows of B at a time: a register of K is the right operand as it is
+#pragma unroll 16
+                for (int e = 0; e < 32; ++e) {
+                    const int row = e * 2 + h;
+                    const int64_t yy = (int64_t)(t0 + k) * kTile + ys + row;
+                    coef[row * 32 + r] = r < n && yy < a.B.n ? a.coef[yy * a.ldc + c0 + r] : 0.f;
+                }
+                float* const at = a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + 4 * h) * mp + row0 + xs + r;
+                v16f sum[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const int c = 8 * (q >> 2) + (q & 3);
+                        sum[j][q] = k && c + 4 * h < n ? at[c * mp + j * 32] : 0.f;
+                    }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const float w = coef[(i * 32 + 8 * (q >> 2) + 4 * h + (q & 3)) * 32 + r];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) sum[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, re[i][j][q], sum[j], 0, 0, 0);
+                    }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const int c = 8 * (q >> 2) + (q & 3);
+                        if (c + 4 * h < n) at[c * mp + j * 32] = sum[j][q];
+                    }
+                __builtin_amdgcn_wave_barrier();
+                continue;
+            }
+#pragma unroll 4
             for (int c = 0; c < n; ++c) coef[c * 64 + lane] = y < a.B.n ? from[c0 + c] : 0.f;
             __builtin_amdgcn_wave_barrier();
             for (int b = 0; b < n; b += 8) {
@@ -1179,10 +1315,10 @@ double tiles_of(const qk_gram8_job& j) {
 // tiles, steps (tiles times chunks): of all jobs of the call
 Gram8Kind kind_of(const qk_gram8_job& j, double tiles, double steps) {
     const int path = g_path.load(std::memory_order_relaxed);
-    // up to 32 rows against more than 2 MiB of codes: memory bound
+    // up to 32 rows against more than 2 MiB of codes, in rows of 16 chunks or more: memory bound
     const int64_t few = std::min(j.A.rows, j.B.rows), many = std::max(j.A.rows, j.B.rows);
     if (!(j.flags & QK_GRAM_SYMMETRIC) && few <= 32 && code_bytes(j.D) <= (int64_t)1 << 26 &&
-        (path == 3 || (path == 0 && many * code_bytes(j.D) > (int64_t)1 << 21))) {
+        (path == 3 || (path == 0 && j.D > 960 && many * code_bytes(j.D) > (int64_t)1 << 21))) {
         const bool swap = j.B.rows < j.A.rows;
         return few <= 8 ? (swap ? GK_THIN8_SWAP : GK_THIN8) : (swap ? GK_THIN32_SWAP : GK_THIN32);
     }
@@ -1379,13 +1515,24 @@ extern "C" int qk_states8_read_dev(const qk_states8* from, int64_t D, const int6
     if (!index && N > from->rows) return fail(QK_ERR_INVALID, std::string(who) + ": more rows than the store holds");
     if (ldpsi < D) return fail(QK_ERR_INVALID, std::string(who) + ": row stride smaller than D");
     if ((uintptr_t)psi & (f32 ? 7 : 15)) return fail(QK_ERR_INVALID, std::string(who) + ": states need the alignment of their type");
-    const int64_t work = N * ((D + 1) / 2);
-    const unsigned grid = (unsigned)std::min<int64_t>((work + 255) / 256, 1 << 20);
+    const bool longer = D >= 512;
+    const int64_t rows = std::max<int64_t>(1, kReadPairs / ((D + 1) / 2)), segments = (D + 511) / 512;
+    const int64_t grid = longer ? (N * segments + 3) / 4 : (N + rows - 1) / rows;
+    if (grid > 0x1fffffffLL) return fail(QK_ERR_UNSUPPORTED, std::string(who) + ": too many amplitudes; split the call");
     const uint8_t *codes = (const uint8_t*)from->codes, *scales = (const uint8_t*)from->scales;
-    if (f32)
-        hipLaunchKernelGGL(states8_read_kernel<float>, dim3(grid), dim3(256), 0, (hipStream_t)stream, codes, scales, index, from->rows, N, D, psi, ldpsi);
-    else
-        hipLaunchKernelGGL(states8_read_kernel<double>, dim3(grid), dim3(256), 0, (hipStream_t)stream, codes, scales, index, from->rows, N, D, psi, ldpsi);
+    const bool vec = !((uintptr_t)psi & 15) && (ldpsi * (f32 ? 8 : 16)) % 16 == 0;
+    const dim3 g((unsigned)grid), b(256);
+    const hipStream_t s = (hipStream_t)stream;
+#define QK_READ8(T, VEC)                                                                                                             \
+    if (longer)                                                                                                                      \
+        hipLaunchKernelGGL((states8_read_long_kernel<T, VEC>), g, b, 0, s, codes, scales, index, from->rows, (uint32_t)(N * segments), D, \
+                           psi, ldpsi, (uint32_t)segments);                                                                          \
+    else                                                                                                                             \
+        hipLaunchKernelGGL((states8_read_kernel<T, VEC>), g, b, 0, s, codes, scales, index, from->rows, N, D, psi, ldpsi, (uint32_t)rows)
+    if (!f32) { QK_READ8(double, true); }
+    else if (vec) { QK_READ8(float, true); }
+    else { QK_READ8(float, false); }
+#undef QK_READ8
     QK_HIP(hipGetLastError());
     return QK_OK;
 }
