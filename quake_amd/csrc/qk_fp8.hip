@@ -794,10 +794,15 @@ template <bool NATIVE> struct TilePipe {
         }
     }
 
-    // work(k, w): the k-th piece of this workgroup's work, false behind the last.  finish(k, more, gains, room, re, im): more: the next
+    // work(k, w): the k-th piece of this workgroup's work, false behind the last.  finish(k, more, gains, room, side, re, im): more: the next
     // one is open; room: 8 KiB of LDS for this wave, the buffer of the last chunk.  STORES: finish issues at least 63 memory
-    // instructions.
-    template <bool STORES, typename Work, typename Finish> __device__ __forceinline__ void run(Work work, Finish finish) {
+    // instructions.  ASIDE: instead of the next tile's first chunk, aside(k, buffer) fills the free buffer while the last chunk is
+    // multiplied, and finish finds it there.
+    struct Nothing {
+        __device__ void operator()(int, uint8_t*) const {}
+    };
+    template <bool STORES, bool ASIDE = false, typename Work, typename Finish, typename Aside = Nothing>
+    __device__ __forceinline__ void run(Work work, Finish finish, Aside aside = Aside()) {
         TileWork w;
         if (!work(0, w)) return;
         open(w, 0, 0);
@@ -822,12 +827,18 @@ template <bool NATIVE> struct TilePipe {
                 area = (c + 1) & 7 ? area : next_area;
             }
             const bool more = work(k + 1, w);
-            if (more) open(w, buf ^ 1, (k + 1) & 1);
+            if (ASIDE) aside(k, lds + (buf ^ 1) * kStage);
+            else if (more) open(w, buf ^ 1, (k + 1) & 1);
             compute<false>(c, re, im);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            finish(k, more, (const float*)(lds + kGains + (k & 1) * 1024), lds + buf * kStage + wave * 8192, re, im);
+            if constexpr (ASIDE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            finish(k, more, (const float*)(lds + kGains + (k & 1) * 1024), lds + buf * kStage + wave * 8192, lds + (buf ^ 1) * kStage, re, im);
             if (!more) return;
             buf ^= 1;
+            if constexpr (ASIDE) {
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                open(w, buf, (k + 1) & 1);
+            }
             // memory instructions end in order: behind a tile's stores it is enough that all but the youngest 63 have
             if constexpr (STORES) asm volatile("s_waitcnt vmcnt(63) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -895,7 +906,7 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
         w.c1 = p.slice < 0 ? J.chunks : min(J.chunks, w.c0 + J.per);
         return true;
     };
-    auto finish = [&](int, bool more, const float* gains, uint8_t* room, v16f (&re)[2][2], v16f (&im)[2][2]) {
+    auto finish = [&](int, bool more, const float* gains, uint8_t* room, const uint8_t* side, v16f (&re)[2][2], v16f (&im)[2][2]) {
         const Where w = more ? before : now, p = {uniform(w.job), uniform(w.t), uniform(w.ti), uniform(w.tj), uniform(w.slice)};
         const Gram8JobDev& J = args.job[p.job];
         if (p.slice >= 0) {
@@ -1121,22 +1132,24 @@ template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_t
 }
 
 // The same over 128 x 128 tiles: a workgroup keeps 128 rows of A and walks B's tiles of its range.  Each of the two waves that
-// share rows of A keeps its own sums of the C columns: in LDS up to eight columns, in the workspace (which stays in L2) above, where
-// every lane adds to entries that no other lane touches.  A wave brings the coefficients of its 64 rows of B through its part of the free buffer,
-// [32 columns][64]; a lane reads four at once, the same for its whole half.
+// share rows of A keeps its own sums of the C columns.
+// Up to eight columns: sums in LDS, the coefficients of a wave's 64 rows of B through its part of the free buffer, [column][64]; a
+// lane reads four at once, the same for its whole half, and its part of K stays in its registers.
+// MANY: out^T += coef^T K^T on FP32 matrix instructions, 32 columns at a time: a register of K is the right operand as it is.  The
+// coefficients of the tile come to the free buffer, [128][C], while the last chunk is multiplied; the sums wait in the workspace
+// (which stays in L2), where every lane adds to entries that no other lane touches.
 constexpr int kLdsColumns = 8;
-constexpr int kMatrixColumns = 12;      // from here on FP32 matrix instructions for 32 columns (4096 clocks a tile and wave) beat 340 a column
 constexpr int kDecisionLds = kPipeLds + 2 * kLdsColumns * kTile * 4;
 static_assert(2 * kDecisionLds <= 160 * 1024, "two workgroups per CU");
+static_assert(QK_DECISION8_MAX_C * kTile * 4 <= kStage, "a tile's coefficients fit a buffer");
 
-__global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a) {
+template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a) {
     extern __shared__ uint8_t lds[];
     TilePipe<false> pipe(lds);
     const int tid = threadIdx.x, wave = pipe.wave, lane = pipe.lane, r = pipe.r, h = pipe.h;
     const int xs = (wave & 1) * 64, ys = (wave >> 1) * 64;
     const int64_t row0 = (int64_t)blockIdx.x * kTile, mp = (int64_t)gridDim.x * kTile;
     float* const sums = (float*)(lds + kPipeLds);
-    const bool in_lds = a.C <= kLdsColumns;
     const int tiles = (int)((a.B.n + kTile - 1) / kTile), t0 = (int)blockIdx.y * a.per, t1 = min(tiles, t0 + a.per);
     auto work = [&](int k, TileWork& w) {
         if (t0 + k >= t1) return false;
@@ -1150,11 +1163,10 @@ __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a)
         w.c1 = a.chunks;
         return true;
     };
-    auto finish = [&](int k, bool, const float* gains, uint8_t* room, v16f (&re)[2][2], v16f (&im)[2][2]) {
-        float* const coef = (float*)room;
-        const int64_t y = (int64_t)(t0 + k) * kTile + ys + lane;
-        const float* from = a.coef + min(y, a.B.n - 1) * a.ldc;
+    // re <- K of this wave's 64 x 64, 0 behind B's last row
+    auto kernel = [&](int k, const float* gains, v16f (&re)[2][2], v16f (&im)[2][2]) {
         const float gx[2] = {gains[kTile + xs + r], gains[kTile + xs + 32 + r]};
+        const int left = (int)min((int64_t)64, a.B.n - (int64_t)(t0 + k) * kTile - ys) - 4 * h;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1164,91 +1176,99 @@ __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        re[i][j][q + e] = (re[i][j][q + e] * re[i][j][q + e] + im[i][j][q + e] * im[i][j][q + e]) * (gx[j] * g[e]);
+                    for (int j = 0; j < 2; ++j) {
+                        const float v = (re[i][j][q + e] * re[i][j][q + e] + im[i][j][q + e] * im[i][j][q + e]) * (gx[j] * g[e]);
+                        re[i][j][q + e] = i * 32 + 2 * q + e < left ? v : 0.f;
+                    }
             }
-        for (int c0 = 0; c0 < a.C; c0 += 32) {
-            const int n = min(32, a.C - c0);
-            if (n >= kMatrixColumns) {
-                // out^T += coef^T K^T, two rows of B at a time: a register of K is the right operand as it is
-#pragma unroll 16
-                for (int e = 0; e < 32; ++e) {
-                    const int row = e * 2 + h;
-                    const int64_t yy = (int64_t)(t0 + k) * kTile + ys + row;
-                    coef[row * 32 + r] = r < n && yy < a.B.n ? a.coef[yy * a.ldc + c0 + r] : 0.f;
+    };
+    if constexpr (MANY) {
+        auto aside = [&](int k, uint8_t* to) {
+            // element n of the tile's [128][C]: rows behind the last repeat it (their K is 0)
+            const int64_t y0 = (int64_t)(t0 + k) * kTile;
+            const int last = (int)min((int64_t)kTile, a.B.n - y0) - 1, total = kTile * a.C, dr = 256 / a.C, dc = 256 - dr * a.C;
+            int row = tid / a.C, c = tid - row * a.C;
+            for (int n = 0; n < total; n += 256) {      // (the last round may run over: the buffer has the room, the row is repeated)
+                __builtin_amdgcn_global_load_lds((gptr_t)(a.coef + (y0 + min(row, last)) * a.ldc + c), (lptr_t)(to + n * 4 + wave * 256), 4, 0, 0);
+                row += dr;
+                c += dc;
+                if (c >= a.C) {
+                    c -= a.C;
+                    ++row;
                 }
+            }
+        };
+        auto finish = [&](int k, bool, const float* gains, uint8_t*, const uint8_t* side, v16f (&re)[2][2], v16f (&im)[2][2]) {
+            kernel(k, gains, re, im);
+            for (int c0 = 0; c0 < a.C; c0 += 32) {
+                const int n = a.C - c0 - 4 * h;
                 float* const at = a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + 4 * h) * mp + row0 + xs + r;
+                float old[2][16];
                 v16f sum[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int q = 0; q < 16; ++q)
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
+                    for (int j = 0; j < 2; ++j) {
                         const int c = 8 * (q >> 2) + (q & 3);
-                        sum[j][q] = k && c + 4 * h < n ? at[c * mp + j * 32] : 0.f;
+                        old[j][q] = 0.f;
+                        if (k && c < n) old[j][q] = at[c * mp + j * 32];
+                        sum[j][q] = 0.f;
                     }
-                __builtin_amdgcn_wave_barrier();
+                const float* const coef = (const float*)side + min(c0 + r, a.C - 1) + (ys + 4 * h) * a.C;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int q = 0; q < 16; ++q) {
-                        const float w = coef[(i * 32 + 8 * (q >> 2) + 4 * h + (q & 3)) * 32 + r];
+                        const float w = coef[(i * 32 + 8 * (q >> 2) + (q & 3)) * a.C];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) sum[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, re[i][j][q], sum[j], 0, 0, 0);
                     }
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int q = 0; q < 16; ++q)
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
+                    for (int j = 0; j < 2; ++j) {
                         const int c = 8 * (q >> 2) + (q & 3);
-                        if (c + 4 * h < n) at[c * mp + j * 32] = sum[j][q];
+                        if (c < n) at[c * mp + j * 32] = old[j][q] + sum[j][q];
                     }
-                __builtin_amdgcn_wave_barrier();
-                continue;
             }
+        };
+        pipe.run<false, true>(work, finish, aside);
+    } else {
+        auto finish = [&](int k, bool, const float* gains, uint8_t* room, const uint8_t*, v16f (&re)[2][2], v16f (&im)[2][2]) {
+            float* const coef = (float*)room;
+            const int64_t y = min((int64_t)(t0 + k) * kTile + ys + lane, a.B.n - 1);
 #pragma unroll 4
-            for (int c = 0; c < n; ++c) coef[c * 64 + lane] = y < a.B.n ? from[c0 + c] : 0.f;
+            for (int c = 0; c < a.C; ++c) coef[c * 64 + lane] = a.coef[y * a.ldc + c];
+            kernel(k, gains, re, im);
             __builtin_amdgcn_wave_barrier();
-            for (int b = 0; b < n; b += 8) {
-                // eight columns at a time, the sums so far on their way while the new ones are formed
-                float* at[8];
-                float old[8];
+            for (int c = 0; c < a.C; ++c) {
+                float s[2] = {0.f, 0.f};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int c = min(b + e, n - 1);
-                    at[e] = in_lds ? sums + ((wave >> 1) * kLdsColumns + c) * kTile + xs + lane
-                                   : a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + c) * mp + row0 + xs + lane;
-                    old[e] = k ? *at[e] : 0.f;
-                }
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (b + e >= n) break;
-                    float s[2] = {0.f, 0.f};
+                    for (int q = 0; q < 16; q += 4) {
+                        const float4 w = *(const float4*)(coef + c * 64 + i * 32 + 2 * q + 4 * h);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                        for (int j = 0; j < 2; ++j)
+                            s[j] += re[i][j][q] * w.x + re[i][j][q + 1] * w.y + re[i][j][q + 2] * w.z + re[i][j][q + 3] * w.w;
+                    }
 #pragma unroll
-                        for (int q = 0; q < 16; q += 4) {
-                            const float4 w = *(const float4*)(coef + (b + e) * 64 + i * 32 + 2 * q + 4 * h);
-#pragma unroll
-                            for (int j = 0; j < 2; ++j)
-                                s[j] += re[i][j][q] * w.x + re[i][j][q + 1] * w.y + re[i][j][q + 2] * w.z + re[i][j][q + 3] * w.w;
-                        }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) s[j] += __shfl_xor(s[j], 32, 64);
-                    *at[e] = old[e] + (h ? s[1] : s[0]);             // lane half h keeps the rows of matrix tile j = h
-                }
+                for (int j = 0; j < 2; ++j) s[j] += __shfl_xor(s[j], 32, 64);
+                float* const to = sums + ((wave >> 1) * kLdsColumns + c) * kTile + xs + lane;
+                const float mine = h ? s[1] : s[0];                  // lane half h keeps the rows of matrix tile j = h
+                *to = k ? *to + mine : mine;
             }
             __builtin_amdgcn_wave_barrier();
+        };
+        pipe.run<false>(work, finish);
+        __syncthreads();
+        for (int k = tid; k < kTile * a.C; k += 256) {
+            const int row = k & (kTile - 1), c = k >> 7;
+            if (row0 + row >= a.A.n) continue;
+            const float s = sums[c * kTile + row] + sums[(kLdsColumns + c) * kTile + row];
+            if (a.parts == 0) a.out[(row0 + row) * a.ldo + c] = s + (a.intercept ? a.intercept[c] : 0.f);
+            else a.ws[((int64_t)blockIdx.y * a.C + c) * mp + row0 + row] = s;
         }
-    };
-    pipe.run<false>(work, finish);
-    if (!in_lds) return;
-    __syncthreads();
-    for (int k = tid; k < kTile * a.C; k += 256) {
-        const int row = k & (kTile - 1), c = k >> 7;
-        if (row0 + row >= a.A.n) continue;
-        const float s = sums[c * kTile + row] + sums[(kLdsColumns + c) * kTile + row];
-        if (a.parts == 0) a.out[(row0 + row) * a.ldo + c] = s + (a.intercept ? a.intercept[c] : 0.f);
-        else a.ws[((int64_t)blockIdx.y * a.C + c) * mp + row0 + row] = s;
     }
 }
 
@@ -1667,8 +1687,10 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
         return QK_OK;
     }
     if (tile) {
-        static DeviceOnce once;
-        rc = launch8(decision8_tile_kernel, dim3((unsigned)((x->rows + kTile - 1) / kTile), (unsigned)a.splits), kDecisionLds, s, a, once, kDecisionLds);
+        static DeviceOnce once[2];
+        const dim3 grid((unsigned)((x->rows + kTile - 1) / kTile), (unsigned)a.splits);
+        rc = C > kLdsColumns ? launch8(decision8_tile_kernel<true>, grid, kPipeLds, s, a, once[0], kPipeLds)
+                             : launch8(decision8_tile_kernel<false>, grid, kDecisionLds, s, a, once[1], kDecisionLds);
     } else {
         const int side = x->rows <= 8 ? 8 : 32, sums = 4 * 32 * C * (int)sizeof(float);
         constexpr int most = 4 * 32 * QK_DECISION8_MAX_C * (int)sizeof(float), ring8 = 4 * 3 * ThinPipe<8, 3>::kBytes, ring32 = 4 * 3 * ThinPipe<32, 3>::kBytes;
