@@ -239,6 +239,11 @@ int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, size_t* bytes
 int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_t D, const float* coef, int64_t ldc, int C,
                      const float* intercept, float* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream);
 
+/* Host-pointer convenience: qk_evaluate (or, mode != QK_NOISE_NONE, qk_evaluate_noisy) over 8-bit stores.  The statevectors are
+ * simulated in FP64, a few gigabytes at a time, and stored in 8 bits; K is float64. */
+int qk_evaluate8(const qk_circuit* c, const double* X, int64_t N, const double* Y, int64_t M, int n_features, int mode,
+                 double param, uint64_t seed, double* K_host);
+
 /*
  * Replaces: kernel.evaluate(x_vec, y_vec=None) of FidelityStatevectorKernel
  * (reference qsvm/train.py:92,152,154; qsvm_tester.py:684-686; genetic_v3.py:619).
@@ -364,9 +369,10 @@ int qk_evaluate_noisy(const qk_circuit* c, const double* X, int64_t N, const dou
  *   K_host : count pointers (entries may be NULL: statistics only), N[g] x N[g] float64 each
  *   stats  : NULL or count x QK_STATS_LEN float64 (needs labels)
  */
+#define QK_BATCH_FP8 1
 typedef struct qk_batch_opts {
     int32_t noise_mode;     /* QK_NOISE_* */
-    int32_t reserved;
+    int32_t flags;          /* 0, or QK_BATCH_FP8: the kernels over 8-bit stores (qk_gram8_jobs_dev, all genomes in one call) */
     double noise_param;
     uint64_t seed;
 } qk_batch_opts;

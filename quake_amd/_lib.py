@@ -23,6 +23,7 @@ QK_GRAM_MAX_JOBS = 16
 QK_GRAM8_F16 = 2
 QK_GRAM8_F64 = 4
 QK_DECISION8_MAX_C = 64
+QK_BATCH_FP8 = 1
 
 
 class QkError(RuntimeError):
@@ -41,7 +42,7 @@ class qk_gram_job(C.Structure):
 
 
 class qk_batch_opts(C.Structure):
-    _fields_ = [("noise_mode", C.c_int32), ("reserved", C.c_int32), ("noise_param", C.c_double),
+    _fields_ = [("noise_mode", C.c_int32), ("flags", C.c_int32), ("noise_param", C.c_double),
                 ("seed", C.c_uint64)]
 
 
@@ -94,6 +95,7 @@ SIGNATURES = {
     "qk_decision8_workspace": (C.c_int, [_I64, _I64, _I64, C.c_int, C.POINTER(C.c_size_t)]),
     "qk_decision8_dev": (C.c_int, [C.POINTER(qk_states8), C.POINTER(qk_states8), _I64, _P, _I64, C.c_int, _P, _P, _I64, _P,
                                    C.c_size_t, _P]),
+    "qk_evaluate8": (C.c_int, [_P, _P, _I64, _P, _I64, C.c_int, C.c_int, C.c_double, C.c_uint64, _P]),
     "qk_evaluate_f32": (C.c_int, [_P, _P, _I64, _P, _I64, C.c_int, _P]),
     "qk_evaluate": (C.c_int, [_P, _P, _I64, _P, _I64, C.c_int, _P]),
     "qk_rdm1_dev": (C.c_int, [_P, _I64, C.c_int, _P, _P]),

@@ -283,11 +283,17 @@ struct NoiseSpec {
     uint64_t seed = 0;
 };
 
-int gram_to_host(const void* dPx, int64_t N, const void* dPy, int64_t M, int64_t D, bool f32, double* K_host,
-                 const NoiseSpec& noise = NoiseSpec()) {
-    const bool sym = (dPy == nullptr);
-    const size_t esz = f32 ? 8 : 16;
-    auto launch = f32 ? qk_gram32_jobs_dev : qk_gram_jobs_dev;
+// One block of K: rows [r0, r1) of the first set of states against rows [c0, c1) of the second (symmetric: of the first)
+struct GramBlock {
+    int64_t r0, r1, c0, c1;
+    bool sym;
+    double *K, *KT;
+    int64_t ldk, ldkt;
+};
+
+// launch(blocks, count, stream): enqueues them in one call.
+template <typename Launch>
+int gram_to_host(Launch launch, int64_t N, int64_t M, bool sym, int64_t D, double* K_host, const NoiseSpec& noise = NoiseSpec()) {
     DevBuf dK;
     QK_HIP(dK.alloc((size_t)N * M * sizeof(double)));
     double* K = (double*)dK.p;
@@ -316,11 +322,8 @@ int gram_to_host(const void* dPx, int64_t N, const void* dPy, int64_t M, int64_t
     if (nbands == 1) {
         // small problems (the reference's own sizes): one launch on the null stream behind the simulation,
         // one blocking copy -- no streams or events to create, the call is latency-bound
-        qk_gram_job job;
-        std::memset(&job, 0, sizeof(job));
-        job.A = dPx; job.B = sym ? dPx : dPy; job.K = K;
-        job.ma = N; job.nb = M; job.ldk = M; job.flags = sym ? QK_GRAM_SYMMETRIC : 0;
-        int rc1 = launch(&job, 1, D, nullptr);
+        const GramBlock block{0, N, 0, M, sym, K, nullptr, M, 0};
+        int rc1 = launch(&block, 1, nullptr);
         if (rc1) return rc1;
         if ((rc1 = launch_noise(K, 0, N, M, M, sym, noise.mode, noise.param, noise.seed, nullptr))) return rc1;
         QK_HIP(hipMemcpy(K_host, K, (size_t)N * M * sizeof(double), hipMemcpyDeviceToHost));
@@ -350,26 +353,15 @@ int gram_to_host(const void* dPx, int64_t N, const void* dPy, int64_t M, int64_t
     const size_t first_band_event = done.size();
     for (int64_t bi = 0; bi < nbands && rc == QK_OK; ++bi) {
         const int64_t r0 = cut[bi], r1 = cut[bi + 1];
-        qk_gram_job jobs[2];
-        std::memset(jobs, 0, sizeof(jobs));
+        GramBlock blocks[2];
         int nj = 0;
-        const char* A = (const char*)dPx + (size_t)r0 * D * esz;
         if (sym) {
-            jobs[nj].A = A; jobs[nj].B = A; jobs[nj].K = K + r0 * M + r0;
-            jobs[nj].ma = jobs[nj].nb = r1 - r0; jobs[nj].ldk = M; jobs[nj].flags = QK_GRAM_SYMMETRIC;
-            ++nj;
-            if (r1 < N) {
-                jobs[nj].A = A; jobs[nj].B = (const char*)dPx + (size_t)r1 * D * esz;
-                jobs[nj].K = K + r0 * M + r1; jobs[nj].KT = K + r1 * M + r0;
-                jobs[nj].ma = r1 - r0; jobs[nj].nb = N - r1; jobs[nj].ldk = M; jobs[nj].ldkt = M;
-                ++nj;
-            }
+            blocks[nj++] = GramBlock{r0, r1, r0, r1, true, K + r0 * M + r0, nullptr, M, 0};
+            if (r1 < N) blocks[nj++] = GramBlock{r0, r1, r1, N, false, K + r0 * M + r1, K + r1 * M + r0, M, M};
         } else {
-            jobs[nj].A = A; jobs[nj].B = dPy; jobs[nj].K = K + r0 * M;
-            jobs[nj].ma = r1 - r0; jobs[nj].nb = M; jobs[nj].ldk = M;
-            ++nj;
+            blocks[nj++] = GramBlock{r0, r1, 0, M, false, K + r0 * M, nullptr, M, 0};
         }
-        rc = launch(jobs, nj, D, compute);
+        rc = launch(blocks, nj, compute);
         if (rc != QK_OK) break;
         // a band's draws: its rows right of the diagonal, mirrored into the later bands' rows (symmetric), or all of
         // its rows (cross block); ordered behind the band's Gram launch on the same stream
@@ -447,13 +439,131 @@ int evaluate_host(const char* who, const qk_circuit* c, const double* X, int64_t
             QK_HIP(dPy.alloc((size_t)M * D * esz));
             if ((rc = simulate((const double*)dY.p, M, dPy.p))) return rc;
         }
-        rc = gram_to_host(dPx.p, N, sym ? nullptr : dPy.p, M, D, f32, K_host, noise);
+        const void *px = dPx.p, *py = sym ? dPx.p : dPy.p;
+        auto launch = [&](const GramBlock* blocks, int n, hipStream_t stream) {
+            qk_gram_job jobs[2];
+            std::memset(jobs, 0, sizeof(jobs));
+            for (int k = 0; k < n; ++k) {
+                const GramBlock& g = blocks[k];
+                jobs[k].A = (const char*)px + (size_t)g.r0 * D * esz;
+                jobs[k].B = (const char*)py + (size_t)g.c0 * D * esz;
+                jobs[k].K = g.K;
+                jobs[k].KT = g.KT;
+                jobs[k].ma = g.r1 - g.r0;
+                jobs[k].nb = g.c1 - g.c0;
+                jobs[k].ldk = g.ldk;
+                jobs[k].ldkt = g.ldkt;
+                jobs[k].flags = g.sym ? QK_GRAM_SYMMETRIC : 0;
+            }
+            return f32 ? qk_gram32_jobs_dev(jobs, n, D, stream) : qk_gram_jobs_dev(jobs, n, D, stream);
+        };
+        rc = gram_to_host(launch, N, M, sym, D, K_host, noise);
     }
     g_profile.t[6] = now_s() - t_begin;
     return rc;
 }
 }  // namespace
 }  // namespace qk
+
+namespace qk {
+namespace {
+// Device memory of an 8-bit store
+struct Store8 {
+    DevBuf codes, scales, gains;
+    int64_t rows = 0, cb = 0, sb = 0;
+    int alloc(int64_t n, int64_t D) {
+        rows = n;
+        const int rc = qk_states8_layout(D, &cb, &sb);
+        if (rc) return rc;
+        QK_HIP(codes.alloc((size_t)n * cb));
+        QK_HIP(scales.alloc((size_t)n * sb));
+        QK_HIP(gains.alloc((size_t)n * sizeof(float)));
+        return QK_OK;
+    }
+    qk_states8 at(int64_t first, int64_t n) const {
+        return qk_states8{(char*)codes.p + first * cb, (char*)scales.p + first * sb, (float*)gains.p + first, n};
+    }
+};
+
+// Simulates rows of x_dev into an 8-bit store, some gigabytes of statevectors at a time: Psi never exists whole.
+int simulate8(const qk_circuit* c, const double* x_dev, int64_t rows, int64_t D, DevBuf& psi, int64_t psi_rows, const Store8& to) {
+    const int F = c->n_params;
+    for (int64_t r = 0; r < rows; r += psi_rows) {
+        const int64_t n = std::min(psi_rows, rows - r);
+        int rc = qk_simulate_dev(c, x_dev ? x_dev + r * F : nullptr, n, F, psi.p, nullptr);
+        if (rc) return rc;
+        const qk_states8 part = to.at(r, n);
+        if ((rc = qk_states8_write_dev(psi.p, 0, D, D, &part, nullptr))) return rc;
+    }
+    return QK_OK;
+}
+
+qk_gram8_job gram8_job(const qk_states8& a, const qk_states8& b, int64_t D, bool sym, double* K, int64_t ldk, double* KT, int64_t ldkt) {
+    qk_gram8_job j;
+    std::memset(&j, 0, sizeof(j));
+    j.A = a;
+    j.B = b;
+    j.D = D;
+    j.K = K;
+    j.KT = KT;
+    j.ldk = ldk;
+    j.ldkt = ldkt;
+    j.flags = QK_GRAM8_F64 | (sym ? QK_GRAM_SYMMETRIC : 0);
+    return j;
+}
+constexpr size_t kPsi8Bytes = (size_t)4 << 30;      // statevectors that are waiting to be stored
+}  // namespace
+}  // namespace qk
+
+extern "C" int qk_evaluate8(const qk_circuit* c, const double* X, int64_t N, const double* Y, int64_t M, int n_features, int mode,
+                            double param, uint64_t seed, double* K_host) {
+    const char* who = "qk_evaluate8";
+    if (!c || !K_host) return fail(QK_ERR_INVALID, std::string(who) + ": null pointer");
+    if (n_features != c->n_params) return fail(QK_ERR_INVALID, "x_vec and class feature map have incompatible dimensions");
+    if (N < 0 || (Y && M < 0)) return fail(QK_ERR_INVALID, std::string(who) + ": negative row count");
+    if (c->n_params > 0 && N && !X) return fail(QK_ERR_INVALID, std::string(who) + ": X is null");
+    if (mode != QK_NOISE_NONE && mode != QK_NOISE_GAUSSIAN && mode != QK_NOISE_SHOTS)
+        return fail(QK_ERR_INVALID, std::string(who) + ": unknown noise mode");
+    const bool sym = (Y == nullptr);
+    if (sym) M = N;
+    if (N == 0 || M == 0) return QK_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    const int64_t D = (int64_t)1 << c->n_qubits;
+    const int64_t psi_rows = std::max<int64_t>(1, std::min<int64_t>(std::max(N, M), (int64_t)(kPsi8Bytes / ((size_t)D * 16))));
+    NoiseSpec noise;
+    noise.mode = mode; noise.param = param; noise.seed = seed;
+    DevBuf dX, dY, psi, ws;
+    Store8 sx, sy;
+    if ((rc = upload_X(X, N, c->n_params, dX))) return rc;
+    QK_HIP(psi.alloc((size_t)psi_rows * D * 16));
+    if ((rc = sx.alloc(N, D))) return rc;
+    if ((rc = simulate8(c, (const double*)dX.p, N, D, psi, psi_rows, sx))) return rc;
+    if (!sym) {
+        if ((rc = upload_X(Y, M, c->n_params, dY))) return rc;
+        if ((rc = sy.alloc(M, D))) return rc;
+        if ((rc = simulate8(c, (const double*)dY.p, M, D, psi, psi_rows, sy))) return rc;
+    }
+    const Store8& cols = sym ? sx : sy;
+    size_t have = 0;
+    auto launch = [&](const GramBlock* blocks, int n, hipStream_t stream) {
+        qk_gram8_job jobs[2];
+        for (int k = 0; k < n; ++k) {
+            const GramBlock& g = blocks[k];
+            jobs[k] = gram8_job(sx.at(g.r0, g.r1 - g.r0), cols.at(g.c0, g.c1 - g.c0), D, g.sym, g.K, g.ldk, g.KT, g.ldkt);
+        }
+        size_t need = 0;
+        int r = qk_gram8_workspace(jobs, n, &need);
+        if (r) return r;
+        if (need > have) {      // (releasing the smaller one waits for the launches that use it)
+            ws.release();
+            QK_HIP(ws.alloc(need));
+            have = need;
+        }
+        return qk_gram8_jobs_dev(jobs, n, ws.p, have, stream);
+    };
+    return gram_to_host(launch, N, M, sym, D, K_host, noise);
+}
 
 extern "C" int qk_evaluate(const qk_circuit* c, const double* X, int64_t N, const double* Y, int64_t M,
                            int n_features, double* K_host) {
@@ -517,6 +627,21 @@ constexpr size_t kBatchPsiBytes = (size_t)48 << 30;       // statevectors of one
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
+// One chromosome's symmetric kernel through an 8-bit store
+int batch_gram8(const void* psi, int64_t n, int64_t D, double* K) {
+    Store8 store;
+    DevBuf ws;
+    int rc = store.alloc(n, D);
+    if (rc) return rc;
+    const qk_states8 all = store.at(0, n);
+    if ((rc = qk_states8_write_dev(psi, 0, D, D, &all, nullptr))) return rc;
+    const qk_gram8_job job = gram8_job(all, all, D, true, K, n, nullptr, 0);
+    size_t need = 0;
+    if ((rc = qk_gram8_workspace(&job, 1, &need))) return rc;
+    if (need) QK_HIP(ws.alloc(need));
+    return qk_gram8_jobs_dev(&job, 1, ws.p, need, nullptr);
+}
+
 // Chromosomes whose circuit does not run on the wave-resident simulator (more than 10 qubits): one after the
 // other on the null stream, one K buffer reused when the matrix is not asked for.
 int batch_one_by_one(const std::vector<int>& idx, const qk_circuit* const* circuits, const double* const* X, const int64_t* N,
@@ -528,6 +653,7 @@ int batch_one_by_one(const std::vector<int>& idx, const qk_circuit* const* circu
         x_bytes = std::max(x_bytes, (size_t)N[g] * circuits[g]->n_params * 8);
         l_bytes = std::max(l_bytes, (size_t)N[g] * 4);
     }
+    const bool fp8 = opts && (opts->flags & QK_BATCH_FP8);
     DevBuf dX, dL, dPsi, dK, dS, dW;
     QK_HIP(dX.alloc(x_bytes));
     QK_HIP(dPsi.alloc(psi_bytes));
@@ -543,7 +669,7 @@ int batch_one_by_one(const std::vector<int>& idx, const qk_circuit* const* circu
         int rc;
         if (c->n_params) QK_HIP(hipMemcpy(dX.p, X[g], (size_t)n * c->n_params * 8, hipMemcpyHostToDevice));
         if ((rc = qk_simulate_dev(c, (const double*)dX.p, n, c->n_params, dPsi.p, nullptr))) return rc;
-        if ((rc = qk_gram_dev(dPsi.p, n, nullptr, n, D, (double*)dK.p, n, nullptr))) return rc;
+        if ((rc = fp8 ? batch_gram8(dPsi.p, n, D, (double*)dK.p) : qk_gram_dev(dPsi.p, n, nullptr, n, D, (double*)dK.p, n, nullptr))) return rc;
         if (noise != QK_NOISE_NONE &&
             (rc = qk_kernel_noise_dev((double*)dK.p, n, n, noise, opts->noise_param, opts->seed + (uint64_t)g, nullptr)))
             return rc;
@@ -565,6 +691,7 @@ int batch_one_by_one(const std::vector<int>& idx, const qk_circuit* const* circu
 int batch_wave(const std::vector<int>& idx, const qk_circuit* const* circuits, const double* const* X, const int64_t* N,
                const int32_t* const* labels, int noise, const qk_batch_opts* opts, double* const* K_host, double* stats) {
     const int cnt = (int)idx.size();
+    const bool fp8 = opts && (opts->flags & QK_BATCH_FP8);
     bool small = true;
     size_t k_total = 0;
     for (int g : idx) {
@@ -657,8 +784,41 @@ int batch_wave(const std::vector<int>& idx, const qk_circuit* const* circuits, c
                                    r.cs_bytes, nullptr)))
             return rc;
     if (small) {
-        // ---- Gram: 16 chromosomes of one dimension per launch -------------------------------------------------
-        for (int p = 0; p < cnt;) {
+        // ---- Gram: 16 chromosomes of one dimension per launch; over 8-bit stores all of them in one call -----------
+        DevBuf slab, ws8;
+        if (fp8) {
+            std::vector<qk_states8> at(cnt);
+            size_t bytes = 0;
+            auto place = [&](char* base) {      // the stores one after the other, every array on its own 256 bytes
+                bytes = 0;
+                for (int k = 0; k < cnt; ++k) {
+                    const int64_t n = N[idx[k]];
+                    int64_t cb = 0, sb = 0;
+                    (void)qk_states8_layout((int64_t)1 << circuits[idx[k]]->n_qubits, &cb, &sb);
+                    at[k].rows = n;
+                    at[k].codes = base + bytes;
+                    bytes = align_up(bytes + (size_t)n * cb, 256);
+                    at[k].scales = base + bytes;
+                    bytes = align_up(bytes + (size_t)n * sb, 256);
+                    at[k].gains = (float*)(base + bytes);
+                    bytes = align_up(bytes + (size_t)n * sizeof(float), 256);
+                }
+            };
+            place(nullptr);
+            QK_HIP(slab.alloc(bytes));
+            place((char*)slab.p);
+            std::vector<qk_gram8_job> g8(cnt);
+            for (int k = 0; k < cnt; ++k) {
+                const int64_t D = (int64_t)1 << circuits[idx[k]]->n_qubits;
+                if ((rc = qk_states8_write_dev((char*)dPsi.p + psi_off[k], 0, D, D, &at[k], nullptr))) return rc;
+                g8[k] = gram8_job(at[k], at[k], D, true, (double*)((char*)dK.p + k_off[k]), N[idx[k]], nullptr, 0);
+            }
+            size_t need = 0;
+            if ((rc = qk_gram8_workspace(g8.data(), cnt, &need))) return rc;
+            if (need) QK_HIP(ws8.alloc(need));
+            if ((rc = qk_gram8_jobs_dev(g8.data(), cnt, ws8.p, need, nullptr))) return rc;
+        }
+        for (int p = 0; p < cnt && !fp8;) {
             qk_gram_job gj[QK_GRAM_MAX_JOBS];
             std::memset(gj, 0, sizeof(gj));
             const int nq = circuits[idx[order[p]]]->n_qubits;
@@ -686,7 +846,9 @@ int batch_wave(const std::vector<int>& idx, const qk_circuit* const* circuits, c
             const int g = idx[k];
             const int64_t n = N[g], D = (int64_t)1 << circuits[g]->n_qubits;
             double* Kg = (double*)dK.p;
-            if ((rc = qk_gram_dev((char*)dPsi.p + psi_off[k], n, nullptr, n, D, Kg, n, nullptr))) return rc;
+            if ((rc = fp8 ? batch_gram8((char*)dPsi.p + psi_off[k], n, D, Kg)
+                          : qk_gram_dev((char*)dPsi.p + psi_off[k], n, nullptr, n, D, Kg, n, nullptr)))
+                return rc;
             if (noise != QK_NOISE_NONE &&
                 (rc = qk_kernel_noise_dev(Kg, n, n, noise, opts->noise_param, opts->seed + (uint64_t)g, nullptr)))
                 return rc;
@@ -718,6 +880,7 @@ extern "C" int qk_evaluate_batch(int count, const qk_circuit* const* circuits, c
     const int noise = opts ? opts->noise_mode : QK_NOISE_NONE;
     if (noise != QK_NOISE_NONE && noise != QK_NOISE_GAUSSIAN && noise != QK_NOISE_SHOTS)
         return fail(QK_ERR_INVALID, "qk_evaluate_batch: unknown noise mode");
+    if (opts && (opts->flags & ~QK_BATCH_FP8)) return fail(QK_ERR_INVALID, "qk_evaluate_batch: unknown flag");
     if (noise == QK_NOISE_GAUSSIAN && !(opts->noise_param >= 0.0))
         return fail(QK_ERR_INVALID, "qk_evaluate_batch: negative standard deviation");
     if (noise == QK_NOISE_SHOTS && (!(opts->noise_param >= 1.0) || opts->noise_param > 1e9))

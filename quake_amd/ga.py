@@ -335,19 +335,22 @@ class GeneticArtifacts:
 def generation_fitness(solutions, data_cv, data_labels, gate_dict, nb_features, gates_per_qubits, nb_qubits,
                        fit_fun: Callable, projected: bool = False, noise_std=None, depth_fn: Optional[Callable] = None,
                        cv: int = 4, seed: int = 0, variant: str = "v3", coupling_map=None, basis_gates=None,
-                       lower_fn: Optional[Callable] = None):
+                       lower_fn: Optional[Callable] = None, precision: str = "double"):
     """Fitness of many chromosomes at once: the body of the reference's ``fitness_func``
     (genetic_v3.py:604-666) with the kernels of the whole batch computed in one GPU call.
 
     ``coupling_map`` serves the v4 / v5 decoders and, with ``basis_gates``, the lowering of the
     ``without_kernel`` mode (``lower_fn(fmap, coupling_map, basis_gates, optimization_level=0)``, default
-    :func:`quake_amd.transpile.transpile`).
+    :func:`quake_amd.transpile.transpile`).  ``precision``: of the fidelity kernels
+    (:func:`quake_amd.kernels.evaluate_population`); projected kernels are always "double".
     Returns ``(fitness values, per-chromosome stats dicts or None)``."""
     from sklearn.model_selection import cross_val_score
     from sklearn.svm import SVC
 
     from .kernels import evaluate_population, projected_quantum_kernel
 
+    if projected and precision != "double":
+        raise ValueError("projected kernels have no other precision than 'double'")
     data_labels = np.asarray(data_labels)
     decoded = [genetic.to_quantum(s, gate_dict, nb_features, gates_per_qubits, nb_qubits, verbose=False,
                                   variant=variant, coupling_map=coupling_map) for s in solutions]
@@ -365,7 +368,7 @@ def generation_fitness(solutions, data_cv, data_labels, gate_dict, nb_features, 
         stats = [genetic.kernel_statistics(K, data_labels) for K in Ks]
     else:
         noise = ("gaussian", float(noise_std)) if noise_std is not None else None
-        Ks, stats = evaluate_population(maps, xs, labels=data_labels, noise=noise, seed=seed)
+        Ks, stats = evaluate_population(maps, xs, labels=data_labels, noise=noise, seed=seed, precision=precision)
     values = []
     for fmap, K, st in zip(maps, Ks, stats):
         acc = cross_val_score(SVC(kernel="precomputed"), K, data_labels, cv=cv, scoring="accuracy").mean()
@@ -377,12 +380,13 @@ def generation_fitness(solutions, data_cv, data_labels, gate_dict, nb_features, 
 def genetic_instance(gene_space, data_cv, data_labels, backend, gate_dict, nb_features, gates_per_qubits, nb_qubits,
                      projected, suffix, coupling_map, basis_gates, fit_fun, noise_std=None, *,
                      save_dir="../../Output_genetic", depth_fn: Optional[Callable] = None, variant: str = "v3",
-                     verbose: bool = True, **kwargs) -> GeneticRun:
+                     verbose: bool = True, precision: str = "double", **kwargs) -> GeneticRun:
     """Same positional signature as reference ``genetic_instance`` (genetic_v3.py:451-533); returns
     a :class:`GeneticRun` where the reference returns ``pygad.GA``.  ``backend`` is accepted and
     unused (as in the reference's statevector path).  ``depth`` comes from
     ``transpile.transpiled_depth(fmap, coupling_map, basis_gates)``, the native stand-in for
-    ``transpile(...).depth()`` (reference :652-654), unless ``depth_fn`` is given."""
+    ``transpile(...).depth()`` (reference :652-654), unless ``depth_fn`` is given.  ``precision``: see
+    :func:`generation_fitness`."""
     from .transpile import transpiled_depth
 
     if depth_fn is None:
@@ -395,7 +399,7 @@ def genetic_instance(gene_space, data_cv, data_labels, backend, gate_dict, nb_fe
         values, stats = generation_fitness(solutions, data_cv, data_labels, gate_dict, nb_features, gates_per_qubits,
                                            nb_qubits, fit_fun, projected=projected, noise_std=noise_std,
                                            depth_fn=depth_fn, seed=counter["seed"], variant=variant,
-                                           coupling_map=coupling_map, basis_gates=basis_gates)
+                                           coupling_map=coupling_map, basis_gates=basis_gates, precision=precision)
         counter["seed"] += len(solutions)
         for k, sol in enumerate(solutions):
             st = stats[k] if stats is not None else None

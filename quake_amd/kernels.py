@@ -104,10 +104,13 @@ class HipFidelityKernel:
                  parameter_values: Optional[Sequence[float]] = None,
                  shots=None, cache_size=None, auto_clear_cache: bool = True, precision: str = "double",
                  seed: Optional[int] = None):
-        if precision not in ("double", "single"):
-            raise ValueError("precision must be 'double' or 'single'")
+        if precision not in ("double", "single", "fp8"):
+            raise ValueError("precision must be 'double', 'single' or 'fp8'")
         # 'single': statevectors stored as complex64 and the Gram stage on FP32 MFMA (|dK| <= 1e-5); a
-        # build option with no counterpart in the reference, whose kernel is always complex128
+        # build option with no counterpart in the reference, whose kernel is always complex128.
+        # 'fp8': statevectors kept in 8 bits with a scale for each block of 128 amplitudes and restored norms
+        # (qk_states8); K is a valid kernel with unit diagonal whose entries are off by about 0.07 sqrt(K / 2^n) for
+        # states spread over their 2^n amplitudes, at most 0.13
         self._precision = precision
         if shots is not None and int(shots) < 1:
             raise ValueError("shots must be a positive integer")
@@ -213,14 +216,22 @@ class HipFidelityKernel:
             self._shot_calls += 1
             seed = (self._shot_seed + self._shot_calls) & (2**64 - 1)
             K = _lib.host_empty((n, m))
+            if self._precision == "fp8":
+                _lib.check(lib.qk_evaluate8(circ.handle, _lib.ptr(x), n, _lib.ptr(y) if y is not None else None, m, x.shape[1],
+                                            _lib.NOISE_SHOTS, float(self._shots), seed, _lib.ptr(K)))
+                return K
             _lib.check(lib.qk_evaluate_noisy(
                 circ.handle, _lib.ptr(x), n, _lib.ptr(y) if y is not None else None, m, x.shape[1],
                 0 if self._precision == "double" else 1, _lib.NOISE_SHOTS, float(self._shots), seed, _lib.ptr(K)))
             return K
         K = out if out is not None else _lib.host_empty((n, m))
-        _lib.check((lib.qk_evaluate if self._precision == "double" else lib.qk_evaluate_f32)(
-            circ.handle, _lib.ptr(x), n,
-            _lib.ptr(y) if y is not None else None, m, x.shape[1], _lib.ptr(K)))
+        if self._precision == "fp8":
+            _lib.check(lib.qk_evaluate8(circ.handle, _lib.ptr(x), n, _lib.ptr(y) if y is not None else None, m, x.shape[1],
+                                        _lib.NOISE_NONE, 0.0, 0, _lib.ptr(K)))
+        else:
+            _lib.check((lib.qk_evaluate if self._precision == "double" else lib.qk_evaluate_f32)(
+                circ.handle, _lib.ptr(x), n,
+                _lib.ptr(y) if y is not None else None, m, x.shape[1], _lib.ptr(K)))
         _pin_equal_rows(K, x, y)
         if y is None and self._enforce_psd:
             K = self._make_psd(K)
@@ -244,10 +255,10 @@ class HipFidelityKernel:
         return np.ascontiguousarray((v @ np.diag(np.maximum(0, w)) @ v.transpose()).real)
 
 
-def make_kernels(maps: List[QuantumCircuit], backend=None) -> List[HipFidelityKernel]:
+def make_kernels(maps: List[QuantumCircuit], backend=None, *, precision: str = "double") -> List[HipFidelityKernel]:
     """Quantum kernels for a list of feature maps (reference qsvm_tester.py:382-413).
 
-    ``backend`` is accepted and ignored, as in the reference's statevector branch.
+    ``backend`` is accepted and ignored, as in the reference's statevector branch; ``precision`` goes to the kernels.
     A map with more parameters than qubits (the ``align=True`` theta prefix) gets its
     trailing parameters as training parameters, like the reference's
     ``TrainableFidelityQuantumKernel`` branch (initialised to zero)."""
@@ -256,9 +267,9 @@ def make_kernels(maps: List[QuantumCircuit], backend=None) -> List[HipFidelityKe
         params = fmap.parameters
         if len(params) > fmap.num_qubits:
             theta = params[fmap.num_qubits:]
-            kernels.append(HipFidelityKernel(feature_map=fmap, training_parameters=theta))
+            kernels.append(HipFidelityKernel(feature_map=fmap, training_parameters=theta, precision=precision))
         else:
-            kernels.append(HipFidelityKernel(feature_map=fmap))
+            kernels.append(HipFidelityKernel(feature_map=fmap, precision=precision))
     return kernels
 
 
@@ -298,7 +309,7 @@ def statistics_from_sums(sums: np.ndarray, N: int) -> dict:
 
 
 def evaluate_population(feature_maps: Sequence[QuantumCircuit], x_vecs: Sequence[np.ndarray], labels=None,
-                        noise: Optional[tuple] = None, seed: int = 0, return_kernels: bool = True):
+                        noise: Optional[tuple] = None, seed: int = 0, return_kernels: bool = True, precision: str = "double"):
     """Symmetric fidelity kernels of many (circuit, data) pairs in ONE library call: the GA's
     generation (reference genetic_v3.py:587-661 runs them one by one).
 
@@ -307,7 +318,11 @@ def evaluate_population(feature_maps: Sequence[QuantumCircuit], x_vecs: Sequence
             reduced on the device and returned as dicts (``statistics_from_sums``).
     noise:  None, ``("gaussian", std)`` or ``("shots", shots)``, applied on the device before the
             statistics (genome g uses ``seed + g``).
+    precision: "double", or "fp8": the kernels over 8-bit stores (HipFidelityKernel's "fp8"), all genomes in one launch
+            whatever their sizes.
     Returns ``(kernels or None, stats or None)``."""
+    if precision not in ("double", "fp8"):
+        raise ValueError("precision must be 'double' or 'fp8'")
     count = len(feature_maps)
     if len(x_vecs) != count:
         raise ValueError("one data array per feature map")
@@ -345,10 +360,11 @@ def evaluate_population(feature_maps: Sequence[QuantumCircuit], x_vecs: Sequence
     if Ks is None and sums is None:
         raise ValueError("nothing to compute: return_kernels=False needs labels")
     opts = None
-    if noise is not None:
-        mode, param = noise
-        code = {"gaussian": _lib.NOISE_GAUSSIAN, "shots": _lib.NOISE_SHOTS}[mode]
-        opts = C.pointer(_lib.qk_batch_opts(code, 0, float(param), int(seed) & (2**64 - 1)))
+    flags = _lib.QK_BATCH_FP8 if precision == "fp8" else 0
+    if noise is not None or flags:
+        mode, param = noise if noise is not None else (None, 0.0)
+        code = {None: _lib.NOISE_NONE, "gaussian": _lib.NOISE_GAUSSIAN, "shots": _lib.NOISE_SHOTS}[mode]
+        opts = C.pointer(_lib.qk_batch_opts(code, flags, float(param), int(seed) & (2**64 - 1)))
     _lib.check(lib.qk_evaluate_batch(count, circ_arr, x_arr, n_arr, lab_arr, opts, k_arr,
                                      sums.ctypes.data if sums is not None else None))
     if Ks is not None and noise is None:

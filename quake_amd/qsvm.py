@@ -37,18 +37,19 @@ def rearrange_scale(train_set, val_set, test_set, should_do_scaling: bool) -> li
     return full
 
 
-def load_quantum_kernels(qubits: int, maps: Optional[Sequence[Tuple[str, dict]]] = None):
+def load_quantum_kernels(qubits: int, maps: Optional[Sequence[Tuple[str, dict]]] = None, precision: str = "double"):
     """Kernel objects and their titles (reference ``train.py:169-187``: c2, gen1, gen2 over
     ``x = ParameterVector("x", qubits)``).  ``maps`` optionally replaces the hard-wired
-    list with runcard entries ``[(name, {"repeats": .., "align": ..}), ...]``."""
+    list with runcard entries ``[(name, {"repeats": .., "align": ..}), ...]``.  ``precision``: of the kernels
+    (:class:`quake_amd.kernels.HipFidelityKernel`)."""
     if maps is not None:
         circuits = [build_featuremap(name, qubits, **(opts or {})) for name, opts in maps]
-        return make_kernels(circuits, None), [name for name, _ in maps]
+        return make_kernels(circuits, None, precision=precision), [name for name, _ in maps]
     x = ParameterVector("x", length=qubits)
     c2 = custom2_featuremap(x, qubits)
     gen1 = genetic_featuremap(x)
     gen2 = genetic_featuremap_2(x)
-    return make_kernels([c2, gen1, gen2], None), ["c2", "gen1", "gen2"]
+    return make_kernels([c2, gen1, gen2], None, precision=precision), ["c2", "gen1", "gen2"]
 
 
 def qsvm_hyperparameter_training(train_folder, dataset, labels, qt_kernels, kernel_titles,
@@ -145,7 +146,7 @@ def qsvm_train_from_features(features, labels, train_folder, setup: dict, seed: 
     labels = list(labels)
     dataset[0], labels[0] = train_test_split(dataset[0], labels[0], train_size=q["split_ratio"], random_state=seed)[::2]
     qubits = dataset[0].shape[1]
-    kernels, titles = load_quantum_kernels(qubits, q.get("feature_maps"))
+    kernels, titles = load_quantum_kernels(qubits, q.get("feature_maps"), q.get("precision", "double"))
     models = qsvm_hyperparameter_training(train_folder, dataset, labels, kernels, titles,
                                           q.get("should_add_extra_feats", False),
                                           final_kernel=q.get("final_kernel", "rbf"))

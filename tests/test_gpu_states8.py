@@ -398,3 +398,115 @@ def test_refusals():
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"case {k} was taken")
+
+
+# ---- the framework's own paths ---------------------------------------------------------------------------------------------
+def fp8_kernel(circ, X, Y=None):
+    """K of HipFidelityKernel(precision="fp8") in float64 from the library's own FP64 states, with its error bound."""
+    from quake_amd.kernels import HipFidelityKernel
+    exact = HipFidelityKernel(circ)
+    def side(v):
+        codes, scales, gains = S8.write(exact.statevectors(v))
+        return S8.rows(codes, scales, 1 << circ.num_qubits), gains.astype(np.float32).astype(np.float64)
+    a, ga = side(X)
+    b, gb = (a, ga) if Y is None else side(Y)
+    K, tol, _ = S8.kernel(a, ga, b, gb)
+    if Y is None:
+        np.fill_diagonal(K, 1.0)
+    return K, tol
+
+
+@pytest.mark.parametrize("n,N,M", [(1, 5, 3), (4, 100, 17), (6, 33, 70), (8, 300, 1), (12, 40, 65), (14, 5, 9)])
+def test_kernel_object_fp8(n, N, M):
+    from quake_amd import featuremaps as fm
+    from quake_amd.circuit import ParameterVector
+    from quake_amd.kernels import HipFidelityKernel
+    rng = np.random.default_rng(n)
+    X, Y = rng.uniform(-1.5, 1.5, size=(N, n)), rng.uniform(-1.5, 1.5, size=(M, n))
+    circ = fm.zz_featuremap(ParameterVector("x", n), n, 2) if n > 1 else fm.z_featuremap(ParameterVector("x", n), n, 2)
+    k8 = HipFidelityKernel(circ, precision="fp8")
+    K = k8.evaluate(X)
+    ref, tol = fp8_kernel(circ, X)
+    assert K.dtype == np.float64 and np.array_equal(K, K.T) and (np.diag(K) == 1).all() and (np.abs(K - ref) <= tol).all()
+    assert np.linalg.eigvalsh(K).min() > -(tol.max() + 1e-12) * N            # positive semidefinite up to its rounding
+    ref, tol = fp8_kernel(circ, X, Y)
+    assert (np.abs(k8.evaluate(X, Y) - ref) <= tol).all()
+    out = np.empty((N, N))
+    assert k8.evaluate(X, out=out) is out and np.array_equal(out, K)
+    full = HipFidelityKernel(circ).evaluate(X)
+    assert np.abs(K - full).max() <= 0.13
+    shots = HipFidelityKernel(circ, precision="fp8", shots=1000, seed=3)
+    S = shots.evaluate(X)
+    assert np.array_equal(S, S.T) and (S * 1000 == np.round(S * 1000)).all() and np.abs(S - K).max() < 6 * 0.5 / np.sqrt(1000)
+
+
+def test_kernel_object_fp8_in_bands():
+    """Enough rows for the host path's bands (symmetric blocks, mirrored blocks) and for several batches of states."""
+    from quake_amd import featuremaps as fm
+    from quake_amd.circuit import ParameterVector
+    from quake_amd.kernels import HipFidelityKernel
+    rng = np.random.default_rng(0)
+    X = rng.uniform(-1.5, 1.5, size=(4500, 6))
+    circ = fm.zz_featuremap(ParameterVector("x", 6), 6, 1)
+    K = HipFidelityKernel(circ, precision="fp8").evaluate(X)
+    assert np.array_equal(K, K.T) and (np.diag(K) == 1).all()
+    pick = np.concatenate([np.arange(0, 4500, 271), [1023, 1024, 1151, 1152, 4499]])
+    ref, tol = fp8_kernel(circ, X[pick], X)
+    got = K[pick]
+    own = np.zeros(got.shape, dtype=bool)
+    own[np.arange(len(pick)), pick] = True
+    assert (np.abs(got - ref)[~own] <= tol[~own]).all()
+    Kx = HipFidelityKernel(circ, precision="fp8").evaluate(X, X[:77])
+    ref, tol = fp8_kernel(circ, X[pick], X[:77])
+    same = pick[:, None] == np.arange(77)[None, :]                  # equal rows: exactly one, as in every precision
+    assert (np.abs(Kx[pick] - ref)[~same] <= tol[~same]).all() and (Kx[pick][same] == 1).all()
+
+
+def test_population_fp8():
+    from quake_amd import featuremaps as fm
+    from quake_amd.circuit import ParameterVector
+    from quake_amd.kernels import evaluate_population
+    rng = np.random.default_rng(5)
+    sizes = [(2, 30), (4, 100), (10, 129), (3, 64), (11, 20), (4, 7)] * 5          # wave-resident circuits and one that is not
+    maps = [fm.zz_featuremap(ParameterVector("x", n), n, 1) for n, _ in sizes]
+    xs = [rng.uniform(-1.5, 1.5, size=(N, n)) for n, N in sizes]
+    labels = [rng.integers(0, 2, size=N) for _, N in sizes]
+    Ks, stats = evaluate_population(maps, xs, labels=labels, precision="fp8")
+    _, exact = evaluate_population(maps, xs, labels=labels)
+    for circ, x, K, st, ex in zip(maps, xs, Ks, stats, exact):
+        ref, tol = fp8_kernel(circ, x)
+        assert np.array_equal(K, K.T) and (np.diag(K) == 1).all() and (np.abs(K - ref) <= tol).all()
+        assert abs(st["offdiagonal_mean"] - np.triu(K, 1).mean()) < 1e-12
+        assert abs(st["offdiagonal_mean"] - ex["offdiagonal_mean"]) < 0.13
+    big, _ = evaluate_population(maps[1:2], [rng.uniform(-1.5, 1.5, size=(1100, 4))], precision="fp8")     # one by one above 1024 rows
+    assert (np.diag(big[0]) == 1).all() and np.linalg.eigvalsh(big[0]).min() > -1e-4
+    noisy, _ = evaluate_population(maps[:2], xs[:2], noise=("gaussian", 0.01), seed=4, precision="fp8")
+    assert 0.001 < np.abs(noisy[1] - Ks[1]).max() < 0.1
+
+
+@pytest.mark.parametrize("classes", [2, 3, 10])
+def test_served_svc(classes):
+    from sklearn.svm import SVC
+    from quake_amd import featuremaps as fm
+    from quake_amd.circuit import ParameterVector
+    from quake_amd.kernels import HipFidelityKernel
+    from quake_amd.serving import ServedSVC
+    rng = np.random.default_rng(classes)
+    n, N = 6, 300
+    X, Q = rng.uniform(-1.5, 1.5, size=(N, n)), rng.uniform(-1.5, 1.5, size=(41, n))
+    y = (X[:, 0] * 2 + X[:, 1] > np.linspace(-3, 3, classes + 1)[1:-1, None]).sum(axis=0)
+    circ = fm.custom2_featuremap(ParameterVector("x", n), n, 1)
+    kernel = HipFidelityKernel(circ, precision="fp8")
+    svc = SVC(kernel="precomputed", C=5, decision_function_shape="ovo").fit(kernel.evaluate(X), y)
+    served = ServedSVC(kernel, svc, X)
+    Kq = kernel.evaluate(Q, X)
+    want = svc.decision_function(Kq).reshape(41, -1)
+    coef = np.abs(svc.dual_coef_).sum()
+    got = served.decision_function(Q).reshape(41, -1)
+    # every entry of K is at most 1: FP32's rounding of the coefficients, the products and their sum; and two computations of K,
+    # each off by 2 sqrt(2) sqrt(K) 8 sqrt(2 D) U32 S (tests/_states8.py) with S <= sqrt(2) (1 + 2^-4)^2
+    k_error = 2 * np.sqrt(2) * 8 * np.sqrt(2.0 ** (n + 1)) * S8.U32 * np.sqrt(2) * 1.13
+    assert np.abs(got - want).max() <= ((3 + 8 * np.sqrt(N)) * S8.U32 + 2 * k_error) * coef
+    assert np.array_equal(served.decision_function(Q[3]).ravel(), served.decision_function(Q[3:4]).ravel())
+    clear = np.abs(want).min(axis=1) > 1e-3
+    assert np.array_equal(served.predict(Q)[clear], svc.predict(Kq)[clear]) and clear.sum() > 20

@@ -123,3 +123,67 @@ def test_python_entry_points_refuse_cpu_tensors():
     for dim in (0, (1 << 26) + 1):
         with pytest.raises(ValueError):
             qdev.States8(4, dim)
+
+
+@pytest.mark.parametrize("classes", [2, 3, 5])
+def test_pair_coefficients_are_sklearns_decision(classes):
+    from sklearn.svm import SVC
+    from quake_amd.serving import pair_coefficients
+    rng = np.random.default_rng(classes)
+    psi = S8.states(rng, 60, 16, "product")
+    K = np.abs(psi.conj() @ psi.T) ** 2
+    y = rng.integers(0, classes, size=60)
+    svc = SVC(kernel="precomputed", C=10, decision_function_shape="ovo").fit(K, y)
+    coef, b = pair_coefficients(svc)
+    want = svc.decision_function(K).reshape(60, -1)
+    got = K[:, svc.support_] @ coef + b
+    assert coef.shape == (len(svc.support_), classes * (classes - 1) // 2)
+    assert np.abs(got - want).max() < 1e-9 * np.abs(want).max()
+
+
+def test_served_svc_refusals():
+    from sklearn.svm import SVC
+    from quake_amd import circuit as qc, featuremaps as fm
+    from quake_amd.kernels import HipFidelityKernel
+    from quake_amd.serving import ServedSVC
+    k = HipFidelityKernel(fm.zz_featuremap(qc.ParameterVector("x", 3), 3, 1))
+    X, y = np.random.default_rng(0).uniform(size=(20, 3)), np.arange(20) % 2
+    with pytest.raises(ValueError):
+        ServedSVC(k, SVC(kernel="rbf").fit(X, y), X)
+    with pytest.raises(ValueError):
+        ServedSVC(k, SVC(kernel="precomputed"), X)
+    svc = SVC(kernel="precomputed").fit(X @ X.T, y)
+    with pytest.raises(ValueError):
+        ServedSVC(k, svc, X[:19])
+    with pytest.raises(ValueError):
+        ServedSVC(k, svc, X[:, :2])
+    many = SVC(kernel="precomputed").fit(np.eye(24), np.arange(24) % 12)
+    with pytest.raises(ValueError, match="classes"):
+        ServedSVC(k, many, np.zeros((24, 3)))
+
+
+def test_precision_names():
+    from quake_amd import circuit as qc, featuremaps as fm, ga
+    from quake_amd.kernels import HipFidelityKernel, evaluate_population, make_kernels
+    fmap = fm.z_featuremap(qc.ParameterVector("x", 2), 2)
+    assert make_kernels([fmap], precision="fp8")[0]._precision == "fp8"
+    with pytest.raises(ValueError):
+        HipFidelityKernel(fmap, precision="half")
+    with pytest.raises(ValueError):
+        evaluate_population([fmap], [np.zeros((3, 2))], precision="single")
+    with pytest.raises(ValueError, match="projected"):
+        ga.generation_fitness([], np.zeros((3, 2)), np.zeros(3), {}, 2, 1, 2, lambda accuracy: 0, projected=True, precision="fp8")
+
+
+def test_evaluate8_and_batch_refusals(lib):
+    from quake_amd import circuit as qc, featuremaps as fm
+    h = _lib.CircuitHandle(fm.z_featuremap(qc.ParameterVector("x", 2), 2).compile())
+    X, K = np.zeros((3, 2)), np.zeros((3, 3))
+    call = lambda x=X.ctypes.data, n=3, f=2, mode=0, k=K.ctypes.data: lib.qk_evaluate8(h.handle, x, n, None, 0, f, mode, 0.0, 0, k)
+    bad = _lib.QK_ERR_INVALID
+    assert call(f=3) == bad and call(n=-1) == bad and call(x=None) == bad and call(mode=9) == bad and call(k=None) == bad
+    assert call(n=0) == 0
+    opts = _lib.qk_batch_opts(0, 2, 0.0, 0)
+    P = C.c_void_p
+    assert lib.qk_evaluate_batch(1, (P * 1)(h.handle), (P * 1)(X.ctypes.data), (C.c_int64 * 1)(3), None, C.byref(opts),
+                                 (P * 1)(K.ctypes.data), None) == bad and "flag" in _lib.last_error()
