@@ -846,16 +846,16 @@ template <bool NATIVE> struct TilePipe {
     }
 };
 
-// Position in a launch -> item: groups of 64 consecutive items (what an XCD runs at a time: 8 x 8 tiles of a strip) are dealt to
-// the eight XCDs in turn, the rest of the list evenly.
+// Position in a launch -> item: groups of 8 consecutive items (a column of a strip's tiles) are dealt to the eight XCDs in turn, so
+// that the 64 tiles of a round on an XCD are 8 columns of one strip; the rest of the list evenly.
 __device__ __forceinline__ bool gram8_item(uint32_t total, uint32_t position, uint32_t& item) {
-    const uint32_t xcd = position & 7u, seq = position >> 3, full = total >> 9;
-    if ((seq >> 6) < full) {
-        item = ((((seq >> 6) << 3) + xcd) << 6) + (seq & 63u);
+    const uint32_t xcd = position & 7u, seq = position >> 3, full = total >> 6;
+    if ((seq >> 3) < full) {
+        item = ((((seq >> 3) << 3) + xcd) << 3) + (seq & 7u);
         return true;
     }
-    const uint32_t rest = total - (full << 9), share = (rest + 7u) >> 3, in = seq - (full << 6);
-    item = (full << 9) + xcd * share + in;
+    const uint32_t rest = total - (full << 6), share = (rest + 7u) >> 3, in = seq - (full << 3);
+    item = (full << 6) + xcd * share + in;
     return in < share && item < total;
 }
 
@@ -885,7 +885,9 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
     struct Where { int job; uint32_t t, ti, tj; int slice; } now{}, before{};      // of the tile that was opened last and the one before
     auto work = [&](int k, TileWork& w) {
         uint32_t item;
-        if (!gram8_item(args.total, blockIdx.x + (uint32_t)k * gridDim.x, item)) return false;
+        // every other round backwards: the list goes from long rows to short ones
+        const uint32_t in = k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+        if (!gram8_item(args.total, in + (uint32_t)k * gridDim.x, item)) return false;
         before = now;
         Where& p = now;
         p.job = uniform(gram8_job(args, item));
@@ -1605,11 +1607,11 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
     const hipStream_t s = (hipStream_t)stream;
     return gram8_launches(jobs, n_jobs, [&](Gram8Plan& p, Gram8Kind kind) {
         p.args.ws = (float*)ws;
-        const uint32_t total = p.args.total, full = total >> 9;
+        const uint32_t total = p.args.total, full = total >> 6;
         // two workgroups per CU that stay, or, for long rows, one for each item: the hardware then starts neighbours together, and they
         // keep sharing rows in L2 (12000 rows: 16384 amplitudes 4.37 against 4.12 ms, 65536 20.3 against 17.3; 4096 rows of 4096
         // amplitudes the same; 256 amplitudes 27.5 against 28.4 us)
-        const dim3 dealt(std::min<uint32_t>(p.args.job[0].chunks > 64 ? 0x7fffffffu : 512u, (full << 9) + 8 * ((total - (full << 9) + 7) >> 3)));      // two workgroups per CU
+        const dim3 dealt(std::min<uint32_t>(p.args.job[0].chunks > 64 ? 0x7fffffffu : 512u, (full << 6) + 8 * ((total - (full << 6) + 7) >> 3)));      // two workgroups per CU
         if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, dim3(total), dim3(256), 0, s, p.args);
         else if (kind == GK_THIN8) QK_THIN8(8, false);
         else if (kind == GK_THIN8_SWAP) QK_THIN8(8, true);
