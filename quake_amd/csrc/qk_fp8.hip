@@ -869,8 +869,10 @@ template <typename T> __device__ __forceinline__ void put(T v, __amdgpu_buffer_r
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, v), to, off, soff, 0);
     }
 }
-__device__ __forceinline__ void put16(uint4 v, __amdgpu_buffer_rsrc_t to, int off, int soff) {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), to, off, soff, 0);
+// (No scalar offset here: behind a 16-byte buffer store with one the compiler puts no wait state before the next write to its
+// data registers, and lanes 12 .. 15 of every 16 were seen to store the new value of the first.)
+__device__ __forceinline__ void put16(uint4 v, __amdgpu_buffer_rsrc_t to, int off) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), to, off, 0, 0);
 }
 
 // The same in every lane, and known to be: addresses and descriptors made from it stay in scalar registers.
@@ -956,10 +958,11 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
         T* const mirror = (T*)(sym ? J.K : J.KT);
         if (!mirror) return;
         // The mirror through LDS, [column][its rows], 16-byte pieces of a column at piece ^ key(column); out in whole lines where the
-        // rows allow it.
+        // rows start on 16 bytes.
         const int64_t ldm = sym ? J.ldk : J.ldkt;
         const int mstep = (int)ldm * S;
-        const bool whole = rows == 64 && cols == 64 && !diagonal && !(((uintptr_t)mirror | (uint32_t)mstep) & 15);
+        const bool aligned = !(((uintptr_t)mirror | (uint32_t)mstep) & 15), whole = rows >= 64 && cols >= 64 && (!diagonal || ahead > 0);
+        if (diagonal && ahead < 0) return;
         const __amdgpu_buffer_rsrc_t M = __builtin_amdgcn_make_buffer_rsrc((char*)mirror + (col_t * ldm + row_t) * S, 0, kRange, kRsrc);
         constexpr int E = 16 / sizeof(T), IP = sizeof(T) == 8 ? 1 : 2, JP = sizeof(T) == 2 ? 2 : 1;      // matrix tiles that 8 KiB hold
         constexpr int RB = IP * 32 * sizeof(T), L = RB / 16;                                             // bytes and pieces of a column
@@ -984,21 +987,37 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
                                 for (int e = 0; e < 4; e += E) *(uint4*)(at + (((byte >> 4) + e / E) ^ key) * 16) = *(const uint4*)(u + e);
                         }
                 __builtin_amdgcn_wave_barrier();                // (a wave's LDS accesses stay in order)
-                const int s = lane % L;
+                const int s = lane % L, so = j0 * 32 * mstep + i0 * 32 * S;
+                // entries of mirror row c that exist: the first ones, up to `limit`
+                auto limit_of = [&](int c) {
+                    const int col = j0 * 32 + c;
+                    int limit = rows;
+                    if (diagonal) limit = min(limit, col + ahead);
+                    return col < cols ? limit - i0 * 32 : 0;
+                };
+                if (aligned) {
 #pragma unroll 4
-                for (int n = 0; n < JP * L / 2; ++n) {
-                    const int c = n * (64 / L) + lane / L, key = sizeof(T) == 2 ? (c >> 1) & 7 : c & 15, col = j0 * 32 + c;
-                    const uint4 u = *(const uint4*)(room + c * RB + ((s ^ key) << 4));
-                    const int off = c * mstep + s * 16, so = j0 * 32 * mstep + i0 * 32 * S;
-                    if (whole) put16(u, M, off, so);
-                    else {
-                        int limit = rows;
-                        if (diagonal) limit = min(limit, col + ahead);
-                        if (col >= cols) limit = 0;
+                    for (int n = 0; n < JP * L / 2; ++n) {
+                        const int c = n * (64 / L) + lane / L, key = sizeof(T) == 2 ? (c >> 1) & 7 : c & 15;
+                        const uint4 u = *(const uint4*)(room + c * RB + ((s ^ key) << 4));
+                        put16(u, M, whole || (s + 1) * E <= limit_of(c) ? so + c * mstep + s * 16 : -1);
+                    }
+                    if (!whole) {      // the piece that a row ends in: one lane for each row
+                        const int c = lane & (JP * 32 - 1), key = sizeof(T) == 2 ? (c >> 1) & 7 : c & 15;
+                        const int limit = lane < JP * 32 ? min(limit_of(c), IP * 32) : 0, last = max(limit, 0) / E;
                         T v[E] __attribute__((aligned(16)));
-                        *(uint4*)v = u;
+                        *(uint4*)v = *(const uint4*)(room + c * RB + (((last & (L - 1)) ^ key) << 4));
 #pragma unroll
-                        for (int e = 0; e < E; ++e) put<T>(v[e], M, i0 * 32 + s * E + e < limit ? off + e * S : -1, so);
+                        for (int e = 0; e < E; ++e) put<T>(v[e], M, last * E + e < limit ? c * mstep + last * 16 + e * S : -1, so);
+                    }
+                } else {
+#pragma unroll 2
+                    for (int n = 0; n < JP * L / 2; ++n) {
+                        const int c = n * (64 / L) + lane / L, key = sizeof(T) == 2 ? (c >> 1) & 7 : c & 15;
+                        T v[E] __attribute__((aligned(16)));
+                        *(uint4*)v = *(const uint4*)(room + c * RB + ((s ^ key) << 4));
+#pragma unroll
+                        for (int e = 0; e < E; ++e) put<T>(v[e], M, s * E + e < limit_of(c) ? c * mstep + s * 16 + e * S : -1, so);
                     }
                 }
                 __builtin_amdgcn_wave_barrier();
