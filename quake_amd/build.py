@@ -36,6 +36,8 @@ def build_library(force: bool = False, verbose: bool = True, extra_flags=()) -> 
     objdir.mkdir(exist_ok=True)
     flags = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", f"-I{INCLUDE}", f"-I{CSRC}",
              "-Wall", "-Wno-unused-function", *extra_flags]
+    # no packed FP32 arithmetic: the compiler must not form it from pairs of ordinary float operations
+    flags += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     # qk_wave.hip keeps a statevector in registers across a large scalar dispatch; two middle-end transforms
     # defeat that (common-code sinking merges the per-qubit arms into pointer selects, the AMDGPU alloca-to-vector
     # pass turns the amplitude array into one 32-register tuple): both off for that file
@@ -47,9 +49,7 @@ def build_library(force: bool = False, verbose: bool = True, extra_flags=()) -> 
     uniform_flow = keep_in_regs + ["-mllvm", "-structurizecfg-skip-uniform-regions"]
     # (the LDS simulator's stage dispatch gains a few per cent from the same switch: 16 qubits ZZ r = 2 3.10 -> 3.02 ms per 4 GiB;
     # the Gram and projected-kernel files compile to the same code with and without it and are left alone)
-    per_file = {"qk_wave.hip": uniform_flow, "qk_reg.hip": uniform_flow, "qk_sim.hip": ["-mllvm", "-structurizecfg-skip-uniform-regions"],
-                # no packed FP32 arithmetic: the compiler must not form it from pairs of ordinary float operations
-                "qk_fp8.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
+    per_file = {"qk_wave.hip": uniform_flow, "qk_reg.hip": uniform_flow, "qk_sim.hip": ["-mllvm", "-structurizecfg-skip-uniform-regions"]}
     procs = []
     for s in SOURCES:
         obj = objdir / (s.rsplit(".", 1)[0] + ".o")
