@@ -794,6 +794,19 @@ template <bool NATIVE> struct TilePipe {
         }
     }
 
+    // Of two workgroups on a CU the matrix unit serves the older one first; left alone, one is through its tile in half the
+    // other's time, and the workgroups that share rows in L2 drift apart.  Every 4 steps a wave goes down one level of four and
+    // then back to the highest, so the one behind has the higher level most of the time (12000 rows of 65536 amplitudes, half K:
+    // 16.4 -> 14.8 ms; 8192 of 4096: 470 -> 423 us, float32 820 -> 783; turns of 1, 2, 8 or 16 steps within 2 % of that.  The level
+    // changes before the barrier of a step: behind it 15.3 ms).
+    __device__ __forceinline__ void turn(int c) {
+        const int t = (c >> 2) & 3;
+        if (t == 0) __builtin_amdgcn_s_setprio(3);
+        else if (t == 1) __builtin_amdgcn_s_setprio(2);
+        else if (t == 2) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+    }
+
     // work(k, w): the k-th piece of this workgroup's work, false behind the last.  finish(k, more, gains, room, side, re, im): more: the next
     // one is open; room: 8 KiB of LDS for this wave, the buffer of the last chunk.  STORES: finish issues at least 63 memory
     // instructions.  ASIDE: instead of the next tile's first chunk, aside(k, buffer) fills the free buffer while the last chunk is
@@ -818,9 +831,11 @@ template <bool NATIVE> struct TilePipe {
             int c = w.c0;
             const int c1 = w.c1;
             area = next_area;
+            turn(c);
             for (; c + 1 < c1; ++c) {
                 compute<true>(c, re, im);
                 buf ^= 1;
+                if (!((c + 1) & 3)) turn(c + 1);
                 __builtin_amdgcn_sched_barrier(0);      // (matrix instructions that sink behind the barrier would not hide it)
                 // the copies of the next chunk have landed, and every wave has read the buffer that is filled after it
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -1380,13 +1395,13 @@ constexpr int64_t slots(Gram8Kind kind) { return kind == GK_WAVE ? 1024 : kind =
 // Which of a job's tiles are cut into slices of their rows, and into how many: those of the last round over the chip's slots,
 // where cutting brings more than it costs.  Measured: a step (a chunk of a tile) takes 3.0 us with all slots busy (fp8 1.7;
 // 32 x 32 tiles 0.4), joining a call's slices 5 us and what writing and reading them takes at 5 TB/s.
-void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double rest, Gram8JobDev& d) {
+void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double behind, Gram8JobDev& d) {
     const int64_t all = slots(kind), side = kind < GK_TILE ? 32 : kTile, last = (taken + live) % all, tail = std::min(live, last);
     const double step = kind < GK_TILE ? 0.4 : kind == GK_TILE_NATIVE ? 1.7 : 3.0;
     d.whole = (uint32_t)live;
     d.slices = 1;
     d.per = chunks;
-    if (tail == 0 || rest >= 0.5 * (double)((all - last) * chunks)) return;      // the jobs behind it fill the round
+    if (tail == 0 || behind >= 0.5 * (double)((all - last) * chunks)) return;      // the jobs behind it fill the round
     double best = (double)chunks * step;
     const int most = std::min(kind < GK_TILE ? chunks / 16 : chunks / 4, 256);
     for (int n = 2; n <= most; ++n) {
@@ -1421,10 +1436,16 @@ int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind
         d.tiles_m = (int32_t)((j.A.rows + side - 1) / side);
         d.tiles_n = (int32_t)((j.B.rows + side - 1) / side);
         const int64_t live = live_tiles(j, side);
-        // what the jobs behind this one (shorter rows) bring to the slots that its last tiles leave free, in steps
-        double rest = 0;
-        for (int l = k + 1; l < n; ++l) rest += (double)live_tiles(jobs[which[l]], side) * (double)((jobs[which[l]].D + kChunk - 1) / kChunk);
-        cut(kind, live, d.chunks, items % slots(kind), rest, d);
+        // what the jobs behind this one (shorter rows) bring to the slots that its last tiles leave free in their round, in steps
+        double behind = 0;
+        const int64_t taken = items % slots(kind);
+        int64_t room = slots(kind) - (taken + live) % slots(kind);
+        for (int l = k + 1; l < n && room; ++l) {
+            const int64_t some = std::min(room, live_tiles(jobs[which[l]], side));
+            behind += (double)some * (double)((jobs[which[l]].D + kChunk - 1) / kChunk);
+            room -= some;
+        }
+        cut(kind, live, d.chunks, taken, behind, d);
         if (items + live * d.slices > 0x7fffffffLL) return fail(QK_ERR_UNSUPPORTED, "qk_gram8_jobs_dev: too many tiles; split the call");
         d.live = (uint32_t)live;
         d.begin = (uint32_t)items;
