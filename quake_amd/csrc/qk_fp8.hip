@@ -289,7 +289,8 @@ struct Gram8JobDev {
     int32_t chunks;            // chunks per row
     int32_t sb;                // scale bytes per row
     int32_t tiles_m, tiles_n;  // tile rows and columns
-    int32_t slices;            // the tiles behind the first `whole` are cut into this many slices of `per` chunks
+    int32_t slices;            // the tiles behind the first `whole` are cut into this many slices of `per` chunks,
+    int32_t small;             // or (1) into 16 tiles of 32 x 32
     int32_t per;
     uint32_t live;             // tiles that have to be computed
     uint32_t whole;
@@ -300,6 +301,7 @@ struct Gram8Args {
     Gram8JobDev job[kGram8Jobs];
     int32_t n_jobs;
     uint32_t total;            // items
+    uint32_t small;            // the items from here on are 32 x 32 tiles of the last job (launches of 128 x 128 tiles)
     float* ws;
 };
 static_assert(sizeof(Gram8Args) <= 4096, "kernel arguments");
@@ -442,23 +444,16 @@ __device__ __forceinline__ void wave_product(const uint8_t* pa, const uint8_t* s
     }
 }
 
-// A 32 x 32 tile per workgroup, the chunks of its slice dealt to four waves, their sums joined in LDS.
-__global__ __launch_bounds__(256, 3) void gram8_wave_kernel(Gram8Args args) {
+// A 32 x 32 tile of a job by four waves: chunks c0 .. c1 - 1 dealt to them, their sums joined in LDS; the entries, or (ws) a
+// slice's sums.
+__device__ __forceinline__ void wave_tile(const Gram8JobDev& J, int64_t row, int64_t col, int c0, int c1, float (*part)[32][64], float2* ws) {
     constexpr int W = 4;
-    __shared__ float part[W][32][64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, h = lane >> 5;
-    const uint32_t item = blockIdx.x;
-    const Gram8JobDev& J = args.job[gram8_job(args, item)];
-    uint32_t t, ti, tj;
-    int slice;
-    gram8_part(J, item - J.begin, t, slice);
-    gram8_tile(J, t, ti, tj);
     const int64_t cb = (int64_t)J.chunks * kChunkBytes;
-    const int64_t ra = min((int64_t)ti * 32 + r, J.A.n - 1), rb = min((int64_t)tj * 32 + r, J.B.n - 1);
+    const int64_t ra = min(row + r, J.A.n - 1), rb = min(col + r, J.B.n - 1);
     v16f re, im;
 #pragma unroll
     for (int i = 0; i < 16; ++i) re[i] = im[i] = 0.f;
-    const int c0 = max(slice, 0) * J.per, c1 = slice < 0 ? J.chunks : min(J.chunks, c0 + J.per);
     wave_product(J.A.codes + ra * cb + 16 * h, J.A.scales + ra * J.sb, J.B.codes + rb * cb + 16 * h, J.B.scales + rb * J.sb, c0 + wave,
                  c1, W, re, im);
 #pragma unroll
@@ -476,13 +471,22 @@ __global__ __launch_bounds__(256, 3) void gram8_wave_kernel(Gram8Args args) {
             x += part[w][i][lane];
             y += part[w][16 + i][lane];
         }
-        if (slice < 0) {
-            emit(J, (int64_t)ti * 32 + acc_row(lane, i), (int64_t)tj * 32 + r, x, y);
-        } else {
-            float2* ws = (float2*)(args.ws + J.ws) + ((int64_t)(t - J.whole) * J.slices + slice) * 1024;
-            ws[i * 64 + lane] = make_float2(x, y);
-        }
+        if (ws) ws[i * 64 + lane] = make_float2(x, y);
+        else emit(J, row + acc_row(lane, i), col + r, x, y);
     }
+}
+
+__global__ __launch_bounds__(256, 3) void gram8_wave_kernel(Gram8Args args) {
+    __shared__ float part[4][32][64];
+    const uint32_t item = blockIdx.x;
+    const Gram8JobDev& J = args.job[gram8_job(args, item)];
+    uint32_t t, ti, tj;
+    int slice;
+    gram8_part(J, item - J.begin, t, slice);
+    gram8_tile(J, t, ti, tj);
+    const int c0 = max(slice, 0) * J.per, c1 = slice < 0 ? J.chunks : min(J.chunks, c0 + J.per);
+    wave_tile(J, (int64_t)ti * 32, (int64_t)tj * 32, c0, c1, part,
+              slice < 0 ? nullptr : (float2*)(args.ws + J.ws) + ((int64_t)(t - J.whole) * J.slices + slice) * 1024);
 }
 
 // ---- few rows against many ---------------------------------------------------------------------------------------------
@@ -900,11 +904,16 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
     TilePipe<NATIVE> pipe(lds);
     const int wave = pipe.wave, lane = pipe.lane, r = pipe.r, h = pipe.h;
     struct Where { int job; uint32_t t, ti, tj; int slice; } now{}, before{};      // of the tile that was opened last and the one before
-    auto work = [&](int k, TileWork& w) {
-        uint32_t item;
+    int round = 0;
+    auto item_of = [&](int k, uint32_t& item) {
         // every other round backwards: the list goes from long rows to short ones
         const uint32_t in = k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-        if (!gram8_item(args.total, in + (uint32_t)k * gridDim.x, item)) return false;
+        return gram8_item(args.total, in + (uint32_t)k * gridDim.x, item);
+    };
+    auto work = [&](int k, TileWork& w) {
+        uint32_t item;
+        round = k;
+        if (!item_of(k, item) || item >= args.small) return false;
         before = now;
         Where& p = now;
         p.job = uniform(gram8_job(args, item));
@@ -1039,6 +1048,18 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
             }
     };
     pipe.template run<true>(work, finish);
+    // the last round in small tiles
+    for (uint32_t item; item_of(round, item) && item >= args.small; ++round) {
+        const Gram8JobDev& J = args.job[args.n_jobs - 1];
+        uint32_t t, ti, tj;
+        int slice;
+        gram8_part(J, item - J.begin, t, slice);
+        gram8_tile(J, t, ti, tj);
+        const int64_t row = (int64_t)ti * kTile + (slice >> 2) * 32, col = (int64_t)tj * kTile + (slice & 3) * 32;
+        if (row >= J.A.n || col >= J.B.n || ((J.flags & QK_GRAM_SYMMETRIC) && row > col)) continue;
+        __syncthreads();
+        wave_tile(J, row, col, 0, J.chunks, (float (*)[32][64])lds, nullptr);
+    }
 }
 
 // Adds the slices of every tile in order and finishes its entries: one thread per entry.  SUB: matrix tiles per tile (1 or 16).
@@ -1394,12 +1415,14 @@ constexpr int64_t slots(Gram8Kind kind) { return kind == GK_WAVE ? 1024 : kind =
 
 // Which of a job's tiles are cut into slices of their rows, and into how many: those of the last round over the chip's slots,
 // where cutting brings more than it costs.  Measured: a step (a chunk of a tile) takes 3.0 us with all slots busy (fp8 1.7;
-// 32 x 32 tiles 0.4), joining a call's slices 5 us and what writing and reading them takes at 5 TB/s.
-void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double behind, Gram8JobDev& d) {
+// 32 x 32 tiles 0.4), joining a call's slices 5 us and what writing and reading them takes at 5 TB/s.  second: the call's last
+// tiles are in the second round.
+void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double behind, bool second, Gram8JobDev& d) {
     const int64_t all = slots(kind), side = kind < GK_TILE ? 32 : kTile, last = (taken + live) % all, tail = std::min(live, last);
     const double step = kind < GK_TILE ? 0.4 : kind == GK_TILE_NATIVE ? 1.7 : 3.0;
     d.whole = (uint32_t)live;
     d.slices = 1;
+    d.small = 0;
     d.per = chunks;
     if (tail == 0 || behind >= 0.5 * (double)((all - last) * chunks)) return;      // the jobs behind it fill the round
     double best = (double)chunks * step;
@@ -1415,12 +1438,21 @@ void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double behind,
             d.whole = (uint32_t)(live - tail);
         }
     }
+    // Few tiles of short rows behind one full round: as 32 x 32 tiles they take one step of every workgroup.  (4096 rows of 256
+    // amplitudes, 528 tiles: half K 24.5 -> 21.8 us, float32 37.5 -> 30.0; 46 tiles over 20.0 against 19.6 us, 128 tiles 19.7 against
+    // 29.5; behind four rounds, where the workgroups are out of step, 53.7 against 54.5.)
+    if (second && kind >= GK_TILE && d.slices == 1 && chunks <= 8 && last <= live && 16 * tail <= all) {
+        d.small = 1;
+        d.slices = 16;
+        d.whole = (uint32_t)(live - tail);
+    }
 }
 
 int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind, Gram8Plan& p) {
     std::memset(&p, 0, sizeof(p));
     const int64_t side = kind < GK_TILE ? 32 : kTile;
     int64_t items = 0;
+    p.args.small = 0xffffffffu;
     for (int k = 0; k < n; ++k) {
         const qk_gram8_job& j = jobs[which[k]];
         Gram8JobDev& d = p.args.job[p.args.n_jobs++];
@@ -1445,12 +1477,13 @@ int plan_gram8(const qk_gram8_job* jobs, const int* which, int n, Gram8Kind kind
             behind += (double)some * (double)((jobs[which[l]].D + kChunk - 1) / kChunk);
             room -= some;
         }
-        cut(kind, live, d.chunks, taken, behind, d);
+        cut(kind, live, d.chunks, taken, behind, k == n - 1 && items + live > slots(kind) && items + live < 2 * slots(kind), d);
         if (items + live * d.slices > 0x7fffffffLL) return fail(QK_ERR_UNSUPPORTED, "qk_gram8_jobs_dev: too many tiles; split the call");
         d.live = (uint32_t)live;
         d.begin = (uint32_t)items;
         items += d.whole + (live - d.whole) * d.slices;
-        if (d.whole < live) {
+        if (d.small) p.args.small = d.begin + d.whole;
+        else if (d.whole < live) {
             d.ws = (int64_t)p.ws_floats;
             p.ws_floats += (size_t)(live - d.whole) * d.slices * 2 * side * side;
             p.join_tiles += (uint32_t)(live - d.whole);

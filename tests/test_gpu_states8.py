@@ -172,6 +172,25 @@ def test_gram8_larger(M, N, D, dtype, path):
 
 
 @pytest.mark.parametrize("dtype", list(NP))
+@pytest.mark.parametrize("N,M,D", [(4001, 0, 64), (4090, 0, 200), (4096, 0, 300), (2011, 4195, 60), (4195, 2011, 130), (16, 4096, 16)])
+def test_gram8_a_full_round_and_a_few_tiles(N, M, D, dtype):
+    """Up to 32 tiles of 128 x 128 behind the first 512 (another shape of the last tiles); beside a job that comes first too."""
+    rng = np.random.default_rng(N + D)
+    x, a, ga = fill(S8.states(rng, N, D, "product"))
+    if not M:
+        check_k(qdev.gram8(x, dtype=dtype), a, ga, a, ga, symmetric=True)
+        return
+    y, b, gb = fill(S8.states(rng, M, D, "spread"))
+    z, c, gc = fill(S8.states(rng, 140, 256))
+    KT = torch.full((M, N), -3.0, dtype=dtype, device="cuda")
+    KZ, K = qdev.gram8_jobs([dict(A=z), dict(A=x, B=y, KT=KT)], dtype=dtype)
+    check_k(KZ, c, gc, c, gc, symmetric=True)
+    check_k(K, a, ga, b, gb)
+    assert torch.equal(KT, K.T)
+    check_k(qdev.gram8(x, y, dtype=dtype), a, ga, b, gb)
+
+
+@pytest.mark.parametrize("dtype", list(NP))
 def test_gram8_writes_its_block_only(dtype, path):
     rng = np.random.default_rng(8)
     x, a, ga = fill(S8.states(rng, 150, 256))
