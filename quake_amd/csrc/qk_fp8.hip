@@ -1681,10 +1681,10 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
     return gram8_launches(jobs, n_jobs, [&](Gram8Plan& p, Gram8Kind kind) {
         p.args.ws = (float*)ws;
         const uint32_t total = p.args.total, full = total >> 6;
-        // two workgroups per CU that stay, or, for long rows, one for each item: the hardware then starts neighbours together, and they
-        // keep sharing rows in L2 (12000 rows: 16384 amplitudes 4.37 against 4.12 ms, 65536 20.3 against 17.3; 4096 rows of 4096
-        // amplitudes the same; 256 amplitudes 27.5 against 28.4 us)
-        const dim3 dealt(std::min<uint32_t>(p.args.job[0].chunks > 64 ? 0x7fffffffu : 512u, (full << 6) + 8 * ((total - (full << 6) + 7) >> 3)));      // two workgroups per CU
+        // two workgroups per CU that stay (one for each item: 5000 x 7001 rows of 64 amplitudes, half K 33 against 29.4 us; rows of 1024
+        // and more within 2 %); where the last round is of small tiles, one for each item: those start wherever one ends (4096 rows
+        // of 256 amplitudes, float32 30.6 -> 28.0 us)
+        const dim3 dealt(std::min<uint32_t>(p.args.small < total ? 0x7fffffffu : 512u, (full << 6) + 8 * ((total - (full << 6) + 7) >> 3)));
         if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, dim3(total), dim3(256), 0, s, p.args);
         else if (kind == GK_THIN8) QK_THIN8(8, false);
         else if (kind == GK_THIN8_SWAP) QK_THIN8(8, true);
