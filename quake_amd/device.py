@@ -261,7 +261,7 @@ class States8:
         code, scale = cls._layout(dim)
         rows = gains.numel()
         if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or gains.dtype is not torch.float32 \
-                or gains.shape != (rows,) or codes.shape != (rows, code) or scales.shape != (rows, scale) \
+                or gains.dim() != 1 or codes.shape != (rows, code) or scales.shape != (rows, scale) \
                 or not (codes.is_contiguous() and scales.is_contiguous() and gains.is_contiguous()):
             raise ValueError("need contiguous codes uint8 [rows, 128 ceil(dim / 64)], scales uint8 [rows, 4 ceil(dim / 512)], "
                              "gains float32 [rows]")
@@ -344,10 +344,6 @@ class States8:
 _K8_FLAGS = {torch.float32: 0, torch.float16: _lib.QK_GRAM8_F16, torch.float64: _lib.QK_GRAM8_F64}
 
 
-def _padded(entries: int) -> int:
-    return (entries + 127) & ~127
-
-
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -356,15 +352,15 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
     """Fidelity kernels of several pairs of 8-bit stores in one call (one launch for up to 24 of them), every job with its
     own rows and its own dim: the kernels of a population.  Each job: dict(A=, B=None, K=None, KT=None) with A, B
     :class:`States8`; B is None: the symmetric kernel of A with an exact unit diagonal.  K (allocated as ``dtype`` if not
-    given, several of them in one allocation) and KT, the transposed copy (not for symmetric jobs): float32, float16 or float64 [len(A), len(B)] views with unit
-    column stride.  Returns the Ks."""
+    given, several of them in one allocation) and KT, the transposed copy (not for symmetric jobs): float32, float16 or
+    float64 [len(A), len(B)] views with unit column stride.  Returns the Ks."""
     if not jobs:
         return []
     if dtype not in _K8_FLAGS:
         raise ValueError("K must be float32, float16 or float64")
-    packed, Ks, gpu, device, flat, used = [], [], None, None, None, 0
+    several, pairs, gpu, entries = len(jobs) > 1, [], None, 0
     for j in jobs:
-        A, B, K, KT = j["A"], j.get("B"), j.get("K"), j.get("KT")
+        A, B, K = j["A"], j.get("B"), j.get("K")
         sym = B is None
         if sym:
             B = A
@@ -376,16 +372,19 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
             gpu, device = A._gpu, A.codes.device
         if A._gpu != gpu or B._gpu != gpu:
             raise ValueError("stores on different GPUs")
+        if K is None:
+            entries += (A._rows * B._rows + 127) & ~127
+        pairs.append((A, B, sym, K, j.get("KT")))
+    flat, used = torch.empty(entries, dtype=dtype, device=device) if several and entries else None, 0
+    packed, Ks = [], []
+    for A, B, sym, K, KT in pairs:
         m, n = A._rows, B._rows
         if K is None:
-            if len(jobs) == 1:
+            if flat is None:
                 K = torch.empty((m, n), dtype=dtype, device=device)
             else:                       # views of one allocation, which lives as long as any of them
-                if flat is None:
-                    flat = torch.empty(sum(_padded(len(j["A"]) * len(j["A" if j.get("B") is None else "B"])) for j in jobs
-                                           if j.get("K") is None), dtype=dtype, device=device)
                 K = flat.as_strided((m, n), (n or 1, 1), used)
-                used += _padded(m * n)
+                used += (m * n + 127) & ~127
             ldk = n or 1
         else:
             K = from_dlpack(K)
