@@ -227,8 +227,8 @@ class States8:
 
     ``codes`` uint8 [capacity, 128 * ceil(dim / 64)], ``scales`` uint8 [capacity, 4 * ceil(dim / 512)] and ``gains`` float32
     [capacity] are plain tensors (layout and formulas: ``qk_states8`` in quake_hip.h); ``len(store)`` rows are written.  A
-    component is off by at most 2^-4 of itself, the fidelity of two states by up to 0.13 in the worst case and by about
-    0.07 sqrt(K / dim) for states spread over their ``dim`` amplitudes."""
+    component is off by at most 2^-4 of itself (or, where that is more, 2^-17 of the largest in its block), the fidelity of two
+    states by up to 0.13 in the worst case and by about 0.07 sqrt(K / dim) for states spread over their ``dim`` amplitudes."""
 
     def __init__(self, capacity: int, dim: int, device=None):
         code, scale = self._layout(dim)
