@@ -1258,7 +1258,7 @@ template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_ke
     };
     if constexpr (MANY) {
         auto aside = [&](int k, uint8_t* to) {
-            // element n of the tile's [128][C]: rows behind the last repeat it (their K is 0)
+            // element n of the tile's [128][C]: rows behind the last repeat it
             const int64_t y0 = (int64_t)(t0 + k) * kTile;
             const int last = (int)min((int64_t)kTile, a.B.n - y0) - 1, total = kTile * a.C, dr = 256 / a.C, dc = 256 - dr * a.C;
             int row = tid / a.C, c = tid - row * a.C;
@@ -1274,6 +1274,7 @@ template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_ke
         };
         auto finish = [&](int k, bool, const float* gains, uint8_t*, const uint8_t* side, v16f (&re)[2][2], v16f (&im)[2][2]) {
             kernel(k, gains, re, im);
+            const int left = (int)min((int64_t)64, a.B.n - (int64_t)(t0 + k) * kTile - ys) - 4 * h;
             for (int c0 = 0; c0 < a.C; c0 += 32) {
                 const int n = a.C - c0 - 4 * h;
                 float* const at = a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + 4 * h) * mp + row0 + xs + r;
@@ -1293,7 +1294,8 @@ template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_ke
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int q = 0; q < 16; ++q) {
-                        const float w = coef[(i * 32 + 8 * (q >> 2) + (q & 3)) * a.C];
+                        const int row = i * 32 + 8 * (q >> 2) + (q & 3);
+                        const float v = coef[row * a.C], w = row < left ? v : 0.f;
 #pragma unroll
                         for (int j = 0; j < 2; ++j) sum[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(w, re[i][j][q], sum[j], 0, 0, 0);
                     }
@@ -1310,9 +1312,13 @@ template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_ke
     } else {
         auto finish = [&](int k, bool, const float* gains, uint8_t* room, const uint8_t*, v16f (&re)[2][2], v16f (&im)[2][2]) {
             float* const coef = (float*)room;
-            const int64_t y = min((int64_t)(t0 + k) * kTile + ys + lane, a.B.n - 1);
+            // (0 behind B's last row: K is 0 there, and an infinite coefficient must not meet it)
+            const int64_t at = (int64_t)(t0 + k) * kTile + ys + lane, y = min(at, a.B.n - 1);
 #pragma unroll 4
-            for (int c = 0; c < a.C; ++c) coef[c * 64 + lane] = a.coef[y * a.ldc + c];
+            for (int c = 0; c < a.C; ++c) {
+                const float v = a.coef[y * a.ldc + c];
+                coef[c * 64 + lane] = at == y ? v : 0.f;
+            }
             kernel(k, gains, re, im);
             __builtin_amdgcn_wave_barrier();
             for (int c = 0; c < a.C; ++c) {

@@ -285,6 +285,20 @@ def test_decision8(M, N, D, C, path):
     assert (out[0] == -3).all() and (out[M + 1] == -3).all() and (out[:, :2] == -3).all() and (out[:, 2 + C:] == -3).all()
 
 
+@pytest.mark.parametrize("M,N,D,C", [(70, 200, 64, 1), (70, 200, 64, 3), (70, 193, 64, 45), (3, 33, 1024, 2)])
+def test_decision8_infinite_coefficients(M, N, D, C, path):
+    """An infinite coefficient of the last row, whose place behind the end of a tile must not meet a zero."""
+    rng = np.random.default_rng(M + C)
+    x, y = fill(S8.states(rng, M, D, "product")), fill(S8.states(rng, N, D, "spread"))
+    coef = rng.normal(size=(N, C)).astype(np.float32)
+    coef[-1, 0] = np.inf
+    out = qdev.decision8(x[0], y[0], torch.from_numpy(coef).cuda())
+    assert (S8.kernel(x[1], x[2], y[1], y[2])[0][:, -1] > 0).all()
+    assert torch.isposinf(out[:, 0]).all()
+    if C > 1:
+        check_decision(out[:, 1:], x, y, coef[:, 1:], None)
+
+
 def test_decision8_empty_sides():
     x, y = fill(S8.states(np.random.default_rng(1), 9, 32)), fill(S8.states(np.random.default_rng(2), 4, 32))
     b = torch.tensor([1.5, -2.0], device="cuda")
