@@ -37,6 +37,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 constexpr int kChunk = 64;            // amplitudes per chunk
 constexpr int kChunkBytes = 128;
 constexpr int kBlock = 128;           // amplitudes per scale
+constexpr int64_t kThreads = 0xffffffffLL;      // of a launch: one with more does not fail, it wraps around
 constexpr int kGram8Jobs = 24;        // jobs of one launch (their records travel as kernel arguments: under 4 KiB)
 
 static inline int64_t code_bytes(int64_t D) { return (D + kChunk - 1) / kChunk * kChunkBytes; }
@@ -307,6 +308,7 @@ struct Gram8Args {
     Gram8JobDev job[kGram8Jobs];
     int32_t n_jobs;
     uint32_t total;            // items
+    uint32_t first;            // item of the launch's first workgroup (32 x 32 tiles)
     uint32_t small;            // the items from here on are 32 x 32 tiles of the last job (launches of 128 x 128 tiles)
     float* ws;
 };
@@ -486,7 +488,7 @@ __device__ __forceinline__ void wave_tile(const Gram8JobDev& J, int64_t row, int
 // from call to call; 24 kernels of 100 rows and 16 to 1024 amplitudes 9 to 15 us.
 __global__ __launch_bounds__(256, 3) void gram8_wave_kernel(Gram8Args args) {
     __shared__ float part[4][32][64];
-    const uint32_t item = blockIdx.x;
+    const uint32_t item = args.first + blockIdx.x;
     const Gram8JobDev& J = args.job[gram8_job(args, item)];
     uint32_t t, ti, tj;
     int slice;
@@ -596,7 +598,7 @@ template <int AR, bool SWAP> __global__ __launch_bounds__(256) void gram8_thin_k
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     ThinPipe<AR, S> pipe(lds + wave * S * ThinPipe<AR, S>::kBytes);
     const int lane = pipe.lane, r = pipe.r;
-    const uint32_t item = blockIdx.x;
+    const uint32_t item = args.first + blockIdx.x;
     const Gram8JobDev& J = args.job[gram8_job(args, item)];
     uint32_t t, ti, tj;
     int slice;
@@ -1357,19 +1359,23 @@ template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_ke
 __global__ __launch_bounds__(256) void decision8_join_kernel(Decision8Args a) {
     __shared__ double sum[16][17];
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.y;
-    const int64_t row = (int64_t)blockIdx.x * 16 + x;
-    double s = 0.0;
-    if (row < a.A.n) {
+    for (int64_t row0 = (int64_t)blockIdx.x * 16; row0 < a.A.n; row0 += (int64_t)gridDim.x * 16) {
+        const int64_t row = row0 + x;
+        double s = 0.0;
+        if (row < a.A.n) {
 #pragma unroll 4
-        for (int p = y; p < a.parts; p += 16) s += (double)a.ws[((int64_t)p * a.C + c) * a.stride + row];
-    }
-    sum[y][x] = s;
-    __syncthreads();
-    if (y || row >= a.A.n) return;
-    s = a.intercept ? (double)a.intercept[c] : 0.0;
+            for (int p = y; p < a.parts; p += 16) s += (double)a.ws[((int64_t)p * a.C + c) * a.stride + row];
+        }
+        sum[y][x] = s;
+        __syncthreads();
+        if (y == 0 && row < a.A.n) {
+            s = a.intercept ? (double)a.intercept[c] : 0.0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += sum[k][x];
-    a.out[row * a.ldo + c] = (float)s;
+            for (int k = 0; k < 16; ++k) s += sum[k][x];
+            a.out[row * a.ldo + c] = (float)s;
+        }
+        __syncthreads();
+    }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
@@ -1607,14 +1613,18 @@ extern "C" int qk_states8_write_dev(const void* psi, int f32, int64_t ldpsi, int
     const hipStream_t s = (hipStream_t)stream;
     // a wave takes two blocks at a time: one wave per row up to 8 blocks, sixteen for the longest rows
     const int wpr = blocks <= 8 ? 1 : blocks <= 64 ? 4 : 16;
-    const int64_t grid = wpr == 1 ? (N + 3) / 4 : N;
-    if (grid > 0x7fffffffLL) return fail(QK_ERR_UNSUPPORTED, std::string(who) + ": too many rows");
-#define QK_WRITE8(T, W) \
-    hipLaunchKernelGGL((states8_write_kernel<T, W>), dim3((unsigned)grid), dim3(W < 4 ? 256 : 64 * W), 0, s, psi, N, D, ldpsi, codes, scales, gains)
-    if (f32) {
-        if (wpr == 1) QK_WRITE8(float, 1); else if (wpr == 4) QK_WRITE8(float, 4); else QK_WRITE8(float, 16);
-    } else {
-        if (wpr == 1) QK_WRITE8(double, 1); else if (wpr == 4) QK_WRITE8(double, 4); else QK_WRITE8(double, 16);
+    const int rows = wpr == 1 ? 4 : 1, threads = wpr == 16 ? 1024 : 256;      // of a workgroup
+    const int64_t most = kThreads / threads * rows, cb = code_bytes(D), sb = scale_bytes(D);
+#define QK_WRITE8(T, W)                                                                                                       \
+    hipLaunchKernelGGL((states8_write_kernel<T, W>), dim3((unsigned)((n + rows - 1) / rows)), dim3(threads), 0, s,            \
+                       (const char*)psi + first * ldpsi * (f32 ? 8 : 16), n, D, ldpsi, codes + first * cb, scales + first * sb, gains + first)
+    for (int64_t first = 0; first < N; first += most) {
+        const int64_t n = std::min(most, N - first);
+        if (f32) {
+            if (wpr == 1) QK_WRITE8(float, 1); else if (wpr == 4) QK_WRITE8(float, 4); else QK_WRITE8(float, 16);
+        } else {
+            if (wpr == 1) QK_WRITE8(double, 1); else if (wpr == 4) QK_WRITE8(double, 4); else QK_WRITE8(double, 16);
+        }
     }
 #undef QK_WRITE8
     QK_HIP(hipGetLastError());
@@ -1636,7 +1646,7 @@ extern "C" int qk_states8_read_dev(const qk_states8* from, int64_t D, const int6
     const bool longer = D >= 512;
     const int64_t rows = std::max<int64_t>(1, kReadPairs / ((D + 1) / 2)), segments = (D + 511) / 512;
     const int64_t grid = longer ? (N * segments + 3) / 4 : (N + rows - 1) / rows;
-    if (grid > 0x1fffffffLL) return fail(QK_ERR_UNSUPPORTED, std::string(who) + ": too many amplitudes; split the call");
+    if (grid > kThreads / 256) return fail(QK_ERR_UNSUPPORTED, std::string(who) + ": too many amplitudes; split the call");
     const uint8_t *codes = (const uint8_t*)from->codes, *scales = (const uint8_t*)from->scales;
     const bool vec = !((uintptr_t)psi & 15) && (ldpsi * (f32 ? 8 : 16)) % 16 == 0;
     const dim3 g((unsigned)grid), b(256);
@@ -1686,7 +1696,7 @@ template <typename K, typename A> int launch8(K kernel, dim3 grid, int lds, hipS
     do {                                                                                                             \
         static DeviceOnce once;                                                                                      \
         constexpr int lds8 = AR == 8 ? kThinLds8 : kThinLds32;                                                       \
-        const int rc8 = launch8(gram8_thin_kernel<AR, SWAP>, dim3(total), lds8, s, p.args, once, lds8);              \
+        const int rc8 = launch8(gram8_thin_kernel<AR, SWAP>, some, lds8, s, p.args, once, lds8);                     \
         if (rc8) return rc8;                                                                                         \
     } while (0)
 
@@ -1708,11 +1718,16 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
         // and more within 2 %); where the last round is of small tiles, one for each item: those start wherever one ends (4096 rows
         // of 256 amplitudes, float32 30.6 -> 28.0 us)
         const dim3 dealt(std::min<uint32_t>(p.args.small < total ? 0x7fffffffu : 512u, (full << 6) + 8 * ((total - (full << 6) + 7) >> 3)));
-        if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, dim3(total), dim3(256), 0, s, p.args);
-        else if (kind == GK_THIN8) QK_THIN8(8, false);
-        else if (kind == GK_THIN8_SWAP) QK_THIN8(8, true);
-        else if (kind == GK_THIN32) QK_THIN8(32, false);
-        else if (kind == GK_THIN32_SWAP) QK_THIN8(32, true);
+        const uint32_t most = (uint32_t)(kThreads / 256);
+        if (kind < GK_TILE)
+            for (; p.args.first < total; p.args.first += most) {
+                const dim3 some(std::min(most, total - p.args.first));
+                if (kind == GK_WAVE) hipLaunchKernelGGL(gram8_wave_kernel, some, dim3(256), 0, s, p.args);
+                else if (kind == GK_THIN8) QK_THIN8(8, false);
+                else if (kind == GK_THIN8_SWAP) QK_THIN8(8, true);
+                else if (kind == GK_THIN32) QK_THIN8(32, false);
+                else QK_THIN8(32, true);
+            }
         else if (kind == GK_TILE) QK_TILE8(false, float);
         else if (kind == GK_TILE_F64) QK_TILE8(false, double);
         else QK_TILE8(true, _Float16);
@@ -1777,7 +1792,7 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
     a.ldo = ldo;
     const bool tile = plan_decision8(x->rows, y->rows, D, C, a);
     const hipStream_t s = (hipStream_t)stream;
-    const dim3 joins((unsigned)((x->rows + 15) / 16), (unsigned)C);
+    const dim3 joins((unsigned)std::min<int64_t>((x->rows + 15) / 16, 1 << 20), (unsigned)C);
     if (y->rows == 0) {
         a.parts = 0;
         hipLaunchKernelGGL(decision8_join_kernel, joins, dim3(256), 0, s, a);

@@ -139,6 +139,30 @@ def test_write_appends_overwrites_and_takes_strides():
     assert len(store) == 4 and np.array_equal(store.codes.cpu().numpy()[:4], codes[::3])
 
 
+def test_more_rows_than_one_launch_takes():
+    """2^26 rows and some: more threads than a launch may have, and code offsets far beyond 32 bits."""
+    N = (1 << 26) + 70
+    angle = torch.arange(N, device="cuda", dtype=torch.float32) * 0.37
+    psi = torch.polar(0.5 + 0.5 * torch.sin(angle).abs(), angle).view(N, 1)
+    store = qdev.States8(N, 1)
+    store.write(psi)
+    some = torch.tensor([0, 1, (1 << 26) - 5, (1 << 26) - 4, (1 << 26) - 1, 1 << 26, N - 2, N - 1], device="cuda")
+    codes, scales, gains = S8.write(psi[some].cpu().numpy())
+    assert np.array_equal(store.codes[some].cpu().numpy(), codes) and np.array_equal(store.scales[some].cpu().numpy(), scales)
+    assert (np.abs(store.gains[some].cpu().numpy() - gains) <= 2 * S8.U32 * gains).all()
+    q = S8.rows(codes, scales, 1)
+    assert np.array_equal(store.read(some).cpu().numpy(), q.astype(np.complex64))
+    K = qdev.gram8(store.rows(N - 2, N), store)
+    check_k(K[:, some], q[-2:], gains[-2:], q, gains)
+    check_k(qdev.gram8(store.rows(N - 2, N)), q[-2:], gains[-2:], q[-2:], gains[-2:], symmetric=True)
+    few = qdev.gram8(store.rows(N - 260, N), store, dtype=torch.float16)      # 9 x 2^21 tiles of 32 x 32
+    check_k(few[-2:, some], q[-2:], gains[-2:], q, gains)
+    assert torch.equal(few[:, -260:], few[:, -260:].T)
+    del few
+    out = qdev.decision8(store.rows(N - 2, N), store.rows(N - 1, N), torch.full((1, 1), 2.0, device="cuda"))
+    check_k(out / 2, q[-2:], gains[-2:], q[-1:], gains[-1:])
+
+
 # ---- kernels -------------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (2, 3, 2), (31, 33, 16), (100, 64, 16), (1, 500, 64), (32, 129, 65), (257, 1, 100), (65, 70, 128), (130, 131, 256),
           (200, 257, 1000), (3, 129, 4096), (129, 260, 2048), (1, 40, 65536), (70, 30, 16384), (40, 300, 8192), (8, 70, 300), (9, 33, 1025), (300, 2, 640), (65, 32, 100), (500, 5, 2048)]
