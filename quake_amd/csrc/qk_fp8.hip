@@ -1208,12 +1208,12 @@ template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_t
 // share rows of A keeps its own sums of the C columns.
 // Up to eight columns: sums in LDS, the coefficients of a wave's 64 rows of B through its part of the free buffer, [column][64]; a
 // lane reads four at once, the same for its whole half, and its part of K stays in its registers.
-// MANY: out^T += coef^T K^T on FP32 matrix instructions, 32 columns at a time: a register of K is the right operand as it is.  The
+// MANY: out^T += coef^T K^T on FP32 matrix instructions, 32 or 16 columns at a time: a register of K is the right operand as it is.  The
 // coefficients of the tile come to the free buffer, [128][C], while the last chunk is multiplied; the sums wait in the workspace
 // (which stays in L2), where every lane adds to entries that no other lane touches.
 // 16384 x 16384 rows of 1024 amplitudes, one column: 1.46 ms, 1.51 PFLOP/s (library bf16 product 1.39 .. 1.62), bound by the matrix
-// unit with the widening between its instructions.  3001 x 10007 rows of 256, 45 columns: 115 us; a tile takes 10 us for K and 13
-// for its columns, 7 of them FP32 matrix instructions.
+// unit with the widening between its instructions.  3001 x 10007 rows of 256, 45 columns: 113 us; a tile takes 10 us for K and
+// 12 for its columns, 6 of them FP32 matrix instructions.
 constexpr int kLdsColumns = 8;
 constexpr int kDecisionLds = kPipeLds + 2 * kLdsColumns * kTile * 4;
 static_assert(2 * kDecisionLds <= 160 * 1024, "two workgroups per CU");
@@ -1277,7 +1277,8 @@ template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_ke
         auto finish = [&](int k, bool, const float* gains, uint8_t*, const uint8_t* side, v16f (&re)[2][2], v16f (&im)[2][2]) {
             kernel(k, gains, re, im);
             const int left = (int)min((int64_t)64, a.B.n - (int64_t)(t0 + k) * kTile - ys) - 4 * h;
-            for (int c0 = 0; c0 < a.C; c0 += 32) {
+            int c0 = 0;
+            for (; a.C - c0 > 16; c0 += 32) {
                 const int n = a.C - c0 - 4 * h;
                 float* const at = a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + 4 * h) * mp + row0 + xs + r;
                 float old[2][16];
@@ -1308,6 +1309,39 @@ template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_ke
                         const int c = 8 * (q >> 2) + (q & 3);
                         if (c < n) at[c * mp + j * 32] = old[j][q] + sum[j][q];
                     }
+            }
+            // 16 or fewer are left: four 16 x 16 products at once, two for the rows of either half of the wave, in half the time
+            // (3001 x 10007 rows of 256: 45 columns 119 -> 113 us, 16 columns 83 -> 80)
+            if (c0 < a.C) {
+                const int g = lane >> 4, x = lane & 15, n = a.C - c0 - 4 * g;
+                float* const at = a.ws + (((int64_t)blockIdx.y * 2 + (wave >> 1)) * a.C + c0 + 4 * g) * mp + row0 + xs + x;
+                float old[2][8];
+                v16f sum[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        if (q < 8) {
+                            old[j][q] = 0.f;
+                            if (k && (q & 3) < n) old[j][q] = at[(q & 3) * mp + j * 32 + 16 * (q >> 2)];
+                        }
+                        sum[j][q] = 0.f;
+                    }
+                const float* const coef = (const float*)side + min(c0 + x, a.C - 1) + (ys + 4 * h) * a.C;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const int row = i * 32 + 8 * (q >> 2) + (q & 3);
+                        const float v = coef[row * a.C], w = row < left ? v : 0.f;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x1f32(w, re[i][j][q], sum[j], 0, 0, 0);
+                    }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        if ((q & 3) < n) at[(q & 3) * mp + j * 32 + 16 * (q >> 2)] = old[j][q] + (sum[j][q] + sum[j][q + 8]);
             }
         };
         pipe.run<false, true>(work, finish, aside);
