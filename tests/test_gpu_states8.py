@@ -309,6 +309,15 @@ def test_decision8(M, N, D, C, path):
     assert (out[0] == -3).all() and (out[M + 1] == -3).all() and (out[:, :2] == -3).all() and (out[:, 2 + C:] == -3).all()
 
 
+@pytest.mark.parametrize("C", [1, 8, 9, 32, 33, 45, 50])
+def test_decision8_several_tiles_per_workgroup(C):
+    """Sums that are carried from tile to tile, the last of them ragged."""
+    rng = np.random.default_rng(C)
+    x, y = fill(S8.states(rng, 6500, 20, "product")), fill(S8.states(rng, 2570, 20, "spread"))
+    coef = rng.normal(size=(2570, C)).astype(np.float32)
+    check_decision(qdev.decision8(x[0], y[0], torch.from_numpy(coef).cuda()), x, y, coef, None)
+
+
 @pytest.mark.parametrize("M,N,D,C", [(70, 200, 64, 1), (70, 200, 64, 3), (70, 193, 64, 45), (3, 33, 1024, 2)])
 def test_decision8_infinite_coefficients(M, N, D, C, path):
     """An infinite coefficient of the last row, whose place behind the end of a tile must not meet a zero."""
