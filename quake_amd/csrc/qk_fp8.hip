@@ -1124,7 +1124,7 @@ struct Decision8Args {
 // coefficients is then a sum over the lane's own registers, and only the two halves of the wave have to be added.  32 rows of A
 // (8 with AR = 8) per workgroup against a range of B's.  SPLIT (rows of 8 chunks or more): the four waves share every tile of 32 of
 // B's rows, each multiplies a quarter of the chunks and then finishes a quarter of the tile's rows; else every wave has a tile of
-// its own.  One row against 8192 of 1024 amplitudes (17 MB, 3 us to read): 7.0 us, joining the parts 2.6, 16.5 from call to call.
+// its own (one row against 8192 of 512 amplitudes 8 us shared, 15 each on its own; of 256 the same).  One row against 8192 of 1024 amplitudes (17 MB, 3 us to read): 7.0 us, joining the parts 2.6, 16.5 from call to call.
 template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_thin_kernel(Decision8Args a) {
     constexpr int W = 4, R = SPLIT ? 16 / W : 16, S = 3;      // R: accumulator registers that a wave finishes
     extern __shared__ uint8_t lds[];
@@ -1206,7 +1206,7 @@ template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_t
 
 // The same over 128 x 128 tiles: a workgroup keeps 128 rows of A and walks B's tiles of its range.  Each of the two waves that
 // share rows of A keeps its own sums of the C columns.
-// Up to eight columns: sums in LDS, the coefficients of a wave's 64 rows of B through its part of the free buffer, [column][64]; a
+// Up to eight columns (8000 x 4000 rows of 256: five 67 us, eight 70; as MANY 79 and 76): sums in LDS, the coefficients of a wave's 64 rows of B through its part of the free buffer, [column][64]; a
 // lane reads four at once, the same for its whole half, and its part of K stays in its registers.
 // MANY: out^T += coef^T K^T on FP32 matrix instructions, 32 or 16 columns at a time: a register of K is the right operand as it is.  The
 // coefficients of the tile come to the free buffer, [128][C], while the last chunk is multiplied; the sums wait in the workspace
@@ -1431,11 +1431,16 @@ int check_dim(const char* who, int64_t D) {
 
 Rows8 rows8(const qk_states8& s) { return Rows8{(const uint8_t*)s.codes, (const uint8_t*)s.scales, s.gains, s.rows}; }
 
-// Which kernel takes a job.  The 128 x 128 kernel reads every row from L2 once for 128 others and needs enough tile steps to
-// fill the chip; the 32 x 32 kernel starts at once, takes few rows without waste and spreads a small job over more
-// workgroups.
+// Which kernel takes a job.  The 128 x 128 kernel reads every row from L2 once for 128 others and needs enough tiles, or tile
+// steps, to fill the chip; the 32 x 32 kernel starts at once, takes few rows without waste and spreads a small job over more
+// workgroups.  Measured, us with 32 x 32 / 128 x 128: float32, 61 tiles of 512 amplitudes 18.2 / 18.0, of 1024 25.9 / 27.7; 120 of 512
+// 25.1 / 18.8; 15 of 4096 (977 steps) 27.2 / 27.8, 34 of 4096 (2197) 56 / 35.  float16, whose tiles take half the time: 34 of 512
+// 11.2 / 12.2, 61 of 512 17.7 / 12.4, 15 of 4096 27.9 / 24.4, 34 of 1024 (549 steps) 17.4 / 18.0.
+// The kernels for few rows copy 8 or 32 of them beside every 32 of the others: 32 x 32 tiles / these, one row against 65536 of
+// 512 amplitudes 18.5 / 19.4, of 1024 28.2 / 28.2, of 4096 136 / 98; nine rows against 64 MB of 2048 18.5 / 20.0, of 4096 26.2 / 16.6, against
+// 16 MB 12.4 / 13.0.
 enum Gram8Kind { GK_WAVE, GK_THIN8, GK_THIN32, GK_THIN8_SWAP, GK_THIN32_SWAP, GK_TILE, GK_TILE_F64, GK_TILE_NATIVE, GK_KINDS };
-constexpr double g_tiles = 96, g_steps = 1024;
+constexpr double g_tiles = 96, g_steps = 1024, g_tiles16 = 48, g_steps16 = 900;
 std::atomic<int> g_path{0};      // development hook: 0 by rule, 1 always 32 x 32, 2 always 128 x 128, 3 the kernels for few rows where they can
 
 int64_t live_tiles(const qk_gram8_job& j, int64_t tile) {
@@ -1455,14 +1460,17 @@ double tiles_of(const qk_gram8_job& j) {
 // tiles, steps (tiles times chunks): of all jobs of the call
 Gram8Kind kind_of(const qk_gram8_job& j, double tiles, double steps) {
     const int path = g_path.load(std::memory_order_relaxed);
-    // up to 32 rows against more than 2 MiB of codes, in rows of 16 chunks or more: memory bound
+    // up to 8 rows against more than 2 MiB of codes in rows of 16 chunks or more, or 32 against 16 MiB in rows of 64: memory bound
     const int64_t few = std::min(j.A.rows, j.B.rows), many = std::max(j.A.rows, j.B.rows);
     if (!(j.flags & QK_GRAM_SYMMETRIC) && few <= 32 && code_bytes(j.D) <= (int64_t)1 << 26 &&
-        (path == 3 || (path == 0 && j.D > 960 && many * code_bytes(j.D) > (int64_t)1 << 21))) {
+        (path == 3 || (path == 0 && j.D > (few <= 8 ? 960 : 4032) && many * code_bytes(j.D) > (int64_t)1 << (few <= 8 ? 21 : 24)))) {
         const bool swap = j.B.rows < j.A.rows;
         return few <= 8 ? (swap ? GK_THIN8_SWAP : GK_THIN8) : (swap ? GK_THIN32_SWAP : GK_THIN32);
     }
-    if (path == 1 || path == 3 || tiles_of(j) == 0 || (path == 0 && tiles < g_tiles && steps < g_steps)) return GK_WAVE;
+    const bool half = j.flags & QK_GRAM8_F16;
+    if (path == 1 || path == 3 || tiles_of(j) == 0 ||
+        (path == 0 && tiles < (half ? g_tiles16 : g_tiles) && steps < (half ? g_steps16 : g_steps)))
+        return GK_WAVE;
     return j.flags & QK_GRAM8_F16 ? GK_TILE_NATIVE : j.flags & QK_GRAM8_F64 ? GK_TILE_F64 : GK_TILE;
 }
 
@@ -1477,25 +1485,33 @@ struct Gram8Plan {
 constexpr int64_t slots(Gram8Kind kind) { return kind == GK_WAVE ? 1024 : kind == GK_THIN32 || kind == GK_THIN32_SWAP ? 256 : 512; }
 
 // Which of a job's tiles are cut into slices of their rows, and into how many: those of the last round over the chip's slots,
-// where cutting brings more than it costs.  Measured: a step (a chunk of a tile) takes 3.0 us with all slots busy (fp8 1.7;
-// 32 x 32 tiles 0.4), joining a call's slices 5 us and what writing and reading them takes at 5 TB/s.  second: the call's last
-// tiles are in the second round.
+// where cutting brings more than it costs.  Measured for 128 x 128 tiles: a step (a chunk of a tile) takes 3.0 us with two workgroups on
+// every CU, 1.45 to 1.6 with one (8-bit instruction 1.7, 0.75 to 0.9); another round 4 us more; joining a launch, 0.085 us per
+// tile and 0.01 per slice (64 tiles in two slices 13 us, in eight 14, 121 in two 16).  32 x 32 tiles: 0.4 us a step, 5 us and
+// the slices' way out and back at 5 TB/s.  behind: steps of the jobs behind this one that fill up the round.  second: the call's
+// last tiles are in the second round.
 void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double behind, bool second, Gram8JobDev& d) {
     const int64_t all = slots(kind), side = kind < GK_TILE ? 32 : kTile, last = (taken + live) % all, tail = std::min(live, last);
-    const double step = kind < GK_TILE ? 0.4 : kind == GK_TILE_NATIVE ? 1.7 : 3.0;
+    const double pair = kind == GK_TILE_NATIVE ? 1.7 : 3.0, one = kind == GK_TILE_NATIVE ? 0.85 : 1.55;
+    auto cost = [&](int n, int per) {
+        const int64_t items = tail * n, rounds = (items + all - 1) / all;
+        if (kind < GK_TILE) return (double)(rounds * per) * 0.4 + (n > 1 ? 5.0 + (double)(items * side * side * 16) / 5e6 : 0.0);
+        const double step = behind == 0 && 2 * items <= all ? one : pair * (rounds > 1 ? 1.0 : 0.67 + 0.33 * (double)items / (double)all);
+        return (double)rounds * (per * step + 4.0) + (n > 1 ? 6.0 + 0.085 * (double)tail + 0.01 * (double)items : 0.0);
+    };
     d.whole = (uint32_t)live;
     d.slices = 1;
     d.small = 0;
     d.per = chunks;
     if (tail == 0 || behind >= 0.5 * (double)((all - last) * chunks)) return;      // the jobs behind it fill the round
-    double best = (double)chunks * step;
+    double best = cost(1, chunks);
     const int most = std::min(kind < GK_TILE ? chunks / 16 : chunks / 4, 256);
     for (int n = 2; n <= most; ++n) {
         const int per = (chunks + n - 1) / n;
         if ((chunks + per - 1) / per != n) continue;
-        const double cost = (double)((tail * n + all - 1) / all) * per * step + 5.0 + (double)(tail * n * side * side * 16) / 5e6;
-        if (cost < best) {
-            best = cost;
+        const double here = cost(n, per);
+        if (here < best) {
+            best = here;
             d.slices = n;
             d.per = per;
             d.whole = (uint32_t)(live - tail);
@@ -1600,6 +1616,8 @@ int check_gram8(const qk_gram8_job* jobs, int n) {
 }
 
 // -> whether the 128 x 128 kernel takes it (gram8's rule)
+// (us in 32-row tiles / in 128 x 128 ones, whose rows are not cut: 24 of them of 4096 amplitudes 31 / 94, 61 of 1024 24.0 / 28.3, of 4096
+// 53 / 95, 95 of 1024 38 / 29, of 4096 90 / 93, 120 of 1024 39 / 29; of 256 and less the same)
 bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
     a.C = C;
     a.chunks = (int32_t)((D + kChunk - 1) / kChunk);
@@ -1607,7 +1625,7 @@ bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
     const int path = g_path.load(std::memory_order_relaxed);
     const double area = (double)std::max<int64_t>(M, 64) * (double)std::max<int64_t>(N, 64) / (kTile * kTile);
     const bool tile = code_bytes(D) <= (int64_t)1 << 24 &&
-                      (path == 2 || (path == 0 && M > 32 && (area >= g_tiles || area * a.chunks >= g_steps)));
+                      (path == 2 || (path == 0 && M > 32 && area >= g_tiles));
     const int64_t side = tile ? kTile : M <= 8 ? 8 : 32, tm = (M + side - 1) / side, tn = (N + (tile ? kTile : 32) - 1) / (tile ? kTile : 32);
     const int64_t want = tile ? std::max<int64_t>(1, std::min<int64_t>(tn, 512 / std::max<int64_t>(tm, 1)))
                               : std::max<int64_t>(1, std::min<int64_t>(a.chunks >= 8 ? tn : (tn + 3) / 4, 1024 / std::max<int64_t>(tm, 1)));
@@ -1645,8 +1663,9 @@ extern "C" int qk_states8_write_dev(const void* psi, int f32, int64_t ldpsi, int
     uint8_t *codes = (uint8_t*)to->codes, *scales = (uint8_t*)to->scales;
     float* gains = (float*)to->gains;
     const hipStream_t s = (hipStream_t)stream;
-    // a wave takes two blocks at a time: one wave per row up to 8 blocks, sixteen for the longest rows
-    const int wpr = blocks <= 8 ? 1 : blocks <= 64 ? 4 : 16;
+    // A wave takes two blocks at a time: one wave per row up to 8 blocks, four up to 32, else sixteen.  (complex64, 512 MB: 1024
+    // amplitudes 94 us with one wave, 106 with four; 2048 102 and 89; 8192 96 with four, 90 with sixteen; 16384 99 and 92.)
+    const int wpr = blocks <= 8 ? 1 : blocks <= 32 ? 4 : 16;
     const int rows = wpr == 1 ? 4 : 1, threads = wpr == 16 ? 1024 : 256;      // of a workgroup
     const int64_t most = kThreads / threads * rows, cb = code_bytes(D), sb = scale_bytes(D);
 #define QK_WRITE8(T, W)                                                                                                       \
