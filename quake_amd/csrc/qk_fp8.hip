@@ -1615,7 +1615,7 @@ int check_gram8(const qk_gram8_job* jobs, int n) {
     return QK_OK;
 }
 
-// -> whether the 128 x 128 kernel takes it (gram8's rule)
+// -> whether the 128 x 128 kernel takes it
 // (us in 32-row tiles / in 128 x 128 ones, whose rows are not cut: 24 of them of 4096 amplitudes 31 / 94, 61 of 1024 24.0 / 28.3, of 4096
 // 53 / 95, 95 of 1024 38 / 29, of 4096 90 / 93, 120 of 1024 39 / 29; of 256 and less the same)
 bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
