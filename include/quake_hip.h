@@ -229,10 +229,12 @@ int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* bytes);
 int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream);
 
 /*
- * Decision values of a kernel machine, K never written: out[m][c] = sum_j K(x_m, y_j) coef[j][c] + intercept[c]
+ * Decision values of a kernel machine, K never written (but for up to 32 x against up to 4096 y of more than 4096 amplitudes,
+ * where a small K goes through the workspace): out[m][c] = sum_j K(x_m, y_j) coef[j][c] + intercept[c]
  * (SVC.decision_function on a precomputed kernel: coef = dual_coef_.T over the support vectors in y).  coef: y->rows x C
  * float32, row stride ldc; intercept: C float32 or NULL; out: x->rows x C float32, row stride ldo.  The gradient of a loss by
- * coef is the same call with the stores exchanged: dcoef = decision(y, x, dout).  An empty y gives the intercept.
+ * coef is the same call with the stores exchanged: dcoef = decision(y, x, dout).  An empty y gives the intercept.  ws: as for
+ * qk_gram8_jobs_dev, of qk_decision8_workspace bytes.
  */
 #define QK_DECISION8_MAX_C 64
 int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, size_t* bytes);

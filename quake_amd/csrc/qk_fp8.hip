@@ -5,7 +5,7 @@
 //                                                    max |component of the block| * 2^-e <= 448
 //   read      codes, scales -> code * 2^e
 //   gram8     K_ij = gain_i gain_j |sum_b conj(q_i[b]) q_j[b]|^2,  gain = ||psi||^2 / ||q||^2
-//   decision8 out[m][c] = sum_j K_mj coef[j][c] + intercept[c], K never written
+//   decision8 out[m][c] = sum_j K_mj coef[j][c] + intercept[c], K not written (but for a few long rows)
 //
 // A row of D amplitudes is laid out as chunks of 64 amplitudes: 64 real codes, then 64 imaginary codes (128 bytes, one
 // cache line); the last chunk is padded with zero codes.  Two chunks share one scale byte e + 127.  Scales are powers of
@@ -1412,6 +1412,22 @@ __global__ __launch_bounds__(256) void decision8_join_kernel(Decision8Args a) {
     }
 }
 
+// out = K coef + intercept for a K that is there: one workgroup per entry.
+__global__ __launch_bounds__(256) void decision8_rows_kernel(Decision8Args a) {
+    __shared__ double sum[4];
+    const int64_t row = blockIdx.x;
+    const int c = blockIdx.y;
+    const float* const K = a.ws + row * a.B.n;
+    double s = 0.0;
+#pragma unroll 4
+    for (int64_t j = threadIdx.x; j < a.B.n; j += 256) s += (double)K[j] * (double)a.coef[j * a.ldc + c];
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+    if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) a.out[row * a.ldo + c] = (float)(sum[0] + sum[1] + sum[2] + sum[3] + (a.intercept ? (double)a.intercept[c] : 0.0));
+}
+
 // ---- host side -------------------------------------------------------------------------------------------------------------
 namespace {
 constexpr int64_t kMaxD = (int64_t)1 << 26;
@@ -1635,6 +1651,24 @@ bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
     a.parts = tile && C > kLdsColumns ? 2 * a.splits : a.splits > 1 ? a.splits : 0;
     return tile;
 }
+
+// A few rows against few long ones: the 32-row tiles would be less than one for every other CU, each with a long way to go, so K
+// goes through memory, its rows cut by gram8's rule.  (Tiles / this, us: one row against 1000 of 9000 amplitudes 25 / 14, of 65536 132 / 32;
+// 32 rows against 1000 of 65536 154 / 36; one against 4000 of 9000 25.4 / 25.5, 8000 of 9000 29 / 37.)
+bool decision8_by_rows(int64_t M, int64_t N, int64_t D) {
+    return g_path.load(std::memory_order_relaxed) == 0 && M <= 32 && D > 64 * kChunk && N <= 4096;
+}
+qk_gram8_job decision8_job(const qk_states8& x, const qk_states8& y, int64_t D, void* K) {
+    qk_gram8_job j;
+    std::memset(&j, 0, sizeof(j));
+    j.A = x;
+    j.B = y;
+    j.D = D;
+    j.K = K;
+    j.ldk = y.rows;
+    return j;
+}
+size_t decision8_k_bytes(int64_t M, int64_t N) { return (size_t)((M * N * (int64_t)sizeof(float) + 255) & ~(int64_t)255); }
 }  // namespace
 }  // namespace qk
 
@@ -1816,6 +1850,16 @@ extern "C" int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, si
     if (M == 0 || N == 0) return QK_OK;
     Decision8Args a;
     std::memset(&a, 0, sizeof(a));
+    if (decision8_by_rows(M, N, D)) {
+        const qk_gram8_job job = decision8_job({nullptr, nullptr, nullptr, M}, {nullptr, nullptr, nullptr, N}, D, nullptr);
+        size_t gram = 0;
+        rc = gram8_launches(&job, 1, [&](const Gram8Plan& p, Gram8Kind) {
+            gram = std::max(gram, p.ws_floats * sizeof(float));
+            return (int)QK_OK;
+        });
+        *bytes = decision8_k_bytes(M, N) + gram;
+        return rc;
+    }
     plan_decision8(M, N, D, C, a);
     *bytes = (size_t)a.parts * C * a.stride * sizeof(float);
     return QK_OK;
@@ -1833,6 +1877,7 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
     if (!out || (y->rows && !coef)) return fail(QK_ERR_INVALID, std::string(who) + ": null pointer");
     if (ldc < C || ldo < C) return fail(QK_ERR_INVALID, std::string(who) + ": row stride smaller than C");
     if (need > ws_bytes || (need && !ws)) return fail(QK_ERR_INVALID, std::string(who) + ": workspace smaller than qk_decision8_workspace asks for");
+    if ((uintptr_t)ws & 15) return fail(QK_ERR_INVALID, std::string(who) + ": the workspace needs 16-byte alignment");
     Decision8Args a;
     std::memset(&a, 0, sizeof(a));
     a.A = rows8(*x);
@@ -1849,6 +1894,14 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
     if (y->rows == 0) {
         a.parts = 0;
         hipLaunchKernelGGL(decision8_join_kernel, joins, dim3(256), 0, s, a);
+        QK_HIP(hipGetLastError());
+        return QK_OK;
+    }
+    if (decision8_by_rows(x->rows, y->rows, D)) {
+        const size_t k = decision8_k_bytes(x->rows, y->rows);
+        const qk_gram8_job job = decision8_job(*x, *y, D, ws);
+        if ((rc = qk_gram8_jobs_dev(&job, 1, (char*)ws + k, ws_bytes - k, stream))) return rc;
+        hipLaunchKernelGGL(decision8_rows_kernel, dim3((unsigned)x->rows, (unsigned)C), dim3(256), 0, s, a);
         QK_HIP(hipGetLastError());
         return QK_OK;
     }

@@ -421,7 +421,7 @@ def gram8(x: States8, y: Optional[States8] = None, out: Optional[torch.Tensor] =
 def decision8(x: States8, y: States8, coef: torch.Tensor, intercept: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """What a kernel machine answers, out[m, c] = sum_j K(x_m, y_j) coef[j, c] + intercept[c], float32 [len(x), C], without K
-    in memory: ``SVC.decision_function`` on a precomputed kernel (``coef = dual_coef_.T``, y the support vectors), kernel
+    in memory (a small K for up to 32 rows of x against up to 4096 of y with more than 4096 amplitudes): ``SVC.decision_function`` on a precomputed kernel (``coef = dual_coef_.T``, y the support vectors), kernel
     ridge predictions, or K times a vector inside an iterative solver.  coef: float32 [len(y), C] (or [len(y)] for C = 1) with
     unit column stride, C up to 64.  The gradient of a loss by coef is ``decision8(y, x, dloss/dout)``, the one by the
     intercept the sum over dloss/dout's rows."""

@@ -309,6 +309,21 @@ def test_decision8(M, N, D, C, path):
     assert (out[0] == -3).all() and (out[M + 1] == -3).all() and (out[:, :2] == -3).all() and (out[:, 2 + C:] == -3).all()
 
 
+@pytest.mark.parametrize("M,N,D,C", [(32, 4096, 4160, 3), (33, 100, 8192, 2), (7, 4097, 4200, 1), (31, 5, 20000, 64), (1, 1, 65536, 1)])
+def test_decision8_few_long_rows(M, N, D, C):
+    """Both sides of the sizes that go through K in memory; twice on one workspace, with an infinite coefficient in one column."""
+    rng = np.random.default_rng(D)
+    x, y = fill(S8.states(rng, M, D, "spread")), fill(S8.states(rng, N, D, "spread"))
+    coef, b = rng.normal(size=(N, C)).astype(np.float32), rng.normal(size=C).astype(np.float32)
+    cd, bd = torch.from_numpy(coef).cuda(), torch.from_numpy(b).cuda()
+    out = qdev.decision8(x[0], y[0], cd, bd)
+    check_decision(out, x, y, coef, b)
+    assert torch.equal(qdev.decision8(x[0], y[0], cd, bd), out)
+    cd[-1, 0] = float("inf")
+    last = qdev.decision8(x[0], y[0], cd, bd)
+    assert torch.isposinf(last[:, 0]).all() and torch.equal(last[:, 1:], out[:, 1:])
+
+
 @pytest.mark.parametrize("C", [1, 8, 9, 32, 33, 45, 50])
 def test_decision8_several_tiles_per_workgroup(C):
     """Sums that are carried from tile to tile, the last of them ragged."""
