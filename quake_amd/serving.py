@@ -3,7 +3,7 @@
 The reference answers a new sample by evaluating its kernel row against the whole training set and handing that to
 sklearn (``qsvm/train.py:152-160``), which simulates every training sample again.  Here the support vectors' states are
 simulated and stored once (:class:`quake_amd.device.States8`), and a sample costs its own simulation and one pass over
-the store (:func:`quake_amd.device.decision8`); the kernel matrix is not handed out.
+the store (:func:`quake_amd.device.decision8`); no kernel matrix reaches the host.
 """
 from __future__ import annotations
 
