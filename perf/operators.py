@@ -190,7 +190,7 @@ def _quantise(psi):
     parts = torch.nn.functional.pad(parts, (0, 0, 0, blocks * BLOCK - dim)).view(rows, blocks, BLOCK, 2)
     most = parts.abs().amax(dim=(2, 3))
     m, x = torch.frexp(most)
-    e = torch.where(most > 0, torch.clamp(x - torch.where(m <= 0.875, 9, 8), min=-100), 0)
+    e = torch.where(most > 0, torch.clamp(x - torch.where(m <= 0.875, 9, 8), -127, 127), 0)
     q = _e4m3(torch.ldexp(parts, -e[:, :, None, None]))
     value = torch.ldexp(q, e[:, :, None, None])
     norm = parts.double().square().sum(dim=(1, 2, 3))
@@ -281,7 +281,7 @@ def _exact_write(psi):
                 e = torch.ceil(torch.log2(top / 448.0))          # the least e with top <= 448 * 2^e
                 e = torch.where(top > torch.exp2(e) * 448.0, e + 1, e)
                 e = torch.where(top <= torch.exp2(e - 1) * 448.0, e - 1, e)
-                e = torch.where(top > 0, torch.clamp(e, min=-100), torch.zeros_like(e))
+                e = torch.where(top > 0, torch.clamp(e, -127, 127), torch.zeros_like(e))
                 scales[:, b] = (e + 127).to(torch.uint8)
                 unit = torch.exp2(e)[:, None]
             w = v / unit
