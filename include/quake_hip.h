@@ -211,8 +211,8 @@ int qk_states8_read_dev(const qk_states8* from, int64_t D, const int64_t* index,
  * Jobs are those of qk_gram_jobs_dev (KT not with QK_GRAM_SYMMETRIC), each with its own D: the kernels of a population of circuits of any sizes run together.
  * K (and KT) are float32, or float16 / float64 by flag.  QK_GRAM_SYMMETRIC: the same store on both sides, only tiles on or
  * above the diagonal are computed, the mirror is written and the diagonal is exactly 1.
- * Sums are FP32.  ws: device memory of qk_gram8_workspace bytes (0 for most calls), 16-byte aligned, used until the call's
- * work is done.  Results do not depend on the launch: no atomics, fixed order of summation.
+ * Sums are FP32 for every type of K, which is converted once.  ws: device memory of qk_gram8_workspace bytes (0 for most
+ * calls), 16-byte aligned, used until the call's work is done.  Results do not depend on the launch: no atomics, fixed order of summation.
  */
 #define QK_GRAM8_F16 2
 #define QK_GRAM8_F64 4

@@ -12,12 +12,12 @@
 // two because that is exact: multiplying by one never rounds, and an e4m3 code has the same relative step whatever the
 // scale (the scale only keeps the block inside the format's 2^18 range).
 //
-// Arithmetic of the products, two forms.  float32 and float64 K, decision values and everything that runs in 32 x 32 tiles: codes
-// are widened to bf16 (exact: e4m3 has 4 significant bits, bf16 has 8 and FP32's exponents) with the block's scale applied in the
-// same instruction; a product of two codes is exact in FP32, sums are FP32.  128 x 128 tiles of float16 K: the 8-bit matrix
-// instruction with the scales as operands.  It aligns groups of 8 products to the largest and cuts what falls below about 13 bits of
-// it, so K of similar states comes out up to 1e-4 low -- a fifth of float16's own rounding (2^-11), but too much for float32.  Rates
-// measured: 8-bit instruction 4.2 .. 4.8 PFLOP/s from registers, bf16 2.49, bf16 with two widening instructions each 1.82.
+// Arithmetic of the products, one form for every type of K and every kernel: codes are widened to bf16 (exact: e4m3 has 4
+// significant bits, bf16 has 8 and FP32's exponents) with the block's scale applied in the same instruction; a product of two codes
+// is exact in FP32, sums are FP32, K is converted to its type once.  The 8-bit matrix instruction is not used: it aligns groups of 8
+// products to the largest and cuts what falls below about 13 bits of it, which leaves K of similar states 1e-4 low and small entries
+// (sums that cancel) off by a per cent.  Rates measured from registers: 8-bit instruction 4.2 .. 4.8 PFLOP/s, bf16 2.49, bf16
+// with two widening instructions each 1.82.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -344,12 +344,20 @@ __device__ __forceinline__ void store_k(void* K, int64_t at, float k, int flags)
     else ((float*)K)[at] = k;
 }
 
+// K of an overlap and the two gains' product, in FP32 whatever K's type: which square is fused is written out, and the product is
+// rounded here (the compiler would fuse it with a float16 K's conversion, in some kernels and not in others).
+__device__ __forceinline__ float k_value(float re, float im, float gains) {
+    float k = __builtin_fmaf(re, re, im * im) * gains;
+    asm("" : "+v"(k));
+    return k;
+}
+
 // One entry of K and its mirror (symmetric: the entries below the diagonal are the ones above it, so K is symmetric to the
 // bit; summed on their own they would differ in the order of the imaginary part's two halves).
 __device__ __forceinline__ void emit(const Gram8JobDev& J, int64_t row, int64_t col, float re, float im) {
     const bool sym = J.flags & QK_GRAM_SYMMETRIC;
     if (row >= J.A.n || col >= J.B.n || (sym && row > col)) return;
-    float k = (re * re + im * im) * (J.A.gains[row] * J.B.gains[col]);
+    float k = k_value(re, im, J.A.gains[row] * J.B.gains[col]);
     if (sym && row == col) k = 1.f;
     store_k(J.K, row * J.ldk + col, k, J.flags);
     if (sym && row != col) store_k(J.K, col * J.ldk + row, k, J.flags);
@@ -649,7 +657,6 @@ constexpr int kStage = 2 * kTile * kChunkBytes;
 constexpr int kScales = 2 * kStage;                         // a dword of scales (8 chunks) per row, twice
 constexpr int kGains = kScales + 2 * 2 * kTile * 4;         // the rows' gains, twice
 constexpr int kPipeLds = kGains + 2 * 2 * kTile * 4;
-typedef int v8i __attribute__((ext_vector_type(8)));
 
 struct TileWork {              // what one pass of the pipeline computes; the same for the whole workgroup
     Rows8 A, B;
@@ -657,7 +664,7 @@ struct TileWork {              // what one pass of the pipeline computes; the sa
     int chunks, sb, c0, c1;
 };
 
-template <bool NATIVE> struct TilePipe {
+struct TilePipe {
     uint8_t* lds;
     int wave, lane, r, h;
     const uint8_t* src;        // copies: waves 0 and 1 bring A, 2 and 3 bring B, eight pieces of 8 rows each
@@ -717,7 +724,7 @@ template <bool NATIVE> struct TilePipe {
     }
 
     // One step.  STAGE: the copies of the next chunk are issued in its middle, behind the first matrix instructions (12000 rows
-    // of 16384 amplitudes, half K: 4.13 ms with the copies first, 4.03 in the middle).
+    // of 16384 amplitudes, float32 6.6 ms; with the copies first the same within 1 %).
     template <bool STAGE> __device__ __forceinline__ void compute(int c, v16f (&re)[2][2], v16f (&im)[2][2]) {
         const uint8_t* base = lds + buf * kStage;
         const int shift = (c >> 1 & 3) * 8;
@@ -728,92 +735,53 @@ template <bool NATIVE> struct TilePipe {
             sa[t] = *(const uint32_t*)(scale + (wave >> 1) * 256);
             sc[t] = *(const uint32_t*)(scale + 512 + (wave & 1) * 256);
         }
-        if constexpr (NATIVE) {
-            union F { v4u q[2]; v8i v; };
-            F ar[2], ai[2], br[2], bi[2];
+        const float ea[2] = {scale_value((sa[0] >> shift) & 255u), scale_value((sa[1] >> shift) & 255u)};
+        const float eb[2] = {scale_value((sc[0] >> shift) & 255u), scale_value((sc[1] >> shift) & 255u)};
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+        for (int s = 0; s < 2; ++s) {
+            if (STAGE && s == 1) stage(c + 1, buf ^ 1);
+            v4u ar[2], ai[2], br[2], bi[2];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    ar[t].q[s] = *(const v4u*)(base + fa + t * 4096 + piece[s]);
-                    ai[t].q[s] = *(const v4u*)(base + fa + t * 4096 + piece[2 + s]);
-                    br[t].q[s] = *(const v4u*)(base + fb + t * 4096 + piece[s]);
-                    bi[t].q[s] = *(const v4u*)(base + fb + t * 4096 + piece[2 + s]);
-                }
-            const int ea[2] = {(int)(sa[0] >> shift), (int)(sa[1] >> shift)}, eb[2] = {(int)(sc[0] >> shift), (int)(sc[1] >> shift)};
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    re[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ar[i].v, br[j].v, re[i][j], 0, 0, 0, ea[i], 0, eb[j]);
-                    im[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ar[i].v, bi[j].v, im[i][j], 0, 0, 0, ea[i], 0, eb[j]);
-                }
-            if constexpr (STAGE) {
-                __builtin_amdgcn_sched_barrier(0);
-                stage(c + 1, buf ^ 1);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int t = 0; t < 2; ++t) {
+                ar[t] = *(const v4u*)(base + fa + t * 4096 + piece[s]);
+                ai[t] = *(const v4u*)(base + fa + t * 4096 + piece[2 + s]);
+                br[t] = *(const v4u*)(base + fb + t * 4096 + piece[s]);
+                bi[t] = *(const v4u*)(base + fb + t * 4096 + piece[2 + s]);
             }
-            F na[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) na[i].q[s] = ai[i].q[s] ^ 0x80808080u;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    re[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(ai[i].v, bi[j].v, re[i][j], 0, 0, 0, ea[i], 0, eb[j]);
-                    im[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(na[i].v, br[j].v, im[i][j], 0, 0, 0, ea[i], 0, eb[j]);
-                }
-        } else {
-            const float ea[2] = {scale_value((sa[0] >> shift) & 255u), scale_value((sa[1] >> shift) & 255u)};
-            const float eb[2] = {scale_value((sc[0] >> shift) & 255u), scale_value((sc[1] >> shift) & 255u)};
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (STAGE && s == 1) stage(c + 1, buf ^ 1);
-                v4u ar[2], ai[2], br[2], bi[2];
+            for (int q = 0; q < 4; q += 2) {
+                v8b xr[2], xi[2], xn[2], yr[2], yi[2];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    ar[t] = *(const v4u*)(base + fa + t * 4096 + piece[s]);
-                    ai[t] = *(const v4u*)(base + fa + t * 4096 + piece[2 + s]);
-                    br[t] = *(const v4u*)(base + fb + t * 4096 + piece[s]);
-                    bi[t] = *(const v4u*)(base + fb + t * 4096 + piece[2 + s]);
+                    xr[t] = widen8(ar[t][q], ar[t][q + 1], ea[t]);
+                    xi[t] = widen8(ai[t][q], ai[t][q + 1], ea[t]);
+                    yr[t] = widen8(br[t][q], br[t][q + 1], eb[t]);
+                    yi[t] = widen8(bi[t][q], bi[t][q + 1], eb[t]);
+                    xn[t] = negated(xi[t]);
                 }
 #pragma unroll
-                for (int q = 0; q < 4; q += 2) {
-                    v8b xr[2], xi[2], xn[2], yr[2], yi[2];
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        xr[t] = widen8(ar[t][q], ar[t][q + 1], ea[t]);
-                        xi[t] = widen8(ai[t][q], ai[t][q + 1], ea[t]);
-                        yr[t] = widen8(br[t][q], br[t][q + 1], eb[t]);
-                        yi[t] = widen8(bi[t][q], bi[t][q + 1], eb[t]);
-                        xn[t] = negated(xi[t]);
+                    for (int j = 0; j < 2; ++j) {
+                        re[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr[i], yr[j], re[i][j], 0, 0, 0);
+                        im[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr[i], yi[j], im[i][j], 0, 0, 0);
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            re[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr[i], yr[j], re[i][j], 0, 0, 0);
-                            im[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xr[i], yi[j], im[i][j], 0, 0, 0);
-                        }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            re[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xi[i], yi[j], re[i][j], 0, 0, 0);
-                            im[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xn[i], yr[j], im[i][j], 0, 0, 0);
-                        }
-                }
+                    for (int j = 0; j < 2; ++j) {
+                        re[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xi[i], yi[j], re[i][j], 0, 0, 0);
+                        im[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xn[i], yr[j], im[i][j], 0, 0, 0);
+                    }
             }
         }
     }
 
     // Of two workgroups on a CU the matrix unit serves the older one first; left alone, one is through its tile in half the
     // other's time, and the workgroups that share rows in L2 drift apart.  Every 4 steps a wave goes down one level of four and
-    // then back to the highest, so the one behind has the higher level most of the time (12000 rows of 65536 amplitudes, half K:
-    // 16.4 -> 14.8 ms; 8192 of 4096: 470 -> 423 us, float32 820 -> 783; turns of 1, 2, 8 or 16 steps within 2 % of that.  The level
-    // changes before the barrier of a step: behind it 15.3 ms).
+    // then back to the highest, so the one behind has the higher level most of the time (12000 rows of 16384 amplitudes, float32:
+    // 7.27 -> 6.60 ms; 8192 of 4096: 828 -> 797 us; half K 7.25 -> 6.55 ms and 817 -> 790 us).  The level changes before the barrier of a
+    // step.
     __device__ __forceinline__ void turn(int c) {
         const int t = (c >> 2) & 3;
         if (t == 0) __builtin_amdgcn_s_setprio(3);
@@ -909,14 +877,14 @@ __device__ __forceinline__ void put16(uint4 v, __amdgpu_buffer_rsrc_t to, int of
 template <typename I> __device__ __forceinline__ I uniform(I v) { return (I)__builtin_amdgcn_readfirstlane((int)v); }
 
 // T: the type of K.  128 x 128 entries per workgroup, 64 x 64 per wave: 128 accumulator registers, two workgroups on a CU, so that one
-// multiplies while the other finishes its tile.  Bound by the matrix unit at the clock that the chip holds under it (about
-// 1.6 GHz): 12000 rows of 65536 amplitudes, half K 14.8 ms, 2.55 PFLOP/s (a library product of 8-bit matrices of
-// 16384^3 reaches 2.97); 12000 of 16384, float32 6.6 ms, 1.42 (library bf16 product 1.62).  Short rows by what K takes to
-// write: 4096 of 256 amplitudes, half K 21.5 us of which 6 are for the matrix unit and 8 for 34 MB of stores.
-template <bool NATIVE, typename T>
+// multiplies while the other finishes its tile.  Bound by the matrix unit, with the widening between its instructions, at the
+// clock that the chip holds under it: 12000 rows of 65536 amplitudes, half K 27.0 ms, 1.40 PFLOP/s; of 16384, half 6.55 ms, float32
+// 6.62, float64 6.70, 1.42 (library bf16 product 1.62).  Short rows by what K takes to write: 4096 of 256 amplitudes, half K 24.5 us,
+// float32 26.6, float64 42.
+template <typename T>
 __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
     extern __shared__ uint8_t lds[];
-    TilePipe<NATIVE> pipe(lds);
+    TilePipe pipe(lds);
     const int wave = pipe.wave, lane = pipe.lane, r = pipe.r, h = pipe.h;
     struct Where { int job; uint32_t t, ti, tj; int slice; } now{}, before{};      // of the tile that was opened last and the one before
     int round = 0;
@@ -986,8 +954,7 @@ __global__ __launch_bounds__(256, 2) void gram8_tile_kernel(Gram8Args args) {
                     const float g[4] = {ga.x, ga.y, ga.z, ga.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = re[i][j][q + e], y = im[i][j][q + e];
-                        re[i][j][q + e] = (x * x + y * y) * (g[e] * gb);
+                        re[i][j][q + e] = k_value(re[i][j][q + e], im[i][j][q + e], g[e] * gb);
                         const int n = 2 * q + e;
                         put<T>((T)re[i][j][q + e], K, n < limit ? off : -1, (i * 32 + n) * step);
                     }
@@ -1221,7 +1188,7 @@ static_assert(QK_DECISION8_MAX_C * kTile * 4 <= kStage, "a tile's coefficients f
 
 template <bool MANY> __global__ __launch_bounds__(256, 2) void decision8_tile_kernel(Decision8Args a) {
     extern __shared__ uint8_t lds[];
-    TilePipe<false> pipe(lds);
+    TilePipe pipe(lds);
     const int tid = threadIdx.x, wave = pipe.wave, lane = pipe.lane, r = pipe.r, h = pipe.h;
     const int xs = (wave & 1) * 64, ys = (wave >> 1) * 64;
     const int64_t row0 = (int64_t)blockIdx.x * kTile, mp = (int64_t)gridDim.x * kTile;
@@ -1450,13 +1417,13 @@ Rows8 rows8(const qk_states8& s) { return Rows8{(const uint8_t*)s.codes, (const 
 // Which kernel takes a job.  The 128 x 128 kernel reads every row from L2 once for 128 others and needs enough tiles, or tile
 // steps, to fill the chip; the 32 x 32 kernel starts at once, takes few rows without waste and spreads a small job over more
 // workgroups.  Measured, us with 32 x 32 / 128 x 128: float32, 61 tiles of 512 amplitudes 18.2 / 18.0, of 1024 25.9 / 27.7; 120 of 512
-// 25.1 / 18.8; 15 of 4096 (977 steps) 27.2 / 27.8, 34 of 4096 (2197) 56 / 35.  float16, whose tiles take half the time: 34 of 512
-// 11.2 / 12.2, 61 of 512 17.7 / 12.4, 15 of 4096 27.9 / 24.4, 34 of 1024 (549 steps) 17.4 / 18.0.
+// 25.1 / 18.8; 15 of 4096 (977 steps) 27.2 / 27.8, 34 of 4096 (2197) 56 / 35.  float16: 63 of 512 13.7 / 17.7, 90 of 512 18.5 / 17.8, 120 of 512
+// 23.0 / 17.9, 15 of 4096 26.3 / 25.1, 35 of 4096 57 / 34.
 // The kernels for few rows copy 8 or 32 of them beside every 32 of the others: 32 x 32 tiles / these, one row against 65536 of
 // 512 amplitudes 18.5 / 19.4, of 1024 28.2 / 28.2, of 4096 136 / 98; nine rows against 64 MB of 2048 18.5 / 20.0, of 4096 26.2 / 16.6, against
 // 16 MB 12.4 / 13.0.
-enum Gram8Kind { GK_WAVE, GK_THIN8, GK_THIN32, GK_THIN8_SWAP, GK_THIN32_SWAP, GK_TILE, GK_TILE_F64, GK_TILE_NATIVE, GK_KINDS };
-constexpr double g_tiles = 96, g_steps = 1024, g_tiles16 = 48, g_steps16 = 900;
+enum Gram8Kind { GK_WAVE, GK_THIN8, GK_THIN32, GK_THIN8_SWAP, GK_THIN32_SWAP, GK_TILE, GK_TILE_F64, GK_TILE_F16, GK_KINDS };
+constexpr double g_tiles = 96, g_steps = 1024;
 std::atomic<int> g_path{0};      // development hook: 0 by rule, 1 always 32 x 32, 2 always 128 x 128, 3 the kernels for few rows where they can
 
 int64_t live_tiles(const qk_gram8_job& j, int64_t tile) {
@@ -1483,11 +1450,8 @@ Gram8Kind kind_of(const qk_gram8_job& j, double tiles, double steps) {
         const bool swap = j.B.rows < j.A.rows;
         return few <= 8 ? (swap ? GK_THIN8_SWAP : GK_THIN8) : (swap ? GK_THIN32_SWAP : GK_THIN32);
     }
-    const bool half = j.flags & QK_GRAM8_F16;
-    if (path == 1 || path == 3 || tiles_of(j) == 0 ||
-        (path == 0 && tiles < (half ? g_tiles16 : g_tiles) && steps < (half ? g_steps16 : g_steps)))
-        return GK_WAVE;
-    return j.flags & QK_GRAM8_F16 ? GK_TILE_NATIVE : j.flags & QK_GRAM8_F64 ? GK_TILE_F64 : GK_TILE;
+    if (path == 1 || path == 3 || tiles_of(j) == 0 || (path == 0 && tiles < g_tiles && steps < g_steps)) return GK_WAVE;
+    return j.flags & QK_GRAM8_F16 ? GK_TILE_F16 : j.flags & QK_GRAM8_F64 ? GK_TILE_F64 : GK_TILE;
 }
 
 // One launch's worth of jobs of one kind: tiles, slices, workspace.
@@ -1502,13 +1466,13 @@ constexpr int64_t slots(Gram8Kind kind) { return kind == GK_WAVE ? 1024 : kind =
 
 // Which of a job's tiles are cut into slices of their rows, and into how many: those of the last round over the chip's slots,
 // where cutting brings more than it costs.  Measured for 128 x 128 tiles: a step (a chunk of a tile) takes 3.0 us with two workgroups on
-// every CU, 1.45 to 1.6 with one (8-bit instruction 1.7, 0.75 to 0.9); another round 4 us more; joining a launch, 0.085 us per
+// every CU, 1.45 to 1.6 with one; another round 4 us more; joining a launch, 0.085 us per
 // tile and 0.01 per slice (64 tiles in two slices 13 us, in eight 14, 121 in two 16).  32 x 32 tiles: 0.4 us a step, 5 us and
 // the slices' way out and back at 5 TB/s.  behind: steps of the jobs behind this one that fill up the round.  second: the call's
 // last tiles are in the second round.
 void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double behind, bool second, Gram8JobDev& d) {
     const int64_t all = slots(kind), side = kind < GK_TILE ? 32 : kTile, last = (taken + live) % all, tail = std::min(live, last);
-    const double pair = kind == GK_TILE_NATIVE ? 1.7 : 3.0, one = kind == GK_TILE_NATIVE ? 0.85 : 1.55;
+    const double pair = 3.0, one = 1.55;
     auto cost = [&](int n, int per) {
         const int64_t items = tail * n, rounds = (items + all - 1) / all;
         if (kind < GK_TILE) return (double)(rounds * per) * 0.4 + (n > 1 ? 5.0 + (double)(items * side * side * 16) / 5e6 : 0.0);
@@ -1534,8 +1498,8 @@ void cut(Gram8Kind kind, int64_t live, int chunks, int64_t taken, double behind,
         }
     }
     // Few tiles of short rows behind one full round: as 32 x 32 tiles they take one step of every workgroup.  (4096 rows of 256
-    // amplitudes, 528 tiles: half K 24.5 -> 21.8 us, float32 37.5 -> 30.0; 46 tiles over 20.0 against 19.6 us, 128 tiles 19.7 against
-    // 29.5; behind four rounds, where the workgroups are out of step, 53.7 against 54.5.)
+    // amplitudes, 528 tiles: half K 34.4 -> 24.2 us, float32 35.7 -> 26.7, float64 59 -> 42; 49 tiles over, half: rows of 64 21.2 -> 21.6,
+    // of 256 34.6 -> 32.1; 83 tiles over 22.2 -> 25.6 and 35.3 -> 37.1.)
     if (second && kind >= GK_TILE && d.slices == 1 && chunks <= 8 && last <= live && 16 * tail <= all) {
         d.small = 1;
         d.slices = 16;
@@ -1773,10 +1737,10 @@ template <typename K, typename A> int launch8(K kernel, dim3 grid, int lds, hipS
     QK_HIP(hipGetLastError());
     return QK_OK;
 }
-#define QK_TILE8(NATIVE, T)                                                                                          \
+#define QK_TILE8(T)                                                                                                  \
     do {                                                                                                             \
         static DeviceOnce once;                                                                                      \
-        const int rc8 = launch8(gram8_tile_kernel<NATIVE, T>, dealt, kPipeLds, s, p.args, once, kPipeLds);           \
+        const int rc8 = launch8(gram8_tile_kernel<T>, dealt, kPipeLds, s, p.args, once, kPipeLds);                   \
         if (rc8) return rc8;                                                                                         \
     } while (0)
 #define QK_THIN8(AR, SWAP)                                                                                           \
@@ -1801,8 +1765,8 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
     return gram8_launches(jobs, n_jobs, [&](Gram8Plan& p, Gram8Kind kind) {
         p.args.ws = (float*)ws;
         const uint32_t total = p.args.total, full = total >> 6;
-        // two workgroups per CU that stay (one for each item: 5000 x 7001 rows of 64 amplitudes, half K 33 against 29.4 us; rows of 1024
-        // and more within 2 %); where the last round is of small tiles, one for each item: those start wherever one ends (4096 rows
+        // two workgroups per CU that stay (one for each item: 5000 x 7001 rows of 64 amplitudes, half K 39 against 36 us, float32 43 against 40;
+        // rows of 256 and more within 2 %); where the last round is of small tiles, one for each item: those start wherever one ends (4096 rows
         // of 256 amplitudes, float32 30.6 -> 28.0 us)
         const dim3 dealt(std::min<uint32_t>(p.args.small < total ? 0x7fffffffu : 512u, (full << 6) + 8 * ((total - (full << 6) + 7) >> 3)));
         const uint32_t most = (uint32_t)(kThreads / 256);
@@ -1815,9 +1779,9 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
                 else if (kind == GK_THIN32) QK_THIN8(32, false);
                 else QK_THIN8(32, true);
             }
-        else if (kind == GK_TILE) QK_TILE8(false, float);
-        else if (kind == GK_TILE_F64) QK_TILE8(false, double);
-        else QK_TILE8(true, _Float16);
+        else if (kind == GK_TILE) QK_TILE8(float);
+        else if (kind == GK_TILE_F64) QK_TILE8(double);
+        else QK_TILE8(_Float16);
         QK_HIP(hipGetLastError());
         if (p.join_tiles) {
             if (kind < GK_TILE) hipLaunchKernelGGL(gram8_join_kernel<1>, dim3(p.join_tiles * 4), dim3(256), 0, s, p.args);

@@ -353,7 +353,7 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
     own rows and its own dim: the kernels of a population.  Each job: dict(A=, B=None, K=None, KT=None) with A, B
     :class:`States8`; B is None: the symmetric kernel of A with an exact unit diagonal.  K (allocated as ``dtype`` if not
     given, several of them in one allocation) and KT, the transposed copy (not for symmetric jobs): float32, float16 or
-    float64 [len(A), len(B)] views with unit column stride.  Returns the Ks."""
+    float64 [len(A), len(B)] views with unit column stride, converted once from FP32 sums.  Returns the Ks."""
     if not jobs:
         return []
     if dtype not in _K8_FLAGS:

@@ -1,0 +1,55 @@
+"""Values of the 8-bit stores' operators held to the arithmetic that the header states, against tests/_states8.py."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from quake_amd import _lib, device as qdev
+from tests import _states8 as S8
+from tests.test_gpu_states8 import fill, path, put  # noqa: F401  (path is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def half_step(v):
+    """Half the distance of float16 numbers at v >= 0."""
+    return np.exp2(np.maximum(np.frexp(np.maximum(v, 1e-30))[1] - 1, -14) - 11.0)
+
+
+def close_states(rng, N, D):
+    """States near one another: every K is near 1, where a sum that is cut shows most."""
+    one = S8.states(rng, 1, D, "product")
+    psi = one + 0.1 * S8.states(rng, N, D)
+    return psi / np.linalg.norm(psi, axis=1, keepdims=True)
+
+
+# ---- float16 K: FP32 sums, rounded once ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("M,N,D,kind", [(130, 131, 256, "close"), (700, 500, 128, "close"), (300, 300, 16, "product"), (1100, 1000, 512, "close"),
+                                        (257, 129, 300, "spread"), (64, 300, 64, "product"), (5, 400, 200, "close"), (1500, 1200, 65, "spread")])
+def test_half_kernel_is_rounded_once(M, N, D, kind, path):
+    """Off by FP32's bound and half a step of float16, whatever kernel takes the product."""
+    rng = np.random.default_rng(M + N + D)
+    make = close_states if kind == "close" else lambda r, n, d: S8.states(r, n, d, kind)
+    states = make(rng, M + N, D)
+    x, a, ga = fill(states[:M])
+    y, b, gb = fill(states[M:])
+    ref, t32, _ = S8.kernel(a, ga, b, gb)
+    off = np.abs(qdev.gram8(x, y, dtype=torch.float16).cpu().numpy().astype(np.float64) - ref) - (t32 + half_step(ref + t32))
+    assert (off <= 0).all(), (off.max(), (off > 0).sum())
+    ref, t32, _ = S8.kernel(a, ga, a, ga)
+    np.fill_diagonal(ref, 1.0)
+    off = np.abs(qdev.gram8(x, dtype=torch.float16).cpu().numpy().astype(np.float64) - ref) - (t32 + half_step(ref + t32))
+    assert (off <= 0).all(), (off.max(), (off > 0).sum())
+
+
+@pytest.mark.parametrize("M,N,D", [(130, 131, 256), (700, 900, 4096), (33, 2000, 2048), (1, 5000, 1024), (20, 300, 16384), (200, 0, 16384), (700, 0, 512),
+                                   (1200, 0, 8192), (4090, 0, 256), (3000, 2000, 64)])
+def test_half_and_double_kernel_are_the_single_one_converted(M, N, D, path):
+    """One arithmetic for all types of K: FP32 sums, converted once."""
+    rng = np.random.default_rng(M + N + D)
+    x = fill(S8.states(rng, M, D, "product"))[0]
+    y = fill(S8.states(rng, N, D, "product"))[0] if N else None
+    K = qdev.gram8(x, y)
+    assert torch.equal(qdev.gram8(x, y, dtype=torch.float16), K.half())
+    assert torch.equal(qdev.gram8(x, y, dtype=torch.float64), K.double())
