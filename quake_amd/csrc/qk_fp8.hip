@@ -1099,7 +1099,8 @@ template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_t
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     ThinPipe<AR, S> pipe(lds + wave * S * ThinPipe<AR, S>::kBytes);
     const int lane = pipe.lane, r = pipe.r, h = pipe.h;
-    for (int k = tid; k < W * 32 * a.C; k += 256) acc[k] = 0.f;
+    // a wave clears its own sums: no other wave touches them before the barrier behind the tiles
+    for (int k = lane; k < 32 * a.C; k += 64) acc[wave * 32 * a.C + k] = 0.f;
     const int64_t row0 = (int64_t)blockIdx.x * AR;
     const int64_t cb = (int64_t)a.chunks * kChunkBytes;
     const float ga = a.A.gains[min(row0 + r, a.A.n - 1)];

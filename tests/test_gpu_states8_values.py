@@ -7,7 +7,7 @@ import torch
 
 from quake_amd import _lib, device as qdev
 from tests import _states8 as S8
-from tests.test_gpu_states8 import fill, path, put  # noqa: F401  (path is a fixture)
+from tests.test_gpu_states8 import check_decision, fill, path, put  # noqa: F401  (path is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,17 @@ def test_half_and_double_kernel_are_the_single_one_converted(M, N, D, path):
     K = qdev.gram8(x, y)
     assert torch.equal(qdev.gram8(x, y, dtype=torch.float16), K.half())
     assert torch.equal(qdev.gram8(x, y, dtype=torch.float64), K.double())
+
+
+# ---- decision values --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("M,N,D,C", [(1, 33, 16, 64), (8, 200, 448, 64), (20, 40, 64, 64), (32, 129, 100, 1), (3, 4, 2, 63)])
+def test_short_rows_many_columns_every_run(M, N, D, C):
+    """Rows of fewer than 8 chunks against few others: every wave's sums start from its own zeros, run after run."""
+    rng = np.random.default_rng(M + N + D + C)
+    x, y = fill(S8.states(rng, M, D, "spread")), fill(S8.states(rng, N, D, "spread"))
+    coef = rng.normal(size=(N, C)).astype(np.float32)
+    cd = torch.from_numpy(coef).cuda()
+    first = qdev.decision8(x[0], y[0], cd)
+    check_decision(first, x, y, coef, None)
+    for _ in range(50):
+        assert torch.equal(qdev.decision8(x[0], y[0], cd), first)
