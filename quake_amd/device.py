@@ -252,7 +252,13 @@ class States8:
         self._gpu = gpu = codes.get_device()
         if gpu < 0 or scales.get_device() != gpu or gains.get_device() != gpu:
             raise ValueError("device entry points need tensors in GPU memory, all on one GPU")
-        self._at = codes.data_ptr(), scales.data_ptr(), gains.data_ptr()
+
+    @property
+    def _at(self):      # at every call: a copy of a store (copy.deepcopy, pickle) has arrays of its own
+        return self.codes.data_ptr(), self.scales.data_ptr(), self.gains.data_ptr()
+
+    def __setstate__(self, state) -> None:
+        self._set(state["codes"], state["scales"], state["gains"], state["dim"], state["_rows"])
 
     @classmethod
     def from_arrays(cls, codes: torch.Tensor, scales: torch.Tensor, gains: torch.Tensor, dim: int) -> "States8":

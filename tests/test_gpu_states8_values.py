@@ -67,3 +67,20 @@ def test_short_rows_many_columns_every_run(M, N, D, C):
     check_decision(first, x, y, coef, None)
     for _ in range(50):
         assert torch.equal(qdev.decision8(x[0], y[0], cd), first)
+
+
+# ---- copies of a store ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("again", ["deepcopy", "pickle"])
+def test_a_copy_has_memory_of_its_own(again):
+    import copy
+    import pickle
+    psi = S8.states(np.random.default_rng(3), 9, 200)
+    x, a, ga = fill(psi)
+    before = x.codes.clone()
+    t = copy.deepcopy(x) if again == "deepcopy" else pickle.loads(pickle.dumps(x))
+    t.write(put(psi[::-1]), at=0)
+    assert torch.equal(x.codes, before) and torch.equal(t.codes, before.flip(0))
+    del x
+    K, t32, _ = S8.kernel(a[::-1], ga[::-1], a[::-1], ga[::-1])
+    np.fill_diagonal(K, 1.0)
+    assert (np.abs(qdev.gram8(t).cpu().numpy() - K) <= t32 + S8.U32 * K).all()

@@ -1,0 +1,84 @@
+"""8-bit stores and served models as Python objects, on a machine without a GPU: what reaches the library, and what is refused
+before it.  Tensors in host memory pass for GPU tensors here, and a recorder stands in for the library."""
+import contextlib
+import copy
+import ctypes as C
+import io
+import pickle
+
+import numpy as np
+import pytest
+import torch
+
+from quake_amd import _lib, device as qdev
+
+
+class Recorder:
+    """Takes the entry points' calls, runs nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Host tensors pass for tensors on GPU 0."""
+    lib = Recorder()
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    monkeypatch.setattr(qdev, "_on", lambda gpu: contextlib.nullcontext())
+    monkeypatch.setattr(qdev, "_stream_on", lambda gpu: 0)
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    return lib
+
+
+def store(rows=5, dim=100):
+    code, scale = 128 * -(-dim // 64), 4 * -(-dim // 512)
+    return qdev.States8.from_arrays(torch.zeros((rows, code), dtype=torch.uint8), torch.full((rows, scale), 127, dtype=torch.uint8),
+                                    torch.ones(rows), dim)
+
+
+def addresses(s):
+    return s.codes.data_ptr(), s.scales.data_ptr(), s.gains.data_ptr()
+
+
+def saved(s):
+    f = io.BytesIO()
+    torch.save(s, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)          # (a file that this test wrote itself)
+
+
+@pytest.mark.parametrize("again", [copy.copy, copy.deepcopy, lambda s: pickle.loads(pickle.dumps(s)), saved],
+                         ids=["copy", "deepcopy", "pickle", "torch.save"])
+def test_copies_bring_their_own_addresses(host, again):
+    first = store()
+    t = again(first)
+    assert len(t) == 5 and t.dim == 100 and t.capacity == 5 and torch.equal(t.codes, first.codes)
+    if again is not copy.copy:
+        assert not set(addresses(t)) & set(addresses(first))
+    s = t._struct(2, 1)
+    assert (s.codes, s.scales, s.gains) == (t.codes[2].data_ptr(), t.scales[2].data_ptr(), t.gains[2:].data_ptr()) and s.rows == 1
+    qdev.gram8(t, out=torch.zeros((5, 5)))
+    name, args = host.calls[-1]
+    assert name == "qk_gram8_jobs_dev" and _lib.GRAM8_JOB.unpack(args[0])[:3] == addresses(t)
+
+
+def test_arrays_that_moved_are_found(host):
+    s = store()
+    s.gains = s.gains.clone()
+    s.codes.data = s.codes.data.clone()
+    at = s._struct()
+    assert (at.codes, at.scales, at.gains) == addresses(s)
+
+
+def test_a_copy_in_host_memory_is_refused(host, monkeypatch):
+    raw = pickle.dumps(store())
+    monkeypatch.undo()                                # host tensors are host tensors again
+    with pytest.raises(ValueError, match="GPU memory"):
+        pickle.loads(raw)
