@@ -220,6 +220,13 @@ def _same_gpu(gpu: int, *tensors) -> None:
             raise ValueError("device entry points need tensors in GPU memory, all on one GPU")
 
 
+def _in_memory(*tensors) -> None:
+    """The library reads and writes memory: a lazily negated or conjugated view holds other values there than it shows."""
+    for t in tensors:
+        if t is not None and (t.is_neg() or t.is_conj()):
+            raise ValueError("lazily negated or conjugated tensors are not taken: call resolve_neg() / resolve_conj() first")
+
+
 class States8:
     """Statevectors kept in 8 bits: e4m3 codes, one power-of-two scale for each block of 128 amplitudes, and one float per row
     that restores the row's norm -- 2 bytes per amplitude instead of complex128's 16.  The training states of a kernel model:
@@ -271,6 +278,7 @@ class States8:
                 or not (codes.is_contiguous() and scales.is_contiguous() and gains.is_contiguous()):
             raise ValueError("need contiguous codes uint8 [rows, 128 ceil(dim / 64)], scales uint8 [rows, 4 ceil(dim / 512)], "
                              "gains float32 [rows]")
+        _in_memory(codes, scales, gains)
         store = cls.__new__(cls)
         store._set(codes, scales, gains, dim, rows)
         return store
@@ -310,8 +318,9 @@ class States8:
         psi = from_dlpack(psi)
         _same_gpu(self._gpu, psi)
         if psi.dtype not in (torch.complex128, torch.complex64) or psi.dim() != 2 or psi.shape[1] != self.dim \
-                or (psi.shape[0] and self.dim > 1 and psi.stride(1) != 1) or psi.is_conj():
+                or (psi.shape[0] and self.dim > 1 and psi.stride(1) != 1):
             raise ValueError("psi must be a complex128 / complex64 [rows, dim] tensor with unit column stride")
+        _in_memory(psi)
         n, at = psi.shape[0], self._rows if at is None else at
         if not 0 <= at <= self._rows:
             raise ValueError(f"at = {at}: the store holds {self._rows} rows")
@@ -331,6 +340,7 @@ class States8:
         ``index`` (int64 on the GPU, any order, repeats allowed; a number outside the store gives a row of NaN)."""
         index, out = from_dlpack(index), from_dlpack(out)
         _same_gpu(self._gpu, index, out)
+        _in_memory(index, out)
         if index is not None and (index.dtype != torch.int64 or index.dim() != 1 or not index.is_contiguous()):
             raise ValueError("index must be a contiguous int64 vector")
         n = self._rows if index is None else index.shape[0]
@@ -397,6 +407,7 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
             if K.dtype not in _K8_FLAGS or K.shape != (m, n) or (K.numel() and ((n > 1 and K.stride(1) != 1) or (m > 1 and K.stride(0) < n))):
                 raise ValueError("K must be float32, float16 or float64 [len(A), len(B)] with unit column stride")
             _same_gpu(gpu, K)
+            _in_memory(K)
             ldk = K.stride(0) if m > 1 and n else max(n, 1)
         kt = ldkt = 0
         if KT is not None:
@@ -405,6 +416,7 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
                     or (KT.numel() and ((m > 1 and KT.stride(1) != 1) or (n > 1 and KT.stride(0) < m))):
                 raise ValueError("KT must be of K's type, [len(B), len(A)] with unit column stride, and not for a symmetric job")
             _same_gpu(gpu, KT)
+            _in_memory(KT)
             kt, ldkt = KT.data_ptr(), (KT.stride(0) if n > 1 and m else max(m, 1))
         packed.append(_lib.GRAM8_JOB.pack(*A._at, m, *B._at, n, A.dim, K.data_ptr(), kt, ldk, ldkt,
                                           _K8_FLAGS[K.dtype] | (_lib.QK_GRAM_SYMMETRIC if sym else 0), 0))
@@ -435,6 +447,7 @@ def decision8(x: States8, y: States8, coef: torch.Tensor, intercept: Optional[to
     if not isinstance(x, States8) or not isinstance(y, States8):
         raise ValueError("x and y must be States8 stores")
     _same_gpu(x._gpu, y.codes, coef, intercept, out)
+    _in_memory(coef, intercept, out)
     if x.dim != y.dim:
         raise ValueError(f"stores of different dim: {x.dim} and {y.dim}")
     if coef.dim() == 1:

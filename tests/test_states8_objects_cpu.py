@@ -82,3 +82,28 @@ def test_a_copy_in_host_memory_is_refused(host, monkeypatch):
     monkeypatch.undo()                                # host tensors are host tensors again
     with pytest.raises(ValueError, match="GPU memory"):
         pickle.loads(raw)
+
+
+def test_views_whose_values_are_not_in_memory_are_refused(host):
+    """A lazily negated or conjugated tensor: its memory holds other values than it shows."""
+    x, y = store(4), store(5)
+    full = lambda *s, **k: torch.zeros(s, **k)
+    z = torch.zeros((5, 1), dtype=torch.complex64).conj()
+    assert z.imag.is_neg()
+    neg = torch._neg_view
+    psi, out = full(2, 100, dtype=torch.complex64), full(5, 100, dtype=torch.complex64)
+    coef, b = full(5, 1), full(1)
+    index = torch.zeros(5, dtype=torch.int64)
+    calls = [lambda: qdev.decision8(x, y, z.imag), lambda: qdev.decision8(x, y, z.imag[:, 0]), lambda: qdev.decision8(x, y, neg(coef)),
+             lambda: qdev.decision8(x, y, coef, neg(b)), lambda: qdev.decision8(x, y, coef, b, out=neg(full(4, 1))),
+             lambda: x.write(psi.conj(), at=0), lambda: x.write(neg(psi), at=0), lambda: y.read(out=out.conj()), lambda: y.read(out=neg(out)),
+             lambda: y.read(neg(index)), lambda: qdev.gram8(x, y, out=neg(full(4, 5))),
+             lambda: qdev.gram8_jobs([dict(A=x, B=y, KT=neg(full(5, 4)))]),
+             lambda: qdev.States8.from_arrays(y.codes, y.scales, neg(y.gains), 100)]
+    for k, call in enumerate(calls):
+        with pytest.raises(ValueError, match="conjugated"):
+            call()
+            pytest.fail(f"case {k} was taken")
+    assert not host.calls
+    qdev.decision8(x, y, z.imag.resolve_neg(), b, out=full(4, 1)), x.write(psi.conj().resolve_conj(), at=0), y.read(index, out=out)
+    assert [name for name, _ in host.calls if name.endswith("dev")] == ["qk_decision8_dev", "qk_states8_write_dev", "qk_states8_read_dev"]
