@@ -227,6 +227,15 @@ def _in_memory(*tensors) -> None:
             raise ValueError("lazily negated or conjugated tensors are not taken: call resolve_neg() / resolve_conj() first")
 
 
+def _no_graph(*tensors) -> None:
+    """Nothing here is recorded for autograd: an output without a graph would drop a gradient without a word."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("no gradient is recorded through 8-bit stores: detach() the tensor or call under torch.no_grad() "
+                                 "(the gradient of decision8 by coef is decision8(y, x, dloss/dout))")
+
+
 class States8:
     """Statevectors kept in 8 bits: e4m3 codes, one power-of-two scale for each block of 128 amplitudes, and one float per row
     that restores the row's norm -- 2 bytes per amplitude instead of complex128's 16.  The training states of a kernel model:
@@ -279,6 +288,7 @@ class States8:
             raise ValueError("need contiguous codes uint8 [rows, 128 ceil(dim / 64)], scales uint8 [rows, 4 ceil(dim / 512)], "
                              "gains float32 [rows]")
         _in_memory(codes, scales, gains)
+        _no_graph(gains)
         store = cls.__new__(cls)
         store._set(codes, scales, gains, dim, rows)
         return store
@@ -321,6 +331,7 @@ class States8:
                 or (psi.shape[0] and self.dim > 1 and psi.stride(1) != 1):
             raise ValueError("psi must be a complex128 / complex64 [rows, dim] tensor with unit column stride")
         _in_memory(psi)
+        _no_graph(psi)
         n, at = psi.shape[0], self._rows if at is None else at
         if not 0 <= at <= self._rows:
             raise ValueError(f"at = {at}: the store holds {self._rows} rows")
@@ -341,6 +352,7 @@ class States8:
         index, out = from_dlpack(index), from_dlpack(out)
         _same_gpu(self._gpu, index, out)
         _in_memory(index, out)
+        _no_graph(index, out)
         if index is not None and (index.dtype != torch.int64 or index.dim() != 1 or not index.is_contiguous()):
             raise ValueError("index must be a contiguous int64 vector")
         n = self._rows if index is None else index.shape[0]
@@ -408,6 +420,7 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
                 raise ValueError("K must be float32, float16 or float64 [len(A), len(B)] with unit column stride")
             _same_gpu(gpu, K)
             _in_memory(K)
+            _no_graph(K)
             ldk = K.stride(0) if m > 1 and n else max(n, 1)
         kt = ldkt = 0
         if KT is not None:
@@ -417,6 +430,7 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
                 raise ValueError("KT must be of K's type, [len(B), len(A)] with unit column stride, and not for a symmetric job")
             _same_gpu(gpu, KT)
             _in_memory(KT)
+            _no_graph(KT)
             kt, ldkt = KT.data_ptr(), (KT.stride(0) if n > 1 and m else max(m, 1))
         packed.append(_lib.GRAM8_JOB.pack(*A._at, m, *B._at, n, A.dim, K.data_ptr(), kt, ldk, ldkt,
                                           _K8_FLAGS[K.dtype] | (_lib.QK_GRAM_SYMMETRIC if sym else 0), 0))
@@ -441,13 +455,14 @@ def decision8(x: States8, y: States8, coef: torch.Tensor, intercept: Optional[to
     """What a kernel machine answers, out[m, c] = sum_j K(x_m, y_j) coef[j, c] + intercept[c], float32 [len(x), C], without K
     in memory (a small K for up to 32 rows of x against up to 4096 of y with more than 4096 amplitudes): ``SVC.decision_function`` on a precomputed kernel (``coef = dual_coef_.T``, y the support vectors), kernel
     ridge predictions, or K times a vector inside an iterative solver.  coef: float32 [len(y), C] (or [len(y)] for C = 1) with
-    unit column stride, C up to 64.  The gradient of a loss by coef is ``decision8(y, x, dloss/dout)``, the one by the
-    intercept the sum over dloss/dout's rows."""
+    unit column stride, C up to 64.  Nothing is recorded for autograd (a tensor that requires a gradient is refused): the gradient of
+    a loss by coef is ``decision8(y, x, dloss/dout)``, the one by the intercept the sum over dloss/dout's rows."""
     coef, intercept, out = from_dlpack(coef), from_dlpack(intercept), from_dlpack(out)
     if not isinstance(x, States8) or not isinstance(y, States8):
         raise ValueError("x and y must be States8 stores")
     _same_gpu(x._gpu, y.codes, coef, intercept, out)
     _in_memory(coef, intercept, out)
+    _no_graph(coef, intercept, out)
     if x.dim != y.dim:
         raise ValueError(f"stores of different dim: {x.dim} and {y.dim}")
     if coef.dim() == 1:

@@ -107,3 +107,24 @@ def test_views_whose_values_are_not_in_memory_are_refused(host):
     assert not host.calls
     qdev.decision8(x, y, z.imag.resolve_neg(), b, out=full(4, 1)), x.write(psi.conj().resolve_conj(), at=0), y.read(index, out=out)
     assert [name for name, _ in host.calls if name.endswith("dev")] == ["qk_decision8_dev", "qk_states8_write_dev", "qk_states8_read_dev"]
+
+
+def test_tensors_that_want_a_gradient_are_refused(host):
+    """No graph is recorded: an output without one would drop the gradient without a word."""
+    x, y = store(4), store(5)
+    leaf = lambda *s, **k: torch.zeros(s, requires_grad=True, **k)
+    coef, b = torch.zeros(5, 2), torch.zeros(2)
+    calls = [lambda: qdev.decision8(x, y, leaf(5, 2)), lambda: qdev.decision8(x, y, leaf(5)), lambda: qdev.decision8(x, y, 2 * leaf(5, 2)),
+             lambda: qdev.decision8(x, y, coef, leaf(2)), lambda: qdev.decision8(x, y, coef, b, out=leaf(4, 2)),
+             lambda: x.write(leaf(2, 100, dtype=torch.complex64), at=0), lambda: y.read(out=leaf(5, 100, dtype=torch.complex64)),
+             lambda: qdev.gram8(x, y, out=leaf(4, 5)), lambda: qdev.gram8_jobs([dict(A=x, B=y, KT=leaf(5, 4))])]
+    for k, call in enumerate(calls):
+        with pytest.raises(ValueError, match="detach"):
+            call()
+            pytest.fail(f"case {k} was taken")
+    assert not host.calls
+    out = torch.zeros(4, 2)
+    with torch.no_grad():
+        qdev.decision8(x, y, leaf(5, 2), leaf(2), out=out)
+    qdev.decision8(x, y, leaf(5, 2).detach(), out=out)
+    assert [name for name, _ in host.calls].count("qk_decision8_dev") == 2
