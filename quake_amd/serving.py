@@ -38,7 +38,7 @@ class ServedSVC:
 
     kernel:   the :class:`quake_amd.kernels.HipFidelityKernel` (its feature map and bound training parameters are used; the
               answers come from 8-bit states whatever its precision).
-    svc:      the fitted model; up to 11 classes.
+    svc:      the fitted model; up to 11 classes, not with ``break_ties``.
     x_train:  the rows it was fitted on, in their order."""
 
     def __init__(self, kernel: HipFidelityKernel, svc, x_train, device=None):
@@ -47,6 +47,8 @@ class ServedSVC:
         x, _ = kernel._validate(x_train, None)
         if x.shape[0] != svc.shape_fit_[0]:
             raise ValueError(f"the model was fitted on {svc.shape_fit_[0]} rows, x_train has {x.shape[0]}")
+        if getattr(svc, "break_ties", False) and getattr(svc, "decision_function_shape", "ovr") == "ovr" and len(svc.classes_) > 2:
+            raise ValueError("svc.break_ties is not supported: classes are decided by the votes of their pairs")
         coef, intercept = pair_coefficients(svc)
         if coef.shape[1] > _lib.QK_DECISION8_MAX_C:
             raise ValueError(f"{len(svc.classes_)} classes need {coef.shape[1]} columns, at most {_lib.QK_DECISION8_MAX_C} are possible")

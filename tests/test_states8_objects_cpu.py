@@ -128,3 +128,26 @@ def test_tensors_that_want_a_gradient_are_refused(host):
         qdev.decision8(x, y, leaf(5, 2), leaf(2), out=out)
     qdev.decision8(x, y, leaf(5, 2).detach(), out=out)
     assert [name for name, _ in host.calls].count("qk_decision8_dev") == 2
+
+
+# ---- served models ---------------------------------------------------------------------------------------------------------
+def served(classes, decisions):
+    """A model that answers these decision values."""
+    from quake_amd.serving import ServedSVC
+    m = ServedSVC.__new__(ServedSVC)
+    m.classes = np.asarray(classes)
+    m.decision_function = lambda x: np.asarray(decisions, dtype=np.float32)
+    return m
+
+
+def test_served_svc_refuses_to_break_ties():
+    """break_ties takes the argmax of the ovr values: other answers than the votes of the pairs."""
+    from sklearn.svm import SVC
+    from quake_amd import circuit as qc, featuremaps as fm
+    from quake_amd.kernels import HipFidelityKernel
+    from quake_amd.serving import ServedSVC
+    k = HipFidelityKernel(fm.zz_featuremap(qc.ParameterVector("x", 3), 3, 1))
+    X = np.random.default_rng(0).uniform(size=(21, 3))
+    three = SVC(kernel="precomputed", break_ties=True, decision_function_shape="ovr").fit(np.eye(21), np.arange(21) % 3)
+    with pytest.raises(ValueError, match="break_ties"):
+        ServedSVC(k, three, X)
