@@ -87,10 +87,11 @@ class ServedSVC:
         return out[:, 0] if len(self.classes) == 2 else out
 
     def predict(self, x_vec) -> np.ndarray:
-        """Class labels: the sign for two classes, else most pairs won (a tie goes to the class that comes first)."""
+        """Class labels: the sign for two classes (zero goes to ``classes[1]``), else most pairs won (a tie goes to the class that
+        comes first)."""
         d = self.decision_function(x_vec)
         if len(self.classes) == 2:
-            return self.classes[(d > 0).astype(int)]
+            return self.classes[(d >= 0).astype(int)]
         votes = np.zeros((d.shape[0], len(self.classes)), dtype=int)
         rows, p = np.arange(d.shape[0]), 0
         for i in range(len(self.classes)):

@@ -151,3 +151,17 @@ def test_served_svc_refuses_to_break_ties():
     three = SVC(kernel="precomputed", break_ties=True, decision_function_shape="ovr").fit(np.eye(21), np.arange(21) % 3)
     with pytest.raises(ValueError, match="break_ties"):
         ServedSVC(k, three, X)
+
+
+def test_a_decision_of_exactly_zero_goes_where_sklearn_sends_it():
+    from sklearn.svm import SVC
+    svc = SVC(kernel="precomputed").fit(np.eye(4), [3, 5, 3, 5])
+    rows = np.array([[0, 0, 0, 0], [1, 0, 0, 0], [0, 1, 0, 0]], dtype=float)        # nothing in common with any support vector; one; the other
+    d = svc.decision_function(rows)
+    assert d[0] == 0 and d[1] < 0 < d[2]
+    assert np.array_equal(served([3, 5], d).predict(rows), svc.predict(rows))
+    three = SVC(kernel="precomputed", decision_function_shape="ovo").fit(np.eye(6), [0, 1, 2, 0, 1, 2])
+    rows = np.zeros((1, 6))
+    d = three.decision_function(rows)
+    assert (d == 0).all()
+    assert np.array_equal(served([0, 1, 2], d).predict(rows), three.predict(rows))
