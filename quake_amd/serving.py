@@ -88,8 +88,10 @@ class ServedSVC:
 
     def predict(self, x_vec) -> np.ndarray:
         """Class labels: the sign for two classes (zero goes to ``classes[1]``), else most pairs won (a tie goes to the class that
-        comes first)."""
+        comes first).  A sample whose decision values are NaN (one whose features are not finite) is refused."""
         d = self.decision_function(x_vec)
+        if np.isnan(d).any():
+            raise ValueError(f"{int(np.isnan(d.reshape(len(d), -1)).any(axis=1).sum())} of {len(d)} samples have NaN decision values")
         if len(self.classes) == 2:
             return self.classes[(d >= 0).astype(int)]
         votes = np.zeros((d.shape[0], len(self.classes)), dtype=int)

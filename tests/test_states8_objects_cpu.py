@@ -165,3 +165,11 @@ def test_a_decision_of_exactly_zero_goes_where_sklearn_sends_it():
     d = three.decision_function(rows)
     assert (d == 0).all()
     assert np.array_equal(served([0, 1, 2], d).predict(rows), three.predict(rows))
+
+
+def test_a_sample_without_an_answer_gets_no_label():
+    """sklearn refuses a kernel row with NaN; the votes would name a class for it."""
+    for classes, d in (([0, 1], [0.5, np.nan]), ([0, 1, 2], [[1, 1, 1], [np.nan, 1, -1]])):
+        with pytest.raises(ValueError, match="NaN"):
+            served(classes, d).predict(np.zeros((2, 1)))
+    assert list(served([4, 9], [np.inf, -np.inf]).predict(np.zeros((2, 1)))) == [9, 4]
