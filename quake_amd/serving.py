@@ -56,12 +56,12 @@ class ServedSVC:
 
         from . import device as qdev
         self._torch, self._qdev = torch, qdev
-        self.device = torch.device("cuda" if device is None else device)
         self.classes = np.asarray(svc.classes_)
         self._n_features = x.shape[1]
         self._circuit = qdev.DeviceCircuit(kernel._bound)
         self._rows = max(1, PSI_BYTES // (16 * self._circuit.dim))
-        self.store = qdev.States8(coef.shape[0], self._circuit.dim, device=self.device)
+        self.store = qdev.States8(coef.shape[0], self._circuit.dim, device=device)
+        self.device = self.store.device      # with its index: another GPU may be the current one when the model is asked
         self._coef = torch.as_tensor(coef, dtype=torch.float32).to(self.device).contiguous()
         self._intercept = torch.as_tensor(intercept, dtype=torch.float32).to(self.device)
         self._fill(self.store, torch.as_tensor(x[svc.support_]).to(self.device))
@@ -72,8 +72,10 @@ class ServedSVC:
                 store.write(self._circuit.simulate(x[a:a + self._rows]))
 
     def decide(self, x):
-        """Decision values of device rows: float64 [M, features] tensor -> float32 [M, pairs] tensor, enqueued on the
-        current stream."""
+        """Decision values of device rows: float64 [M, features] tensor on the model's GPU -> float32 [M, pairs] tensor, enqueued
+        on that GPU's current stream."""
+        if x.device != self.device:
+            raise ValueError(f"x is on {x.device}, the model on {self.device}")
         queries = self._qdev.States8(x.shape[0], self._circuit.dim, device=self.device)
         self._fill(queries, x)
         return self._qdev.decision8(queries, self.store, self._coef, self._intercept)

@@ -173,3 +173,52 @@ def test_a_sample_without_an_answer_gets_no_label():
         with pytest.raises(ValueError, match="NaN"):
             served(classes, d).predict(np.zeros((2, 1)))
     assert list(served([4, 9], [np.inf, -np.inf]).predict(np.zeros((2, 1)))) == [9, 4]
+
+
+@pytest.fixture
+def model(monkeypatch):
+    """A served model whose store says that it lies on GPU 2, while another is current; nothing runs."""
+    from sklearn.svm import SVC
+    from quake_amd import circuit as qc, featuremaps as fm
+    from quake_amd.kernels import HipFidelityKernel
+    from quake_amd.serving import ServedSVC
+    entered, synced = [], []
+
+    class Store:
+        def __init__(self, capacity, dim, device=None):
+            wanted = torch.device("cuda" if device is None else device)
+            self.device = torch.device("cuda", 2 if wanted.index is None else wanted.index)
+
+        def write(self, psi):
+            synced.clear()                             # work that nobody has waited for
+
+    class Stream:
+        def __init__(self, device):
+            self.device = device
+
+        def synchronize(self):
+            synced.append(self.device)
+
+    monkeypatch.setattr(qdev, "States8", Store)
+    monkeypatch.setattr(qdev, "decision8", lambda x, y, coef, b: torch.zeros(1, 1))
+    monkeypatch.setattr(qdev.DeviceCircuit, "simulate", lambda self, x: x)
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, *a: self)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: entered.append(d) or contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: Stream(d))
+    k = HipFidelityKernel(fm.zz_featuremap(qc.ParameterVector("x", 3), 3, 1))
+    X = np.random.default_rng(0).uniform(size=(20, 3))
+    m = ServedSVC(k, SVC(kernel="precomputed").fit(X @ X.T, np.arange(20) % 2), X)
+    m.entered, m.synced = entered, synced
+    return m
+
+
+def test_a_served_model_stays_on_its_gpu(model):
+    here = torch.device("cuda", 2)
+    assert model.device == here and all(d == here for d in model.entered) and model.entered
+
+
+def test_samples_on_another_device_are_refused(model):
+    del model.entered[:]
+    with pytest.raises(ValueError, match="cuda:2"):
+        model.decide(torch.zeros((1, 3), dtype=torch.float64))
+    assert not model.entered
