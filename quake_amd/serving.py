@@ -65,6 +65,7 @@ class ServedSVC:
         self._coef = torch.as_tensor(coef, dtype=torch.float32).to(self.device).contiguous()
         self._intercept = torch.as_tensor(intercept, dtype=torch.float32).to(self.device)
         self._fill(self.store, torch.as_tensor(x[svc.support_]).to(self.device))
+        torch.cuda.current_stream(self.device).synchronize()      # whoever asks may do so on another stream
 
     def _fill(self, store, x) -> None:
         with self._torch.cuda.device(self.device):

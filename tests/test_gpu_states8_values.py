@@ -84,3 +84,31 @@ def test_a_copy_has_memory_of_its_own(again):
     K, t32, _ = S8.kernel(a[::-1], ga[::-1], a[::-1], ga[::-1])
     np.fill_diagonal(K, 1.0)
     assert (np.abs(qdev.gram8(t).cpu().numpy() - K) <= t32 + S8.U32 * K).all()
+
+
+# ---- served models ----------------------------------------------------------------------------------------------------------
+def test_served_svc_answers_at_once_on_another_stream():
+    """A model whose simulation takes a while, asked on a side stream as soon as it is there."""
+    from sklearn.svm import SVC
+    from quake_amd import featuremaps as fm
+    from quake_amd.circuit import ParameterVector
+    from quake_amd.kernels import HipFidelityKernel
+    from quake_amd.serving import ServedSVC
+    rng = np.random.default_rng(2)
+    n, N = 4, 60
+    X, Q = rng.uniform(-1.5, 1.5, size=(N, n)), rng.uniform(-1.5, 1.5, size=(7, n))
+    kernel = HipFidelityKernel(fm.zz_featuremap(ParameterVector("x", n), n, 1), precision="fp8")
+    svc = SVC(kernel="precomputed").fit(kernel.evaluate(X), (X[:, 0] > 0).astype(int))
+    want = ServedSVC(kernel, svc, X).decision_function(Q)
+    q = torch.from_numpy(Q).cuda()
+    slow, plain = qdev.DeviceCircuit.simulate, torch.cuda._sleep
+    try:
+        qdev.DeviceCircuit.simulate = lambda self, x, **k: (plain(100_000_000), slow(self, x, **k))[1]
+        served = ServedSVC(kernel, svc, X)
+    finally:
+        qdev.DeviceCircuit.simulate = slow
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = served.decide(q)
+    side.synchronize()
+    assert np.array_equal(got.cpu().numpy()[:, 0], want)

@@ -222,3 +222,8 @@ def test_samples_on_another_device_are_refused(model):
     with pytest.raises(ValueError, match="cuda:2"):
         model.decide(torch.zeros((1, 3), dtype=torch.float64))
     assert not model.entered
+
+
+def test_a_served_model_is_finished_when_it_is_there(model):
+    """It may be asked on any stream at once: its constructor has waited for the store's writes."""
+    assert model.synced == [torch.device("cuda", 2)]
