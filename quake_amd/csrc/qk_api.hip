@@ -24,7 +24,7 @@ int fail(int code, const std::string& msg) {
 }
 
 namespace {
-// Where the wall time of the calling thread's last qk_evaluate / qk_evaluate_f32 went (seconds; development hook
+// Where the wall time of the calling thread's last qk_evaluate / qk_evaluate_f32 / qk_evaluate8 went (seconds; development hook
 // qk_evaluate_profile, used by bench.py to itemise the PCIe-inclusive call of SURVEY.md 8d):
 //   [0] device allocations   [1] host-to-device copies of X / Y   [2] enqueueing the simulations and Gram bands
 //   [3] waiting for the bands while copying the finished ones to the host (the device work, with all copies but
@@ -490,10 +490,12 @@ int simulate8(const qk_circuit* c, const double* x_dev, int64_t rows, int64_t D,
     const int F = c->n_params;
     for (int64_t r = 0; r < rows; r += psi_rows) {
         const int64_t n = std::min(psi_rows, rows - r);
+        const double t0 = now_s();
         int rc = qk_simulate_dev(c, x_dev ? x_dev + r * F : nullptr, n, F, psi.p, nullptr);
         if (rc) return rc;
         const qk_states8 part = to.at(r, n);
         if ((rc = qk_states8_write_dev(psi.p, 0, D, D, &part, nullptr))) return rc;
+        g_profile.t[2] += now_s() - t0;
     }
     return QK_OK;
 }
@@ -529,40 +531,46 @@ extern "C" int qk_evaluate8(const qk_circuit* c, const double* X, int64_t N, con
     if (N == 0 || M == 0) return QK_OK;
     int rc = check_device();
     if (rc) return rc;
+    g_profile = EvalProfile();
+    const double t_begin = now_s();
     const int64_t D = (int64_t)1 << c->n_qubits;
     const int64_t psi_rows = std::max<int64_t>(1, std::min<int64_t>(std::max(N, M), (int64_t)(kPsi8Bytes / ((size_t)D * 16))));
     NoiseSpec noise;
     noise.mode = mode; noise.param = param; noise.seed = seed;
-    DevBuf dX, dY, psi, ws;
-    Store8 sx, sy;
-    if ((rc = upload_X(X, N, c->n_params, dX))) return rc;
-    QK_HIP(psi.alloc((size_t)psi_rows * D * 16));
-    if ((rc = sx.alloc(N, D))) return rc;
-    if ((rc = simulate8(c, (const double*)dX.p, N, D, psi, psi_rows, sx))) return rc;
-    if (!sym) {
-        if ((rc = upload_X(Y, M, c->n_params, dY))) return rc;
-        if ((rc = sy.alloc(M, D))) return rc;
-        if ((rc = simulate8(c, (const double*)dY.p, M, D, psi, psi_rows, sy))) return rc;
+    {
+        DevBuf dX, dY, psi, ws;
+        Store8 sx, sy;
+        if ((rc = upload_X(X, N, c->n_params, dX))) return rc;
+        QK_HIP(psi.alloc((size_t)psi_rows * D * 16));
+        if ((rc = sx.alloc(N, D))) return rc;
+        if ((rc = simulate8(c, (const double*)dX.p, N, D, psi, psi_rows, sx))) return rc;
+        if (!sym) {
+            if ((rc = upload_X(Y, M, c->n_params, dY))) return rc;
+            if ((rc = sy.alloc(M, D))) return rc;
+            if ((rc = simulate8(c, (const double*)dY.p, M, D, psi, psi_rows, sy))) return rc;
+        }
+        const Store8& cols = sym ? sx : sy;
+        size_t have = 0;
+        auto launch = [&](const GramBlock* blocks, int n, hipStream_t stream) {
+            qk_gram8_job jobs[2];
+            for (int k = 0; k < n; ++k) {
+                const GramBlock& g = blocks[k];
+                jobs[k] = gram8_job(sx.at(g.r0, g.r1 - g.r0), cols.at(g.c0, g.c1 - g.c0), D, g.sym, g.K, g.ldk, g.KT, g.ldkt);
+            }
+            size_t need = 0;
+            int r = qk_gram8_workspace(jobs, n, &need);
+            if (r) return r;
+            if (need > have) {      // (releasing the smaller one waits for the launches that use it)
+                ws.release();
+                QK_HIP(ws.alloc(need));
+                have = need;
+            }
+            return qk_gram8_jobs_dev(jobs, n, ws.p, have, stream);
+        };
+        rc = gram_to_host(launch, N, M, sym, D, K_host, noise);
     }
-    const Store8& cols = sym ? sx : sy;
-    size_t have = 0;
-    auto launch = [&](const GramBlock* blocks, int n, hipStream_t stream) {
-        qk_gram8_job jobs[2];
-        for (int k = 0; k < n; ++k) {
-            const GramBlock& g = blocks[k];
-            jobs[k] = gram8_job(sx.at(g.r0, g.r1 - g.r0), cols.at(g.c0, g.c1 - g.c0), D, g.sym, g.K, g.ldk, g.KT, g.ldkt);
-        }
-        size_t need = 0;
-        int r = qk_gram8_workspace(jobs, n, &need);
-        if (r) return r;
-        if (need > have) {      // (releasing the smaller one waits for the launches that use it)
-            ws.release();
-            QK_HIP(ws.alloc(need));
-            have = need;
-        }
-        return qk_gram8_jobs_dev(jobs, n, ws.p, have, stream);
-    };
-    return gram_to_host(launch, N, M, sym, D, K_host, noise);
+    g_profile.t[6] = now_s() - t_begin;
+    return rc;
 }
 
 extern "C" int qk_evaluate(const qk_circuit* c, const double* X, int64_t N, const double* Y, int64_t M,
@@ -580,7 +588,7 @@ extern "C" int qk_evaluate_noisy(const qk_circuit* c, const double* X, int64_t N
 }
 
 // Development hook (not in the public header): the itemised wall time of the calling thread's last qk_evaluate /
-// qk_evaluate_f32, see EvalProfile.
+// qk_evaluate_f32 / qk_evaluate8, see EvalProfile.
 extern "C" int qk_evaluate_profile(double* out, int len) {
     if (!out || len < 1) return QK_ERR_INVALID;
     for (int k = 0; k < len && k < 8; ++k) out[k] = g_profile.t[k];

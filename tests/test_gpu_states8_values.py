@@ -112,3 +112,27 @@ def test_served_svc_answers_at_once_on_another_stream():
         got = served.decide(q)
     side.synchronize()
     assert np.array_equal(got.cpu().numpy()[:, 0], want)
+
+
+# ---- the host path's own account ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("N", [40, 3000])
+def test_profile_of_the_last_call_is_the_fp8_one(N):
+    """The itemised time of a call starts from zero and ends with the call's own total."""
+    import time
+    from quake_amd import featuremaps as fm
+    from quake_amd.circuit import ParameterVector
+    from quake_amd.kernels import HipFidelityKernel
+    fn = _lib.load().qk_evaluate_profile
+    fn.restype, fn.argtypes = C.c_int, [C.POINTER(C.c_double), C.c_int]
+    t = (C.c_double * 8)()
+    circ = fm.zz_featuremap(ParameterVector("x", 4), 4, 1)
+    X = np.random.default_rng(1).uniform(-1, 1, size=(N, 4))
+    HipFidelityKernel(circ).evaluate(np.random.default_rng(2).uniform(-1, 1, size=(6000, 4)))       # a longer call before
+    kernel = HipFidelityKernel(circ, precision="fp8")
+    for _ in range(3):
+        begin = time.perf_counter()
+        kernel.evaluate(X)
+        wall = time.perf_counter() - begin
+        assert fn(t, 8) == 0
+        total, parts = t[6], sum(t[:6])
+        assert 0 < parts <= total * (1 + 1e-9) and total <= wall and t[0] > 0 and t[2] > 0
