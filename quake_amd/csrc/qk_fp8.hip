@@ -131,7 +131,7 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void states8_write_kernel
             if (b0 + 2 * WPR < sb) load(b + 2 * WPR);
             const int e = scale_exponent(half_max(top));
             uint32_t wr = 0, wi = 0;      // byte k: the code of amplitude 32 k + i
-            float sq = 0.f;
+            double sq = 0.0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float a = ldexpf(re[k], -e), c = ldexpf(im[k], -e);
@@ -139,10 +139,10 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void states8_write_kernel
                 p &= ~(((p & 0x7f7fu) + 0x0101u) & 0x8080u);      // one code for NaN: 0x7f
                 wr |= (p & 0xffu) << (8 * k);
                 wi |= ((p >> 8) & 0xffu) << (8 * k);
-                const float qa = __builtin_amdgcn_cvt_f32_fp8((int)p, 0), qc = __builtin_amdgcn_cvt_f32_fp8((int)p, 1);
+                const double qa = __builtin_amdgcn_cvt_f32_fp8((int)p, 0), qc = __builtin_amdgcn_cvt_f32_fp8((int)p, 1);
                 sq += qa * qa + qc * qc;
             }
-            kept += ldexp((double)sq, 2 * e);
+            kept += ldexp(sq, 2 * e);
             wr = quad_transpose(wr, lane);
             wi = quad_transpose(wi, lane);
             const int64_t at = b * kBlock + 32 * (i & 3) + (i & ~3);      // four amplitudes from here on

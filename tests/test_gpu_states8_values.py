@@ -136,3 +136,23 @@ def test_profile_of_the_last_call_is_the_fp8_one(N):
         assert fn(t, 8) == 0
         total, parts = t[6], sum(t[:6])
         assert 0 < parts <= total * (1 + 1e-9) and total <= wall and t[0] > 0 and t[2] > 0
+
+
+# ---- gains --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("single", [False, True])
+def test_gains_are_rounded_once(single):
+    """Sums of squares in FP64: what is left is the quotient's rounding to float32 (and FP64's, 300 times 2^-53 at most).  Four
+    amplitudes of one lane, one of them large and the others in the lower half of the format."""
+    rng = np.random.default_rng(6)
+    psi = np.zeros((2000, 128), dtype=np.complex128)
+    for k, at in enumerate((9, 41, 73, 105)):
+        scale = 1.0 if k == 0 else 2.0 ** -10
+        psi[:, at] = scale * (rng.uniform(0.3, 1, 2000) + 1j * rng.uniform(0.3, 1, 2000))
+    psi[:1000] = S8.states(rng, 1000, 128)
+    if single:
+        psi = psi.astype(np.complex64).astype(np.complex128)
+    store = qdev.States8(2000, 128)
+    store.write(put(psi, single))
+    gains = S8.write(psi)[2]
+    off = np.abs(store.gains.cpu().numpy() - gains) / gains
+    assert (off <= S8.U32 * (1 + 1e-6) + 300 * 2.0 ** -53).all(), ((off > S8.U32 * (1 + 1e-6)).sum(), off.max() / S8.U32)
