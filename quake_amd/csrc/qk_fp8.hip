@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <new>
 #include <vector>
 
 #include "qk_common.h"
@@ -1633,6 +1634,15 @@ qk_gram8_job decision8_job(const qk_states8& x, const qk_states8& y, int64_t D, 
     j.ldk = y.rows;
     return j;
 }
+// An entry point that plans on the heap: no exception leaves the library.
+template <typename F> int no_throw(const char* who, F body) {
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        return fail(QK_ERR_INVALID, std::string(who) + ": out of memory on the host");
+    }
+}
+
 size_t decision8_k_bytes(int64_t M, int64_t N) { return (size_t)((M * N * (int64_t)sizeof(float) + 255) & ~(int64_t)255); }
 }  // namespace
 }  // namespace qk
@@ -1717,7 +1727,8 @@ extern "C" int qk_states8_read_dev(const qk_states8* from, int64_t D, const int6
     return QK_OK;
 }
 
-extern "C" int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* bytes) {
+namespace {
+int gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* bytes) {
     if (!bytes) return fail(QK_ERR_INVALID, "qk_gram8_workspace: null pointer");
     *bytes = 0;
     const int rc = check_gram8(jobs, n_jobs);
@@ -1726,6 +1737,10 @@ extern "C" int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* 
         *bytes = std::max(*bytes, p.ws_floats * sizeof(float));      // the launches of a call use it one after the other
         return QK_OK;
     });
+}
+}  // namespace
+extern "C" int qk_gram8_workspace(const qk_gram8_job* jobs, int n_jobs, size_t* bytes) {
+    return no_throw("qk_gram8_workspace", [&] { return gram8_workspace(jobs, n_jobs, bytes); });
 }
 
 // A launch with more LDS than a kernel may have unasked
@@ -1752,7 +1767,8 @@ template <typename K, typename A> int launch8(K kernel, dim3 grid, int lds, hipS
         if (rc8) return rc8;                                                                                         \
     } while (0)
 
-extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream) {
+namespace {
+int gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream) {
     int rc = check_gram8(jobs, n_jobs);
     if (rc) return rc;
     if ((uintptr_t)ws & 15) return fail(QK_ERR_INVALID, "qk_gram8_jobs_dev: the workspace needs 16-byte alignment");
@@ -1792,6 +1808,10 @@ extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws,
         return (int)QK_OK;
     });
 }
+}  // namespace
+extern "C" int qk_gram8_jobs_dev(const qk_gram8_job* jobs, int n_jobs, void* ws, size_t ws_bytes, void* stream) {
+    return no_throw("qk_gram8_jobs_dev", [&] { return gram8_jobs_dev(jobs, n_jobs, ws, ws_bytes, stream); });
+}
 
 // Development hook (not in the public header): which kernel the products of 8-bit stores use, whatever the rule says.
 extern "C" int qk_gram8_set_path(const char* name) {
@@ -1804,7 +1824,8 @@ extern "C" int qk_gram8_set_path(const char* name) {
     return QK_OK;
 }
 
-extern "C" int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, size_t* bytes) {
+namespace {
+int decision8_workspace(int64_t M, int64_t N, int64_t D, int C, size_t* bytes) {
     const char* who = "qk_decision8_workspace";
     if (!bytes) return fail(QK_ERR_INVALID, std::string(who) + ": null pointer");
     *bytes = 0;
@@ -1830,14 +1851,14 @@ extern "C" int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, si
     return QK_OK;
 }
 
-extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_t D, const float* coef, int64_t ldc, int C,
-                                const float* intercept, float* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
+int decision8_dev(const qk_states8* x, const qk_states8* y, int64_t D, const float* coef, int64_t ldc, int C, const float* intercept,
+                  float* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
     const char* who = "qk_decision8_dev";
     if (!x || !y) return fail(QK_ERR_INVALID, std::string(who) + ": null pointer");
     int rc;
     if ((rc = check_dim(who, D)) || (rc = check_states(who, *x)) || (rc = check_states(who, *y))) return rc;
     size_t need = 0;
-    if ((rc = qk_decision8_workspace(x->rows, y->rows, D, C, &need))) return rc;
+    if ((rc = decision8_workspace(x->rows, y->rows, D, C, &need))) return rc;
     if (x->rows == 0) return QK_OK;
     if (!out || (y->rows && !coef)) return fail(QK_ERR_INVALID, std::string(who) + ": null pointer");
     if (ldc < C || ldo < C) return fail(QK_ERR_INVALID, std::string(who) + ": row stride smaller than C");
@@ -1865,7 +1886,7 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
     if (decision8_by_rows(x->rows, y->rows, D)) {
         const size_t k = decision8_k_bytes(x->rows, y->rows);
         const qk_gram8_job job = decision8_job(*x, *y, D, ws);
-        if ((rc = qk_gram8_jobs_dev(&job, 1, (char*)ws + k, ws_bytes - k, stream))) return rc;
+        if ((rc = gram8_jobs_dev(&job, 1, (char*)ws + k, ws_bytes - k, stream))) return rc;
         hipLaunchKernelGGL(decision8_rows_kernel, dim3((unsigned)x->rows, (unsigned)C), dim3(256), 0, s, a);
         QK_HIP(hipGetLastError());
         return QK_OK;
@@ -1894,4 +1915,14 @@ extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_
         QK_HIP(hipGetLastError());
     }
     return QK_OK;
+}
+}  // namespace
+
+extern "C" int qk_decision8_workspace(int64_t M, int64_t N, int64_t D, int C, size_t* bytes) {
+    return no_throw("qk_decision8_workspace", [&] { return decision8_workspace(M, N, D, C, bytes); });
+}
+
+extern "C" int qk_decision8_dev(const qk_states8* x, const qk_states8* y, int64_t D, const float* coef, int64_t ldc, int C,
+                                const float* intercept, float* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
+    return no_throw("qk_decision8_dev", [&] { return decision8_dev(x, y, D, coef, ldc, C, intercept, out, ldo, ws, ws_bytes, stream); });
 }

@@ -227,3 +227,25 @@ def test_samples_on_another_device_are_refused(model):
 def test_a_served_model_is_finished_when_it_is_there(model):
     """It may be asked on any stream at once: its constructor has waited for the store's writes."""
     assert model.synced == [torch.device("cuda", 2)]
+
+
+# ---- the C entry points ------------------------------------------------------------------------------------------------------
+def test_no_memory_on_the_host_is_an_error_code():
+    """A call of two million jobs in a process that may not grow: an error, no exception across the C boundary."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    child = """
+import ctypes as C, resource
+from quake_amd import _lib
+lib, n = _lib.load(), 1 << 21
+job = _lib.GRAM8_JOB.pack(1 << 20, 1 << 21, 1 << 22, 1, 1 << 20, 1 << 21, 1 << 22, 1, 64, 1 << 23, 0, 1, 0, 0, 0)
+jobs, need = C.create_string_buffer(job * n, len(job) * n), C.c_size_t()
+assert lib.qk_gram8_workspace(jobs, 100, C.byref(need)) == 0
+size = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (size + (1 << 20), resource.RLIM_INFINITY))
+print(lib.qk_gram8_workspace(jobs, n, C.byref(need)), lib.qk_gram8_jobs_dev(jobs, n, None, 0, None), _lib.last_error())
+"""
+    done = subprocess.run([sys.executable, "-c", child], capture_output=True, text=True, cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0, done.stderr[-500:]
+    assert done.stdout.split()[:2] == [str(_lib.QK_ERR_INVALID)] * 2 and "out of memory" in done.stdout
