@@ -220,20 +220,17 @@ def _same_gpu(gpu: int, *tensors) -> None:
             raise ValueError("device entry points need tensors in GPU memory, all on one GPU")
 
 
-def _in_memory(*tensors) -> None:
-    """The library reads and writes memory: a lazily negated or conjugated view holds other values there than it shows."""
+def _plain(*tensors) -> None:
+    """The library reads and writes memory: a lazily negated or conjugated view holds other values there than it shows.  And
+    nothing is recorded for autograd: an output without a graph would drop a gradient without a word."""
     for t in tensors:
-        if t is not None and (t.is_neg() or t.is_conj()):
+        if t is None:
+            continue
+        if t.is_neg() or t.is_conj():
             raise ValueError("lazily negated or conjugated tensors are not taken: call resolve_neg() / resolve_conj() first")
-
-
-def _no_graph(*tensors) -> None:
-    """Nothing here is recorded for autograd: an output without a graph would drop a gradient without a word."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("no gradient is recorded through 8-bit stores: detach() the tensor or call under torch.no_grad() "
-                                 "(the gradient of decision8 by coef is decision8(y, x, dloss/dout))")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("no gradient is recorded through 8-bit stores: detach() the tensor or call under torch.no_grad() "
+                             "(the gradient of decision8 by coef is decision8(y, x, dloss/dout))")
 
 
 class States8:
@@ -287,8 +284,7 @@ class States8:
                 or not (codes.is_contiguous() and scales.is_contiguous() and gains.is_contiguous()):
             raise ValueError("need contiguous codes uint8 [rows, 128 ceil(dim / 64)], scales uint8 [rows, 4 ceil(dim / 512)], "
                              "gains float32 [rows]")
-        _in_memory(codes, scales, gains)
-        _no_graph(gains)
+        _plain(gains)
         store = cls.__new__(cls)
         store._set(codes, scales, gains, dim, rows)
         return store
@@ -330,8 +326,7 @@ class States8:
         if psi.dtype not in (torch.complex128, torch.complex64) or psi.dim() != 2 or psi.shape[1] != self.dim \
                 or (psi.shape[0] and self.dim > 1 and psi.stride(1) != 1):
             raise ValueError("psi must be a complex128 / complex64 [rows, dim] tensor with unit column stride")
-        _in_memory(psi)
-        _no_graph(psi)
+        _plain(psi)
         n, at = psi.shape[0], self._rows if at is None else at
         if not 0 <= at <= self._rows:
             raise ValueError(f"at = {at}: the store holds {self._rows} rows")
@@ -351,8 +346,7 @@ class States8:
         ``index`` (int64 on the GPU, any order, repeats allowed; a number outside the store gives a row of NaN)."""
         index, out = from_dlpack(index), from_dlpack(out)
         _same_gpu(self._gpu, index, out)
-        _in_memory(index, out)
-        _no_graph(index, out)
+        _plain(index, out)
         if index is not None and (index.dtype != torch.int64 or index.dim() != 1 or not index.is_contiguous()):
             raise ValueError("index must be a contiguous int64 vector")
         n = self._rows if index is None else index.shape[0]
@@ -419,8 +413,7 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
             if K.dtype not in _K8_FLAGS or K.shape != (m, n) or (K.numel() and ((n > 1 and K.stride(1) != 1) or (m > 1 and K.stride(0) < n))):
                 raise ValueError("K must be float32, float16 or float64 [len(A), len(B)] with unit column stride")
             _same_gpu(gpu, K)
-            _in_memory(K)
-            _no_graph(K)
+            _plain(K)
             ldk = K.stride(0) if m > 1 and n else max(n, 1)
         kt = ldkt = 0
         if KT is not None:
@@ -429,10 +422,10 @@ def gram8_jobs(jobs: Sequence[dict], dtype=torch.float32) -> List[torch.Tensor]:
                     or (KT.numel() and ((m > 1 and KT.stride(1) != 1) or (n > 1 and KT.stride(0) < m))):
                 raise ValueError("KT must be of K's type, [len(B), len(A)] with unit column stride, and not for a symmetric job")
             _same_gpu(gpu, KT)
-            _in_memory(KT)
-            _no_graph(KT)
+            _plain(KT)
             kt, ldkt = KT.data_ptr(), (KT.stride(0) if n > 1 and m else max(m, 1))
-        packed.append(_lib.GRAM8_JOB.pack(*A._at, m, *B._at, n, A.dim, K.data_ptr(), kt, ldk, ldkt,
+        at = A._at
+        packed.append(_lib.GRAM8_JOB.pack(*at, m, *(at if sym else B._at), n, A.dim, K.data_ptr(), kt, ldk, ldkt,
                                           _K8_FLAGS[K.dtype] | (_lib.QK_GRAM_SYMMETRIC if sym else 0), 0))
         Ks.append(K)
     lib, arr = _lib.load(), b"".join(packed)
@@ -461,8 +454,7 @@ def decision8(x: States8, y: States8, coef: torch.Tensor, intercept: Optional[to
     if not isinstance(x, States8) or not isinstance(y, States8):
         raise ValueError("x and y must be States8 stores")
     _same_gpu(x._gpu, y.codes, coef, intercept, out)
-    _in_memory(coef, intercept, out)
-    _no_graph(coef, intercept, out)
+    _plain(coef, intercept, out)
     if x.dim != y.dim:
         raise ValueError(f"stores of different dim: {x.dim} and {y.dim}")
     if coef.dim() == 1:

@@ -156,3 +156,21 @@ def test_gains_are_rounded_once(single):
     gains = S8.write(psi)[2]
     off = np.abs(store.gains.cpu().numpy() - gains) / gains
     assert (off <= S8.U32 * (1 + 1e-6) + 300 * 2.0 ** -53).all(), ((off > S8.U32 * (1 + 1e-6)).sum(), off.max() / S8.U32)
+
+
+# ---- rows that are not finite -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("N,D", [(1, 4), (3, 100), (40, 300), (200, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.float64])
+def test_diagonal_of_a_symmetric_kernel_is_one_for_every_row(N, D, dtype, path):
+    """As of every symmetric job: also for a row of zeros and for one with a NaN, whose other entries are 0 and NaN."""
+    psi = S8.states(np.random.default_rng(N), N, D)
+    psi[0, 0] = np.nan
+    if N > 2:
+        psi[2] = 0
+    x, _, _ = fill(psi)
+    K = qdev.gram8(x, dtype=dtype).cpu().numpy()
+    assert (np.diag(K) == 1).all() and np.isnan(K[0, 1:]).all() and np.isnan(K[1:, 0]).all()
+    if N > 2:
+        assert (np.delete(K[2], [0, 2]) == 0).all()
+    cross = qdev.gram8(x, x.rows(0, N), dtype=dtype).cpu().numpy()
+    assert np.isnan(cross[0]).all()
