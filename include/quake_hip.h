@@ -210,7 +210,8 @@ int qk_states8_read_dev(const qk_states8* from, int64_t D, const int64_t* index,
  * to the norms of the states they stand for (unit norm: K_ii = 1, K is a valid kernel, positive semidefinite).
  * Jobs are those of qk_gram_jobs_dev (KT not with QK_GRAM_SYMMETRIC), each with its own D: the kernels of a population of circuits of any sizes run together.
  * K (and KT) are float32, or float16 / float64 by flag.  QK_GRAM_SYMMETRIC: the same store on both sides, only tiles on or
- * above the diagonal are computed, the mirror is written and the diagonal is exactly 1.
+ * above the diagonal are computed, the mirror is written and the diagonal is exactly 1 (for a row of zeros and for one whose
+ * gain is NaN as well).
  * Sums are FP32 for every type of K, which is converted once.  ws: device memory of qk_gram8_workspace bytes (0 for most
  * calls), 16-byte aligned, used until the call's work is done.  Results do not depend on the launch: no atomics, fixed order of summation.
  */
@@ -374,7 +375,7 @@ int qk_evaluate_noisy(const qk_circuit* c, const double* X, int64_t N, const dou
 #define QK_BATCH_FP8 1
 typedef struct qk_batch_opts {
     int32_t noise_mode;     /* QK_NOISE_* */
-    int32_t flags;          /* 0, or QK_BATCH_FP8: the kernels over 8-bit stores (qk_gram8_jobs_dev, all genomes in one call) */
+    int32_t flags;          /* 0, or QK_BATCH_FP8 (anything else is refused): the kernels over 8-bit stores (qk_gram8_jobs_dev, all genomes in one call) */
     double noise_param;
     uint64_t seed;
 } qk_batch_opts;

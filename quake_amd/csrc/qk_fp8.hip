@@ -1620,7 +1620,9 @@ bool plan_decision8(int64_t M, int64_t N, int64_t D, int C, Decision8Args& a) {
 
 // A few rows against few long ones: the 32-row tiles would be less than one for every other CU, each with a long way to go, so K
 // goes through memory, its rows cut by gram8's rule.  (Tiles / this, us: one row against 1000 of 9000 amplitudes 25 / 14, of 65536 132 / 32;
-// 32 rows against 1000 of 65536 154 / 36; one against 4000 of 9000 25.4 / 25.5, 8000 of 9000 29 / 37.)
+// 32 rows against 1000 of 65536 154 / 36; one against 4000 of 9000 25.4 / 25.5, 8000 of 9000 29 / 37.)  Its ends hold for the rows they
+// were measured on: behind them the tiles walk whole rows of 65536 amplitudes too -- 33 rows against 1000 take 156 us (gram8 68), one
+// against 4097 174 (gram8 128), 128 against 12288 1.59 ms (gram8 0.70).
 bool decision8_by_rows(int64_t M, int64_t N, int64_t D) {
     return g_path.load(std::memory_order_relaxed) == 0 && M <= 32 && D > 64 * kChunk && N <= 4096;
 }
