@@ -1092,7 +1092,7 @@ struct Decision8Args {
 // coefficients is then a sum over the lane's own registers, and only the two halves of the wave have to be added.  32 rows of A
 // (8 with AR = 8) per workgroup against a range of B's.  SPLIT (rows of 8 chunks or more): the four waves share every tile of 32 of
 // B's rows, each multiplies a quarter of the chunks and then finishes a quarter of the tile's rows; else every wave has a tile of
-// its own (one row against 8192 of 512 amplitudes 8 us shared, 15 each on its own; of 256 the same).  One row against 8192 of 1024 amplitudes (17 MB, 3 us to read): 7.0 us, joining the parts 2.6, 16.5 from call to call.
+// its own (one row against 8192 of 512 amplitudes 8 us shared, 15 each on its own; of 256 the same).  One row against 8192 of 1024 amplitudes (17 MB, 3 us to read): 7.0 us, joining the parts 2.9, 18 from call to call.
 template <int AR, bool SPLIT> __global__ __launch_bounds__(256) void decision8_thin_kernel(Decision8Args a) {
     constexpr int W = 4, R = SPLIT ? 16 / W : 16, S = 3;      // R: accumulator registers that a wave finishes
     extern __shared__ uint8_t lds[];

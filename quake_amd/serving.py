@@ -75,6 +75,7 @@ class ServedSVC:
     def decide(self, x):
         """Decision values of device rows: float64 [M, features] tensor on the model's GPU -> float32 [M, pairs] tensor, enqueued
         on that GPU's current stream."""
+        x = self._qdev.from_dlpack(x)
         if x.device != self.device:
             raise ValueError(f"x is on {x.device}, the model on {self.device}")
         queries = self._qdev.States8(x.shape[0], self._circuit.dim, device=self.device)

@@ -221,6 +221,8 @@ def test_samples_on_another_device_are_refused(model):
     del model.entered[:]
     with pytest.raises(ValueError, match="cuda:2"):
         model.decide(torch.zeros((1, 3), dtype=torch.float64))
+    with pytest.raises(ValueError, match="cuda:2"):
+        model.decide(torch.utils.dlpack.to_dlpack(torch.zeros((1, 3), dtype=torch.float64)))      # by DLPack, like every device entry point
     assert not model.entered
 
 
